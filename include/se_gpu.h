@@ -277,6 +277,38 @@ int se_unique(int32_t key_dtype, const void *keys, size_t num_keys, void *unique
               uint64_t *num_unique_out, int32_t device, void *stream);
 
 /*
+ * Dense operators beside the store (no reference counterpart: its users run
+ * the dense part of a model outside it). Device pointers only, on `device`
+ * (others are refused); asynchronous on `stream`; nothing is allocated and the
+ * host waits for nothing, so the calls can be captured into CUDA graphs. A
+ * workspace belongs to the caller: one per call in flight.
+ */
+
+/* Layer normalisation of `rows` rows of dim values (value_dtype; row i starts
+ * x_stride values after row i - 1):
+ *   mean = sum x / dim, rstd = 1 / sqrt(sum (x - mean)^2 / dim + eps),
+ *   y = (x - mean) rstd weight + bias
+ * weight and bias hold dim values of param_dtype; null means 1 and 0. y is
+ * rows x dim without gaps; mean_out and rstd_out hold rows fp32 values, or
+ * null. Statistics in fp32, y rounded once. Outputs overlap no input. */
+int se_layer_norm(int32_t value_dtype, int32_t param_dtype, const void *x, size_t rows, int64_t dim,
+                  int64_t x_stride, const void *weight, const void *bias, float eps, void *y,
+                  float *mean_out, float *rstd_out, int32_t device, void *stream);
+/* Backward of se_layer_norm for the gradient of y (rows x dim, grad_stride):
+ * with h = (x - mean) rstd and q = grad weight,
+ *   dx = rstd (q - sum q / dim - h sum(q h) / dim)   (rows x dim without gaps)
+ *   dweight = sum over rows of grad h, dbias = sum over rows of grad
+ * dweight and dbias (dim values of param_dtype) may be null: not computed;
+ * with no rows they are zeros. Sums in fp32, in an order that depends on the
+ * sizes and the device only. With dweight or dbias the call needs a workspace
+ * of se_layer_norm_backward_workspace bytes. Outputs overlap no input. */
+int se_layer_norm_backward(int32_t value_dtype, int32_t param_dtype, const void *grad, int64_t grad_stride,
+                           const void *x, int64_t x_stride, size_t rows, int64_t dim, const float *mean,
+                           const float *rstd, const void *weight, void *dx, void *dweight, void *dbias,
+                           void *workspace, size_t workspace_bytes, int32_t device, void *stream);
+int se_layer_norm_backward_workspace(size_t rows, int64_t dim, int32_t device, size_t *bytes);
+
+/*
  * Exchange routing (no reference counterpart: the reference leaves routing to
  * the caller, sparse_embedding/partitioner.py:84-100). Device pointers only.
  * Partitions keys and groups them by destination, stably: send_keys holds the

@@ -29,6 +29,7 @@ from .partitioner import (
     register_partitioner,
 )
 from .unique import async_unique, unique
+from .dense import layer_norm, layer_norm_backward
 from .store import (
     Adagrad,
     Adam,
@@ -60,5 +61,6 @@ __all__ = [
     "Partitioner", "SPARSE_EMBEDDING_FAST_RANGE_ASSIGNMENT_NAME", "SPARSE_EMBEDDING_HASH_ASSIGNMENT_NAME",
     "SPARSE_EMBEDDING_MODULO_ASSIGNMENT_NAME", "SUPPORTED_KEY_DTYPES", "Sgd", "StorageTuningOptions",
     "Uniform", "Zeros", "create_partitioner", "create_strategy", "filter_partition",
-    "generate_reference_vectors", "is_partitioner_registered", "partition", "register_partitioner",
+    "generate_reference_vectors", "is_partitioner_registered", "layer_norm", "layer_norm_backward",
+    "partition", "register_partitioner",
 ]

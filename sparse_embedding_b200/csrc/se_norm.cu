@@ -1,0 +1,647 @@
+// Layer normalisation of rows (pooled bags, looked-up rows, hidden rows) and
+// its backward pass. It has no counterpart in the reference, whose users
+// normalise the rows outside the store.
+//
+// For a row x of D values with weight w and bias b:
+//   mean = sum x / D,  var = sum (x - mean)^2 / D,  r = 1 / sqrt(var + eps)
+//   y = (x - mean) r w + b
+// and for the gradient g of y, with h = (x - mean) r and q = g w:
+//   dx = r (q - sum q / D - h (sum q h) / D)
+//   dw = sum over rows of g h,   db = sum over rows of g
+//
+// Both passes are bound by HBM: the forward reads x and writes y, the
+// backward reads x and g and writes dx. Every row is therefore read once,
+// into registers, by `lanes` threads (a part of a warp, or a whole block for
+// long rows); the variance is taken from the registers around the mean, not
+// as a difference of two sums. All sums are fp32; y, dx, dw and db are rounded
+// once, to the type they are stored in. A block keeps its share of the
+// columns over all the rows it visits, so w and b are loaded once per thread
+// and the sums of dw and db stay in registers until the block's end; the
+// blocks' sums go to the caller's workspace and a second kernel adds them in
+// block order, so equal calls give equal bits.
+
+#include <algorithm>
+#include <type_traits>
+
+#include "se_common.cuh"
+#include "se_dense.hpp"
+
+namespace se_gpu {
+
+namespace {
+
+constexpr int kNormNarrowThreads = 256;  // block of the kernels with several rows per block
+// A block per row: its most threads and the loads of each. Rows of up to 8,192
+// values fit the registers in every layout (the backward holds three fp32
+// values per column besides the row).
+constexpr __host__ __device__ int norm_wide_threads(int vec) { return vec == 1 ? 1024 : 512; }
+constexpr __host__ __device__ int norm_wide_loads(int vec) { return vec == 1 ? 8 : 16 / vec; }
+
+// VEC values of a row: one 16-byte load where the layout allows it, else one value.
+template <class V, int VEC>
+struct Pack {
+  using T = typename V::T;
+  using Raw = std::conditional_t<VEC == 1, T, uint4>;
+  static_assert(VEC == 1 || VEC * sizeof(T) == 16, "a vector is 16 bytes");
+  static __device__ __forceinline__ Raw load(const T *p) {
+    if constexpr (VEC == 1) return *p;
+    else return *reinterpret_cast<const uint4 *>(p);
+  }
+  static __device__ __forceinline__ Raw zero() {
+    if constexpr (VEC == 1) return V::store(0.0f);
+    else return make_uint4(0u, 0u, 0u, 0u);
+  }
+  static __device__ __forceinline__ void open(const Raw &r, float (&f)[VEC]) {
+    if constexpr (VEC == 1) {
+      f[0] = V::load(r);
+    } else {
+      const T *v = reinterpret_cast<const T *>(&r);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) f[i] = V::load(v[i]);
+    }
+  }
+  static __device__ __forceinline__ void store(T *p, const float (&f)[VEC]) {
+    if constexpr (VEC == 1) {
+      *p = V::store(f[0]);
+    } else {
+      uint4 r;
+      T *v = reinterpret_cast<T *>(&r);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[i] = V::store(f[i]);
+      *reinterpret_cast<uint4 *>(p) = r;
+    }
+  }
+};
+
+// Value i of a weight or bias in its own type; `missing` where there is none.
+__device__ __forceinline__ float param_at(const void *p, int type, int64_t i, float missing) {
+  if (p == nullptr) return missing;
+  if (type == SE_FLOAT32) return static_cast<const float *>(p)[i];
+  if (type == SE_FLOAT16) return __half2float(static_cast<const __half *>(p)[i]);
+  return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
+}
+__device__ __forceinline__ void param_put(void *p, int type, int64_t i, float f) {
+  if (type == SE_FLOAT32) static_cast<float *>(p)[i] = f;
+  else if (type == SE_FLOAT16) static_cast<__half *>(p)[i] = __float2half_rn(f);
+  else static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(f);
+}
+
+// Sums of N values over the threads of a row: xor shuffles within the warp's
+// part, and for a whole block (WIDE) one exchange through shared memory.
+// Successive exchanges alternate between two buffers, so one barrier each is
+// enough: a buffer is written again only after the next exchange's barrier.
+template <int N, bool WIDE>
+struct RowSum {
+  int lanes;
+  float (*buf)[32][2];  // [2][32][2]
+  int phase = 0;
+  __device__ __forceinline__ void operator()(float (&v)[N]) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      if (o < lanes) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+      }
+    }
+    if constexpr (WIDE) {
+      static_assert(N <= 2, "two values per exchange");
+      const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+      if (lane == 0) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) buf[phase][warp][i] = v[i];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = lane < warps ? buf[phase][lane][i] : 0.0f;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+      }
+      phase ^= 1;
+    }
+  }
+};
+
+// Rows held in registers: `lanes` threads per row (a power of two up to 32, or
+// with WIDE the block), NV vectors of VEC values per thread, U rows at a time
+// (their loads are in flight together).
+template <class V, int VEC, int NV, int U, bool WIDE>
+__global__ void __launch_bounds__(WIDE ? norm_wide_threads(VEC) : kNormNarrowThreads)
+k_norm_forward(const typename V::T *__restrict__ x, int64_t x_stride, int64_t rows, int dim,
+               const void *__restrict__ weight, const void *__restrict__ bias, int ptype, float eps,
+               typename V::T *__restrict__ y, float *__restrict__ mean_out, float *__restrict__ rstd_out, int lanes) {
+  using P = Pack<V, VEC>;
+  __shared__ float red[2][32][2];
+  const int lane = WIDE ? int(threadIdx.x) : int(threadIdx.x) & (lanes - 1);
+  const int group = WIDE ? 0 : int(threadIdx.x) / lanes;
+  const int groups = WIDE ? 1 : int(blockDim.x) / lanes;
+  float w[NV][VEC], b[NV][VEC];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const int c = (v * lanes + lane) * VEC + i;
+      w[v][i] = c < dim ? param_at(weight, ptype, c, 1.0f) : 0.0f;
+      b[v][i] = c < dim ? param_at(bias, ptype, c, 0.0f) : 0.0f;
+    }
+  }
+  RowSum<U, WIDE> sum{lanes, red};
+  const float inv = 1.0f / float(dim);
+  for (int64_t base = int64_t(blockIdx.x) * groups * U; base < rows; base += int64_t(gridDim.x) * groups * U) {
+    typename P::Raw raw[U][NV];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t row = base + group * U + u;
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        const int c = (v * lanes + lane) * VEC;
+        raw[u][v] = row < rows && c < dim ? P::load(x + row * x_stride + c) : P::zero();
+      }
+    }
+    float m[U], s[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      m[u] = 0.0f;
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        float f[VEC];
+        P::open(raw[u][v], f);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) m[u] += f[i];
+      }
+    }
+    sum(m);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      m[u] *= inv;
+      s[u] = 0.0f;
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        float f[VEC];
+        P::open(raw[u][v], f);
+        if ((v * lanes + lane) * VEC < dim) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            const float d = f[i] - m[u];
+            s[u] = __fmaf_rn(d, d, s[u]);
+          }
+        }
+      }
+    }
+    sum(s);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t row = base + group * U + u;
+      if (row >= rows) continue;
+      const float r = 1.0f / sqrtf(s[u] * inv + eps);
+      if (lane == 0) {
+        if (mean_out) mean_out[row] = m[u];
+        if (rstd_out) rstd_out[row] = r;
+      }
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        const int c = (v * lanes + lane) * VEC;
+        float f[VEC];
+        P::open(raw[u][v], f);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) f[i] = __fmaf_rn((f[i] - m[u]) * r, w[v][i], b[v][i]);
+        if (c < dim) P::store(y + row * dim + c, f);
+      }
+    }
+  }
+}
+
+// Rows longer than a block's registers: three passes over the row (the second
+// and third out of L2).
+template <class V>
+__global__ void __launch_bounds__(512)
+k_norm_forward_long(const typename V::T *__restrict__ x, int64_t x_stride, int64_t rows, int64_t dim,
+                    const void *__restrict__ weight, const void *__restrict__ bias, int ptype, float eps,
+                    typename V::T *__restrict__ y, float *__restrict__ mean_out, float *__restrict__ rstd_out) {
+  __shared__ float red[2][32][2];
+  RowSum<1, true> sum{32, red};
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    const typename V::T *xr = x + row * x_stride;
+    float m[1] = {0.0f}, s[1] = {0.0f};
+    for (int64_t c = threadIdx.x; c < dim; c += blockDim.x) m[0] += V::load(xr[c]);
+    sum(m);
+    m[0] /= float(dim);
+    for (int64_t c = threadIdx.x; c < dim; c += blockDim.x) {
+      const float d = V::load(xr[c]) - m[0];
+      s[0] = __fmaf_rn(d, d, s[0]);
+    }
+    sum(s);
+    const float r = 1.0f / sqrtf(s[0] / float(dim) + eps);
+    if (threadIdx.x == 0) {
+      if (mean_out) mean_out[row] = m[0];
+      if (rstd_out) rstd_out[row] = r;
+    }
+    for (int64_t c = threadIdx.x; c < dim; c += blockDim.x)
+      y[row * dim + c] = V::store(__fmaf_rn((V::load(xr[c]) - m[0]) * r, param_at(weight, ptype, c, 1.0f),
+                                            param_at(bias, ptype, c, 0.0f)));
+  }
+}
+
+// Backward of rows held in registers (layout as k_norm_forward). partial:
+// [gridDim.x][2][dim] fp32, this block's sums of g h and of g per column
+// (null: no weight gradients wanted).
+template <class V, int VEC, int NV, int U, bool WIDE>
+__global__ void __launch_bounds__(WIDE ? norm_wide_threads(VEC) : kNormNarrowThreads)
+k_norm_backward(const typename V::T *__restrict__ grad, int64_t g_stride, const typename V::T *__restrict__ x,
+                int64_t x_stride, int64_t rows, int dim, const float *__restrict__ mean,
+                const float *__restrict__ rstd, const void *__restrict__ weight, int ptype,
+                typename V::T *__restrict__ dx, float *__restrict__ partial, int lanes) {
+  using P = Pack<V, VEC>;
+  __shared__ float red[2][32][2];
+  extern __shared__ float cols[];  // narrow: [warps][dim]
+  const int lane = WIDE ? int(threadIdx.x) : int(threadIdx.x) & (lanes - 1);
+  const int group = WIDE ? 0 : int(threadIdx.x) / lanes;
+  const int groups = WIDE ? 1 : int(blockDim.x) / lanes;
+  float w[NV][VEC], dw[NV][VEC], db[NV][VEC];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const int c = (v * lanes + lane) * VEC + i;
+      w[v][i] = c < dim ? param_at(weight, ptype, c, 1.0f) : 0.0f;
+      dw[v][i] = 0.0f;
+      db[v][i] = 0.0f;
+    }
+  }
+  RowSum<2, WIDE> sum{lanes, red};
+  const float inv = 1.0f / float(dim);
+  for (int64_t base = int64_t(blockIdx.x) * groups * U; base < rows; base += int64_t(gridDim.x) * groups * U) {
+    typename P::Raw xr[U][NV], gr[U][NV];
+    float m[U], r[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t row = base + group * U + u;
+      m[u] = row < rows ? mean[row] : 0.0f;
+      r[u] = row < rows ? rstd[row] : 0.0f;
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        const int c = (v * lanes + lane) * VEC;
+        const bool in = row < rows && c < dim;
+        xr[u][v] = in ? P::load(x + row * x_stride + c) : P::zero();
+        gr[u][v] = in ? P::load(grad + row * g_stride + c) : P::zero();
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t row = base + group * U + u;
+      float s[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        if (row < rows && (v * lanes + lane) * VEC < dim) {
+          float xf[VEC], gf[VEC];
+          P::open(xr[u][v], xf);
+          P::open(gr[u][v], gf);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            const float h = (xf[i] - m[u]) * r[u], q = gf[i] * w[v][i];
+            s[0] += q;
+            s[1] = __fmaf_rn(q, h, s[1]);
+            dw[v][i] = __fmaf_rn(gf[i], h, dw[v][i]);
+            db[v][i] += gf[i];
+          }
+        }
+      }
+      sum(s);
+      s[0] *= inv;
+      s[1] *= inv;
+      if (row < rows) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+          const int c = (v * lanes + lane) * VEC;
+          float xf[VEC], gf[VEC];
+          P::open(xr[u][v], xf);
+          P::open(gr[u][v], gf);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            const float h = (xf[i] - m[u]) * r[u];
+            gf[i] = r[u] * (__fmaf_rn(gf[i], w[v][i], -s[0]) - h * s[1]);
+          }
+          if (c < dim) P::store(dx + row * dim + c, gf);
+        }
+      }
+    }
+  }
+  if (partial == nullptr) return;
+  float *out = partial + int64_t(blockIdx.x) * 2 * dim;
+  if constexpr (WIDE) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const int c = (v * lanes + lane) * VEC + i;
+        if (c < dim) {
+          out[c] = dw[v][i];
+          out[dim + c] = db[v][i];
+        }
+      }
+    }
+  } else {
+    // the warp's row groups by shuffles, then the block's warps in warp order
+    const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          float f = k == 0 ? dw[v][i] : db[v][i];
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) {
+            if (o >= lanes) f += __shfl_xor_sync(0xffffffffu, f, o);
+          }
+          const int c = (v * lanes + lane) * VEC + i;
+          if ((threadIdx.x & 31) < unsigned(lanes) && c < dim) cols[warp * dim + c] = f;
+        }
+      }
+      __syncthreads();
+      for (int c = threadIdx.x; c < dim; c += blockDim.x) {
+        float f = 0.0f;
+        for (int i = 0; i < warps; ++i) f += cols[i * dim + c];
+        out[k * dim + c] = f;
+      }
+      __syncthreads();
+    }
+  }
+}
+
+template <class V>
+__global__ void __launch_bounds__(512)
+k_norm_backward_long(const typename V::T *__restrict__ grad, int64_t g_stride, const typename V::T *__restrict__ x,
+                     int64_t x_stride, int64_t rows, int64_t dim, const float *__restrict__ mean,
+                     const float *__restrict__ rstd, const void *__restrict__ weight, int ptype,
+                     typename V::T *__restrict__ dx) {
+  __shared__ float red[2][32][2];
+  RowSum<2, true> sum{32, red};
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    const typename V::T *xr = x + row * x_stride, *gr = grad + row * g_stride;
+    const float m = mean[row], r = rstd[row];
+    float s[2] = {0.0f, 0.0f};
+    for (int64_t c = threadIdx.x; c < dim; c += blockDim.x) {
+      const float q = V::load(gr[c]) * param_at(weight, ptype, c, 1.0f);
+      s[0] += q;
+      s[1] = __fmaf_rn(q, (V::load(xr[c]) - m) * r, s[1]);
+    }
+    sum(s);
+    s[0] /= float(dim);
+    s[1] /= float(dim);
+    for (int64_t c = threadIdx.x; c < dim; c += blockDim.x) {
+      const float q = V::load(gr[c]) * param_at(weight, ptype, c, 1.0f);
+      dx[row * dim + c] = V::store(r * (q - s[0] - (V::load(xr[c]) - m) * r * s[1]));
+    }
+  }
+}
+
+// Column sums of long rows: a thread per column and split of the rows.
+template <class V>
+__global__ void __launch_bounds__(256)
+k_norm_columns_long(const typename V::T *__restrict__ grad, int64_t g_stride, const typename V::T *__restrict__ x,
+                    int64_t x_stride, int64_t rows, int64_t dim, const float *__restrict__ mean,
+                    const float *__restrict__ rstd, float *__restrict__ partial) {
+  const int64_t c = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
+  if (c >= dim) return;
+  const int64_t each = (rows + gridDim.y - 1) / gridDim.y;
+  const int64_t first = blockIdx.y * each, last = first + each < rows ? first + each : rows;
+  float dw = 0.0f, db = 0.0f;
+  for (int64_t row = first; row < last; ++row) {
+    const float g = V::load(grad[row * g_stride + c]);
+    dw = __fmaf_rn(g, (V::load(x[row * x_stride + c]) - mean[row]) * rstd[row], dw);
+    db += g;
+  }
+  partial[int64_t(blockIdx.y) * 2 * dim + c] = dw;
+  partial[int64_t(blockIdx.y) * 2 * dim + dim + c] = db;
+}
+
+// dw and db: the blocks' sums of each column, added in a fixed order (each of
+// the 16 threads of a column takes every 16th block, then the 16 in order).
+__global__ void __launch_bounds__(512)
+k_norm_columns(const float *__restrict__ partial, int blocks, int64_t dim, void *__restrict__ dweight,
+               void *__restrict__ dbias, int ptype) {
+  __shared__ float part[16][33];
+  const int lane = threadIdx.x & 31, strip = threadIdx.x >> 5;
+  const int64_t c = int64_t(blockIdx.x) * 32 + lane;
+  pdl_wait();
+  float f = 0.0f;
+  if (c < 2 * dim) {
+#pragma unroll 4
+    for (int k = strip; k < blocks; k += 16) f += partial[int64_t(k) * 2 * dim + c];
+  }
+  part[strip][lane] = f;
+  __syncthreads();
+  if (strip == 0 && c < 2 * dim) {
+    f = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) f += part[k][lane];
+    if (c < dim) {
+      if (dweight) param_put(dweight, ptype, c, f);
+    } else if (dbias) {
+      param_put(dbias, ptype, c - dim, f);
+    }
+  }
+}
+
+constexpr int kNormLongSplits = 64;
+
+// How a call's rows are laid over threads.
+struct NormShape {
+  bool vec;    // 16-byte vectors
+  bool wide;   // a block per row
+  bool longer; // rows beyond a block's registers
+  int nv, lanes, threads, unroll;
+};
+
+NormShape norm_shape(int64_t dim, size_t value_size, bool aligned) {
+  NormShape s{};
+  const int per = int(16 / value_size);
+  s.vec = aligned && dim % per == 0;
+  const int64_t n = s.vec ? dim / per : dim;  // loads per row
+  s.threads = kNormNarrowThreads;
+  if (n <= 128) {
+    s.nv = n <= 32 ? 1 : n <= 64 ? 2 : 4;
+    s.unroll = 4 / s.nv;
+    s.lanes = 1;
+    while (s.lanes < n && s.lanes < 32) s.lanes *= 2;
+    return s;
+  }
+  s.nv = norm_wide_loads(s.vec ? per : 1);
+  s.unroll = 1;
+  s.wide = true;
+  const int64_t threads = (n + s.nv - 1) / s.nv;
+  const int most = norm_wide_threads(s.vec ? per : 1);
+  s.longer = threads > most;
+  s.threads = int(std::min<int64_t>(most, (threads + 31) / 32 * 32));
+  s.lanes = s.threads;
+  return s;
+}
+
+// Most blocks of the register kernels: `sms` x 1,024 threads. More
+// blocks would add sums to the workspace and to the second kernel.
+int norm_blocks(int64_t rows, const NormShape &s, int sms) {
+  const int64_t per_block = s.wide ? 1 : int64_t(s.threads / s.lanes) * s.unroll;
+  const int64_t need = (rows + per_block - 1) / per_block;
+  return int(std::max<int64_t>(1, std::min<int64_t>(need, int64_t(sms) * (1024 / s.threads))));
+}
+
+// f with the kernel's constants: values per load, loads per thread, rows at a
+// time, a block per row.
+template <class V, class F>
+void with_norm_shape(const NormShape &s, F &&f) {
+  using std::integral_constant;
+  auto go = [&](auto vec) {
+    constexpr int kVec = decltype(vec)::value;
+    if (s.wide) f(vec, integral_constant<int, norm_wide_loads(kVec)>{}, integral_constant<int, 1>{}, std::true_type{});
+    else if (s.nv == 1) f(vec, integral_constant<int, 1>{}, integral_constant<int, 4>{}, std::false_type{});
+    else if (s.nv == 2) f(vec, integral_constant<int, 2>{}, integral_constant<int, 2>{}, std::false_type{});
+    else f(vec, integral_constant<int, 4>{}, integral_constant<int, 1>{}, std::false_type{});
+  };
+  if (s.vec) go(integral_constant<int, int(16 / sizeof(typename V::T))>{});
+  else go(integral_constant<int, 1>{});
+}
+
+void check_norm(int32_t value_dtype, int32_t param_dtype, size_t rows, int64_t dim) {
+  check_value_dtype(value_dtype, "value_dtype");
+  check_value_dtype(param_dtype, "param_dtype");
+  if (dim <= 0) throw std::invalid_argument("dim must be > 0");
+  if (dim > (int64_t(1) << 30)) throw std::invalid_argument("dim must be at most 2^30");
+  if (rows > (size_t(1) << 40)) throw std::invalid_argument("rows must be at most 2^40");
+}
+
+}  // namespace
+
+}  // namespace se_gpu
+
+using namespace se_gpu;
+
+extern "C" int se_layer_norm(int32_t value_dtype, int32_t param_dtype, const void *x, size_t rows, int64_t dim,
+                             int64_t x_stride, const void *weight, const void *bias, float eps, void *y,
+                             float *mean_out, float *rstd_out, int32_t device, void *stream) {
+  return guarded([&] {
+    check_norm(value_dtype, param_dtype, rows, dim);
+    if (!(eps >= 0.0f) || !std::isfinite(eps)) throw std::invalid_argument("eps must be finite and non-negative");
+    if (rows == 0) return;
+    if (x_stride < dim && rows > 1) throw std::invalid_argument("x_stride must be at least dim");
+    DeviceGuard dg(device);
+    check_device_ptr(x, device, "x");
+    check_device_ptr(y, device, "y");
+    check_device_ptr(weight, device, "weight", true);
+    check_device_ptr(bias, device, "bias", true);
+    check_device_ptr(mean_out, device, "mean", true);
+    check_device_ptr(rstd_out, device, "rstd", true);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const int sms = sm_count(device);
+    const size_t vb = value_bytes(value_dtype);
+    const NormShape s = norm_shape(dim, vb, aligned16(x) && aligned16(y) && (rows == 1 || x_stride * vb % 16 == 0));
+    dispatch_value(value_dtype, [&](auto tag) {
+      using V = decltype(tag);
+      using T = typename V::T;
+      const T *xp = static_cast<const T *>(x);
+      T *yp = static_cast<T *>(y);
+      if (s.longer) {
+        const unsigned grid = unsigned(std::min<size_t>(rows, size_t(sms) * 4));
+        k_norm_forward_long<V><<<grid, 512, 0, st>>>(xp, x_stride, int64_t(rows), dim, weight, bias, param_dtype, eps,
+                                                     yp, mean_out, rstd_out);
+        launched("k_norm_forward_long");
+        return;
+      }
+      const int grid = norm_blocks(int64_t(rows), s, sms * 2);
+      with_norm_shape<V>(s, [&](auto vec, auto nv, auto u, auto wide) {
+        k_norm_forward<V, decltype(vec)::value, decltype(nv)::value, decltype(u)::value, decltype(wide)::value>
+            <<<grid, s.threads, 0, st>>>(xp, x_stride, int64_t(rows), int(dim), weight, bias, param_dtype, eps, yp,
+                                         mean_out, rstd_out, s.lanes);
+      });
+      launched("k_norm_forward");
+    });
+  });
+}
+
+extern "C" int se_layer_norm_backward_workspace(size_t rows, int64_t dim, int32_t device, size_t *bytes) {
+  return guarded([&] {
+    check_norm(SE_FLOAT32, SE_FLOAT32, rows, dim);
+    if (bytes == nullptr) throw std::invalid_argument("bytes is null");
+    // Enough for every type and alignment of the same rows and dim.
+    const int sms = sm_count(device);
+    int blocks = 1;
+    for (const size_t vb : {size_t(2), size_t(4)}) {
+      for (const bool aligned : {false, true}) {
+        const NormShape s = norm_shape(dim, vb, aligned);
+        blocks = std::max(blocks, s.longer ? int(std::min<size_t>(rows, kNormLongSplits))
+                                           : norm_blocks(int64_t(rows), s, sms));
+      }
+    }
+    *bytes = size_t(blocks) * 2 * size_t(dim) * sizeof(float);
+  });
+}
+
+extern "C" int se_layer_norm_backward(int32_t value_dtype, int32_t param_dtype, const void *grad, int64_t grad_stride,
+                                      const void *x, int64_t x_stride, size_t rows, int64_t dim, const float *mean,
+                                      const float *rstd, const void *weight, void *dx, void *dweight, void *dbias,
+                                      void *workspace, size_t workspace_bytes, int32_t device, void *stream) {
+  return guarded([&] {
+    check_norm(value_dtype, param_dtype, rows, dim);
+    if (rows > 1 && (x_stride < dim || grad_stride < dim))
+      throw std::invalid_argument("x_stride and grad_stride must be at least dim");
+    DeviceGuard dg(device);
+    check_device_ptr(weight, device, "weight", true);
+    check_device_ptr(dweight, device, "dweight", true);
+    check_device_ptr(dbias, device, "dbias", true);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const int sms = sm_count(device);
+    const bool sums = dweight != nullptr || dbias != nullptr;
+    int blocks = 0;
+    float *partial = nullptr;
+    if (rows > 0) {
+      check_device_ptr(grad, device, "grad");
+      check_device_ptr(x, device, "x");
+      check_device_ptr(mean, device, "mean");
+      check_device_ptr(rstd, device, "rstd");
+      check_device_ptr(dx, device, "dx");
+      const size_t vb = value_bytes(value_dtype);
+      const NormShape s = norm_shape(dim, vb, aligned16(x) && aligned16(grad) && aligned16(dx) &&
+                                                  (rows == 1 || (x_stride * vb % 16 == 0 && grad_stride * vb % 16 == 0)));
+      blocks = s.longer ? int(std::min<size_t>(rows, kNormLongSplits)) : norm_blocks(int64_t(rows), s, sms);
+      if (sums) {
+        check_device_ptr(workspace, device, "workspace");
+        if (reinterpret_cast<uintptr_t>(workspace) % 4 != 0 ||
+            workspace_bytes < size_t(blocks) * 2 * size_t(dim) * sizeof(float))
+          throw std::invalid_argument("workspace is smaller than se_layer_norm_backward_workspace asks for");
+        partial = static_cast<float *>(workspace);
+      }
+      dispatch_value(value_dtype, [&](auto tag) {
+        using V = decltype(tag);
+        using T = typename V::T;
+        const T *xp = static_cast<const T *>(x), *gp = static_cast<const T *>(grad);
+        T *dxp = static_cast<T *>(dx);
+        if (s.longer) {
+          const unsigned grid = unsigned(std::min<size_t>(rows, size_t(sms) * 4));
+          k_norm_backward_long<V><<<grid, 512, 0, st>>>(gp, grad_stride, xp, x_stride, int64_t(rows), dim, mean, rstd,
+                                                        weight, param_dtype, dxp);
+          launched("k_norm_backward_long");
+          if (sums) {
+            const dim3 cgrid(unsigned((dim + 255) / 256), unsigned(blocks));
+            k_norm_columns_long<V><<<cgrid, 256, 0, st>>>(gp, grad_stride, xp, x_stride, int64_t(rows), dim, mean,
+                                                          rstd, partial);
+            launched("k_norm_columns_long");
+          }
+          return;
+        }
+        with_norm_shape<V>(s, [&](auto vec, auto nv, auto u, auto wide) {
+            const size_t smem = s.wide || !sums ? 0 : size_t(s.threads / 32) * size_t(dim) * sizeof(float);
+          k_norm_backward<V, decltype(vec)::value, decltype(nv)::value, decltype(u)::value, decltype(wide)::value>
+              <<<blocks, s.threads, smem, st>>>(gp, grad_stride, xp, x_stride, int64_t(rows), int(dim), mean, rstd,
+                                                weight, param_dtype, dxp, partial, s.lanes);
+        });
+        launched("k_norm_backward");
+      });
+    }
+    if (sums) {
+      pdl(k_norm_columns, unsigned((2 * dim + 31) / 32), 512, 0, st, static_cast<const float *>(partial), blocks, dim,
+          dweight, dbias, int(param_dtype));
+      count_launch();
+    }
+  });
+}

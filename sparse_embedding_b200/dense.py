@@ -1,0 +1,163 @@
+"""Dense operators that run next to the store: layer normalisation of its rows
+(pooled bags, looked-up rows) with the backward pass. They have no counterpart
+in the reference, whose users run the dense part of a model outside it.
+
+Inputs are CUDA tensors (or DLPack objects in CUDA memory) whose last axis is
+contiguous; rows may lie further apart than their length, as slices of wider
+tensors do. The work runs on the current torch stream of the tensors' device,
+allocates from torch's allocator only and never waits for the GPU, so calls can
+be captured into CUDA graphs. `torch_ops` has the autograd forms.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+from . import _native as N
+from ._tensors import _torch_dtype_name, is_torch_tensor, torch_mod
+
+_FLOATS = {}  # torch dtype -> code of the C ABI
+
+
+def _code(dtype) -> int:
+    if not _FLOATS:
+        torch = torch_mod()
+        _FLOATS.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+    return _FLOATS.get(dtype, -1)
+
+
+def _cuda_tensor(x, what: str):
+    """x as a CUDA tensor of a supported dtype."""
+    if not is_torch_tensor(x):
+        if not hasattr(x, "__dlpack__"):
+            raise TypeError(f"{what} must be a CUDA tensor")
+        x = torch_mod().from_dlpack(x)
+    if not x.is_cuda:
+        raise ValueError(f"{what} must be a CUDA tensor")
+    if _code(x.dtype) < 0:
+        raise ValueError(f"unsupported {what} dtype: {_torch_dtype_name(x)}")
+    return x
+
+
+def _strided(x, last: int):
+    """(count, stride) of the blocks that x's last `last` axes form, over its
+    leading axes; None where no single stride covers them."""
+    count, stride = 1, None
+    for size, step in zip(reversed(x.shape[: x.dim() - last]), reversed(x.stride()[: x.dim() - last])):
+        if size != 1:
+            if stride is None:
+                stride = step
+            elif step != stride * count:
+                return None
+        count *= size
+    return count, stride or 0
+
+
+def _rows(x, what: str):
+    """(rows, dim, row stride) of x as rows of its last axis."""
+    if x.dim() < 1:
+        raise ValueError(f"{what} must have at least one dimension")
+    dim = x.shape[-1]
+    if dim == 0:
+        raise ValueError("dim must be > 0")
+    if x.is_contiguous():
+        return x.numel() // dim, dim, dim
+    if x.numel() == 0:
+        return 0, dim, dim
+    found = _strided(x, 1)
+    if (dim > 1 and x.stride(-1) != 1) or found is None or (found[0] > 1 and found[1] < dim):
+        raise ValueError(f"{what} must be rows at one stride with a contiguous last dimension")
+    rows, stride = found
+    return rows, dim, max(stride, dim)
+
+
+def _same_device(a, b, what: str) -> None:
+    if a.device != b.device:
+        raise ValueError(f"{what} is on {b.device}, the call on {a.device}")
+
+
+def _affine(x, dim: int, weight, bias):
+    if weight is None:
+        if bias is not None:
+            raise ValueError("bias needs a weight")
+        return None, None, 0
+    out = []
+    for p, what in ((weight, "weight"), (bias, "bias")):
+        if p is not None:
+            p = _cuda_tensor(p, what)
+            _same_device(x, p, what)
+            if p.dim() != 1 or p.shape[0] != dim or not p.is_contiguous():
+                raise ValueError(f"{what} must be a contiguous 1D tensor of dim values")
+            if p.dtype != x.dtype and p.dtype != torch_mod().float32:
+                raise ValueError(f"{what} must have x's dtype or float32")
+        out.append(p)
+    if out[1] is not None and out[1].dtype != out[0].dtype:
+        raise ValueError("weight and bias must have the same dtype")
+    return out[0], out[1], _code(out[0].dtype)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _stream(t) -> int:
+    return torch_mod().cuda.current_stream(t.device).cuda_stream
+
+
+def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, return_stats: bool = False):
+    """Normalises the rows of x [..., dim] (float32, float16 or bfloat16):
+    y = (x - mean) / sqrt(var + eps) * weight + bias over the last axis, with
+    fp32 statistics. weight and bias [dim] have x's dtype or float32. Returns
+    y, or with return_stats (y, mean, rstd): fp32, of x's leading shape, as
+    layer_norm_backward takes them. Outside autograd."""
+    x = _cuda_tensor(x, "x")
+    rows, dim, stride = _rows(x, "x")
+    weight, bias, pcode = _affine(x, dim, weight, bias)
+    eps = float(eps)
+    if not math.isfinite(eps) or eps < 0.0:
+        raise ValueError("eps must be finite and non-negative")
+    torch = torch_mod()
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean = rstd = None
+    if return_stats:
+        mean, rstd = (torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) for _ in range(2))
+    N.check(N.lib().se_layer_norm(_code(x.dtype), pcode, x.data_ptr(), rows, dim, stride, _ptr(weight), _ptr(bias), eps,
+                                  y.data_ptr(), _ptr(mean), _ptr(rstd), x.device.index, _stream(x)))
+    return (y, mean, rstd) if return_stats else y
+
+
+def layer_norm_backward(grad, x, mean, rstd, weight=None, with_bias: bool = True):
+    """(dx, dweight, dbias) of layer_norm for the gradient of its y: `grad` has
+    x's shape and dtype, mean and rstd come from the forward pass. Without a
+    weight dweight and dbias are None; dbias also without with_bias. They have
+    the weight's dtype, are summed in fp32, and equal calls on one device give
+    equal bits."""
+    x = _cuda_tensor(x, "x")
+    grad = _cuda_tensor(grad, "grad")
+    _same_device(x, grad, "grad")
+    if grad.shape != x.shape or grad.dtype != x.dtype:
+        raise ValueError("grad must have x's shape and dtype")
+    rows, dim, stride = _rows(x, "x")
+    _, _, gstride = _rows(grad, "grad")
+    weight, _, pcode = _affine(x, dim, weight, None)
+    torch = torch_mod()
+    for t, what in ((mean, "mean"), (rstd, "rstd")):
+        if not is_torch_tensor(t) or t.dtype != torch.float32 or t.numel() != rows or not t.is_contiguous():
+            raise ValueError(f"{what} must be a contiguous float32 tensor with a value per row")
+        _same_device(x, t, what)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dw = db = work = None
+    nbytes = 0
+    L = N.lib()
+    if weight is not None:
+        dw = torch.empty_like(weight)
+        db = torch.empty_like(weight) if with_bias else None
+        size = C.c_size_t()
+        N.check(L.se_layer_norm_backward_workspace(rows, dim, x.device.index, C.byref(size)))
+        nbytes = size.value
+        work = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    N.check(L.se_layer_norm_backward(_code(x.dtype), pcode, grad.data_ptr(), gstride, x.data_ptr(), stride, rows, dim,
+                                     mean.data_ptr(), rstd.data_ptr(), _ptr(weight), dx.data_ptr(), _ptr(dw), _ptr(db),
+                                     _ptr(work), nbytes, x.device.index, _stream(x)))
+    return dx, dw, db
