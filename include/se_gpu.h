@@ -308,6 +308,33 @@ int se_layer_norm_backward(int32_t value_dtype, int32_t param_dtype, const void 
                            void *workspace, size_t workspace_bytes, int32_t device, void *stream);
 int se_layer_norm_backward_workspace(size_t rows, int64_t dim, int32_t device, size_t *bytes);
 
+/* Orthogonalises `batch` updates of m x n values by Newton-Schulz products:
+ * X = U / (|U|_F + eps), then `steps` times (1 to 100) A = X X^T,
+ * X = 3.4445 X + (-4.7750 A + 2.0315 A A) X (on U^T where m > n), which brings
+ * every singular value that is not tiny into about [0.68, 1.2]. Matrix k
+ * starts batch_stride values after matrix k - 1, its rows are row_stride
+ * apart; out is batch x m x n without gaps, of the same dtype, and overlaps
+ * no input. Products of f16 pairs with fp32 sums: a bf16 result is within its
+ * own rounding of the exact one, fp32 and f16 results use three products for
+ * one. `workspace`: se_muon_workspace bytes, 256-byte aligned. A wait inside
+ * the kernels that gives up is reported by the next call (SE_ERR_RUNTIME). */
+int se_orthogonalize(int32_t dtype, const void *update, size_t batch, int64_t m, int64_t n, int64_t batch_stride,
+                     int64_t row_stride, int32_t steps, float eps, void *out, void *workspace,
+                     size_t workspace_bytes, int32_t device, void *stream);
+/* One Muon step of `batch` weight matrices (m x n, weight_dtype), in place:
+ *   momentum = beta momentum + grad                        (fp32)
+ *   U = grad + beta momentum if nesterov, else momentum
+ *   weight = (1 - lr weight_decay) weight - lr scale orthogonalize(U)
+ * Weight, gradient and momentum overlap nowhere. */
+int se_muon_step(int32_t weight_dtype, int32_t grad_dtype, void *weight, int64_t weight_batch_stride,
+                 int64_t weight_row_stride, const void *grad, int64_t grad_batch_stride, int64_t grad_row_stride,
+                 float *momentum, int64_t momentum_batch_stride, int64_t momentum_row_stride, size_t batch,
+                 int64_t m, int64_t n, double lr, double beta, double weight_decay, double scale,
+                 int32_t nesterov, int32_t steps, float eps, void *workspace, size_t workspace_bytes,
+                 int32_t device, void *stream);
+/* Bytes of workspace for either call; out_dtype is the result's, or the weight's. */
+int se_muon_workspace(int32_t out_dtype, size_t batch, int64_t m, int64_t n, size_t *bytes);
+
 /*
  * Exchange routing (no reference counterpart: the reference leaves routing to
  * the caller, sparse_embedding/partitioner.py:84-100). Device pointers only.

@@ -29,7 +29,7 @@ from .partitioner import (
     register_partitioner,
 )
 from .unique import async_unique, unique
-from .dense import layer_norm, layer_norm_backward
+from .dense import layer_norm, layer_norm_backward, muon_step, orthogonalize
 from .store import (
     Adagrad,
     Adam,
@@ -62,5 +62,5 @@ __all__ = [
     "SPARSE_EMBEDDING_MODULO_ASSIGNMENT_NAME", "SUPPORTED_KEY_DTYPES", "Sgd", "StorageTuningOptions",
     "Uniform", "Zeros", "create_partitioner", "create_strategy", "filter_partition",
     "generate_reference_vectors", "is_partitioner_registered", "layer_norm", "layer_norm_backward",
-    "partition", "register_partitioner",
+    "muon_step", "orthogonalize", "partition", "register_partitioner",
 ]

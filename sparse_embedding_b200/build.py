@@ -19,9 +19,9 @@ PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_DIR = PKG_DIR / "_lib"
 LIB_PATH = LIB_DIR / "libse_gpu.so"
-SOURCES = ["se_store.cu", "se_partition.cu", "se_unique.cu", "se_norm.cu"]
+SOURCES = ["se_store.cu", "se_partition.cu", "se_unique.cu", "se_norm.cu", "se_muon.cu"]
 HEADERS = ["se_common.cuh", "se_host.hpp", "se_store_kernels.cuh", "se_partition.cuh", "se_exchange.cuh",
-           "se_accum.cuh", "se_dense.hpp"]
+           "se_accum.cuh", "se_dense.hpp", "se_tcgen05.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

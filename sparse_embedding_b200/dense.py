@@ -1,6 +1,8 @@
 """Dense operators that run next to the store: layer normalisation of its rows
-(pooled bags, looked-up rows) with the backward pass. They have no counterpart
-in the reference, whose users run the dense part of a model outside it.
+(pooled bags, looked-up rows) with the backward pass, and the Muon update of the
+matrices that read them, beside the store's own row optimizers. They have no
+counterpart in the reference, whose users run the dense part of a model outside
+it.
 
 Inputs are CUDA tensors (or DLPack objects in CUDA memory) whose last axis is
 contiguous; rows may lie further apart than their length, as slices of wider
@@ -161,3 +163,87 @@ def layer_norm_backward(grad, x, mean, rstd, weight=None, with_bias: bool = True
                                      mean.data_ptr(), rstd.data_ptr(), _ptr(weight), dx.data_ptr(), _ptr(dw), _ptr(db),
                                      _ptr(work), nbytes, x.device.index, _stream(x)))
     return dx, dw, db
+
+
+def _matrices(x, what: str):
+    """(batch, m, n, batch stride, row stride) of x as matrices of its last two axes."""
+    if x.dim() < 2:
+        raise ValueError(f"{what} must have at least two dimensions")
+    m, n = x.shape[-2:]
+    if x.is_contiguous():
+        return (x.numel() // (m * n) if m * n else 0), m, n, m * n, n
+    if x.numel() == 0:
+        return 0, m, n, m * n, n
+    found = _strided(x, 2)
+    rs = x.stride(-2) if m > 1 else n
+    if (n > 1 and x.stride(-1) != 1) or found is None or rs < n or (found[0] > 1 and found[1] < (m - 1) * rs + n):
+        raise ValueError(f"{what} must be matrices at one stride with contiguous rows")
+    batch, bs = found
+    return batch, m, n, (bs if batch > 1 else m * rs), rs
+
+
+def _muon_work(code: int, batch: int, m: int, n: int, device):
+    size = C.c_size_t()
+    N.check(N.lib().se_muon_workspace(code, batch, m, n, C.byref(size)))
+    # torch's allocations are aligned to 512 bytes
+    return torch_mod().empty(size.value, dtype=torch_mod().uint8, device=device), size.value
+
+
+def orthogonalize(update, steps: int = 5, eps: float = 1e-7):
+    """Newton-Schulz orthogonalisation of update [..., m, n] (float32, float16
+    or bfloat16), as the Muon optimizer applies it: X = U / (|U| + eps), then
+    `steps` times X = 3.4445 X + (-4.7750 A + 2.0315 A A) X with A = X X^T
+    (from the smaller side). Leading axes are a batch of separate matrices.
+    Returns a new tensor of update's shape and dtype."""
+    u = _cuda_tensor(update, "update")
+    batch, m, n, bs, rs = _matrices(u, "update")
+    torch = torch_mod()
+    out = torch.empty(u.shape, dtype=u.dtype, device=u.device)
+    code = _code(u.dtype)
+    work, nbytes = _muon_work(code, batch, m, n, u.device)
+    N.check(N.lib().se_orthogonalize(code, u.data_ptr(), batch, m, n, bs, rs, int(steps), float(eps), out.data_ptr(),
+                                     work.data_ptr(), nbytes, u.device.index, _stream(u)))
+    return out
+
+
+def _span(x):
+    """First and last byte of x's storage range that its elements reach."""
+    size = sum((s - 1) * st for s, st in zip(x.shape, x.stride())) + 1
+    return x.data_ptr(), x.data_ptr() + size * x.element_size()
+
+
+def muon_step(weight, grad, momentum, lr: float = 0.02, beta: float = 0.95, weight_decay: float = 0.0,
+              nesterov: bool = True, steps: int = 5, eps: float = 1e-7, scale: float | None = None) -> None:
+    """One Muon step of weight [..., m, n], in place (outside autograd):
+
+        momentum = beta momentum + grad
+        U = grad + beta momentum if nesterov else momentum
+        weight = (1 - lr weight_decay) weight - lr scale orthogonalize(U)
+
+    momentum is float32 of weight's shape; grad has weight's dtype or float32.
+    scale is sqrt(max(1, m / n)) unless given. The three share no memory."""
+    w, g, mom = (_cuda_tensor(t, what) for t, what in ((weight, "weight"), (grad, "grad"), (momentum, "momentum")))
+    torch = torch_mod()
+    for t, what in ((g, "grad"), (mom, "momentum")):
+        _same_device(w, t, what)
+        if t.shape != w.shape:
+            raise ValueError(f"{what} must have weight's shape")
+    if mom.dtype != torch.float32:
+        raise ValueError("momentum must be float32")
+    if g.dtype != w.dtype and g.dtype != torch.float32:
+        raise ValueError("grad must have weight's dtype or float32")
+    batch, m, n, wbs, wrs = _matrices(w, "weight")
+    _, _, _, gbs, grs = _matrices(g, "grad")
+    _, _, _, mbs, mrs = _matrices(mom, "momentum")
+    if w.numel():
+        spans = sorted(_span(t) for t in (w, g, mom))
+        if spans[0][1] > spans[1][0] or spans[1][1] > spans[2][0]:
+            raise ValueError("weight, grad and momentum must not share memory")
+    if scale is None:
+        scale = math.sqrt(max(1.0, m / n)) if n else 1.0
+    code = _code(w.dtype)
+    work, nbytes = _muon_work(code, batch, m, n, w.device)
+    N.check(N.lib().se_muon_step(code, _code(g.dtype), w.data_ptr(), wbs, wrs, g.data_ptr(), gbs, grs, mom.data_ptr(),
+                                 mbs, mrs, batch, m, n, float(lr), float(beta), float(weight_decay), float(scale),
+                                 int(bool(nesterov)), int(steps), float(eps), work.data_ptr(), nbytes, w.device.index,
+                                 _stream(w)))

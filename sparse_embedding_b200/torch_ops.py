@@ -1,8 +1,9 @@
 """PyTorch autograd wrappers: the store's embedding bag (the forward is
 EmbeddingStore.embedding_bag, the backward accumulates the pooled gradients
 into the store, EmbeddingStore.embedding_bag_backward; the parameters are
-updated by EmbeddingStore.optimizer_step, outside autograd), and the layer
-normalisation of its rows (dense.layer_norm).
+updated by EmbeddingStore.optimizer_step, outside autograd), the layer
+normalisation of its rows (dense.layer_norm), and an optimizer for the dense
+matrices behind them (dense.muon_step).
 """
 
 from __future__ import annotations
@@ -60,3 +61,41 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
         except ValueError:
             x = x.contiguous()
     return LayerNormFunction.apply(x, weight, bias, eps)
+
+
+class Muon(torch.optim.Optimizer):
+    """Muon for the dense matrices of a model, next to the store's own row
+    optimizers: each parameter [..., m, n] takes dense.muon_step with a float32
+    momentum (leading axes are separate matrices: stacked layers or experts).
+    Vectors (biases, normalisation weights) need another optimizer."""
+
+    def __init__(self, params, lr: float = 0.02, momentum: float = 0.95, weight_decay: float = 0.0,
+                 nesterov: bool = True, steps: int = 5, eps: float = 1e-7):
+        super().__init__(params, dict(lr=lr, momentum=momentum, weight_decay=weight_decay, nesterov=nesterov,
+                                      steps=steps, eps=eps))
+
+    def add_param_group(self, param_group) -> None:
+        super().add_param_group(param_group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dim() < 2:
+                raise ValueError("Muon steps matrices: every parameter needs at least two dimensions")
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse:
+                    raise ValueError("Muon needs dense gradients")
+                state = self.state[p]
+                if "momentum_buffer" not in state:
+                    state["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+                dense.muon_step(p, p.grad.contiguous(), state["momentum_buffer"], lr=group["lr"],
+                                beta=group["momentum"], weight_decay=group["weight_decay"],
+                                nesterov=group["nesterov"], steps=group["steps"], eps=group["eps"])
+        return loss
