@@ -51,24 +51,35 @@ struct Strided {  // a batch of matrices with contiguous rows
   int64_t batch, row;
 };
 
-constexpr int kNormParts = 128;  // blocks (and partial sums) per matrix, at most
-
-// Element (i, j) of matrix z as fp32, for a type given at run time.
-__device__ __forceinline__ float strided_at(const Strided &s, int type, int64_t z, int64_t i, int64_t j) {
-  const int64_t at = z * s.batch + i * s.row + j;
-  if (type == SE_FLOAT32) return static_cast<const float *>(s.p)[at];
-  if (type == SE_FLOAT16) return __half2float(static_cast<const __half *>(s.p)[at]);
-  return __bfloat162float(static_cast<const __nv_bfloat16 *>(s.p)[at]);
-}
+constexpr int kNormParts = 512;  // blocks (and partial sums) per matrix, at most
+constexpr int kSpan = 2048;      // values of a row that a block takes at a time, 8 per thread
 
 struct UpdateArgs {
   Strided grad;      // the update itself (orthogonalize), or the gradient
-  int grad_type;
   Strided momentum;  // fp32; p null: the update is grad
   float beta;
   int nesterov;
   int64_t m, n;
+  int vec;           // rows of both start at 16-byte boundaries, n is a multiple of 8
 };
+
+// Eight consecutive values, or with vec = 0 eight that are `step` apart, the first `count`.
+template <class V>
+__device__ __forceinline__ void load_eight(const typename V::T *p, bool vec, int step, int count, float (&f)[8]) {
+  using T = typename V::T;
+  if (vec) {
+    constexpr int kPer = 16 / sizeof(T);
+    uint4 raw[8 / kPer];
+#pragma unroll
+    for (int i = 0; i < 8 / kPer; ++i) raw[i] = count > 0 ? reinterpret_cast<const uint4 *>(p)[i] : make_uint4(0u, 0u, 0u, 0u);
+    const T *v = reinterpret_cast<const T *>(raw);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = V::load(v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = i < count ? V::load(p[i * step]) : 0.0f;
+  }
+}
 
 // U from the gradient and the momentum after its update.
 __device__ __forceinline__ float update_of(const UpdateArgs &a, float g, float mom) {
@@ -76,22 +87,50 @@ __device__ __forceinline__ float update_of(const UpdateArgs &a, float g, float m
 }
 
 // M <- beta M + G, and this block's part of |U|^2 (fp64: squares of fp32
-// values neither overflow nor vanish there).
+// values neither overflow nor vanish there). Zeroes the counters of the launch
+// that follows. Bound by HBM: a matrix without gaps is taken as one row, and
+// every thread has 8 values of each array in flight.
+template <class V, bool MOM>
 __global__ void __launch_bounds__(256)
-k_muon_momentum(UpdateArgs a, double *__restrict__ parts) {
+k_muon_momentum(UpdateArgs a, double *__restrict__ parts, uint32_t *__restrict__ counters, int64_t ncounters) {
   __shared__ double red[8];
-  const int64_t z = blockIdx.y, count = a.m * a.n;
+  const int64_t z = blockIdx.y;
+  if (z == 0) {
+    for (int64_t e = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; e < ncounters; e += int64_t(gridDim.x) * blockDim.x)
+      counters[e] = 0u;
+  }
+  const bool dense = a.grad.row == a.n && (!MOM || a.momentum.row == a.n);
+  const int64_t rows = dense ? 1 : a.m, len = dense ? a.m * a.n : a.n;
+  const int64_t spans = (len + kSpan - 1) / kSpan;
+  const int step = a.vec ? 1 : 256;
   double sum = 0.0;
-  for (int64_t e = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; e < count; e += int64_t(gridDim.x) * blockDim.x) {
-    const int64_t i = e / a.n, j = e - i * a.n;
-    float u = strided_at(a.grad, a.grad_type, z, i, j);
-    if (a.momentum.p) {
+  for (int64_t t = blockIdx.x; t < rows * spans; t += gridDim.x) {
+    const int64_t i = t / spans, j = (t - i * spans) * kSpan + threadIdx.x * (a.vec ? 8 : 1);
+    const int count = j >= len ? 0 : int(min(int64_t(8), (len - j + step - 1) / step));
+    float g[8];
+    load_eight<V>(static_cast<const typename V::T *>(a.grad.p) + z * a.grad.batch + i * a.grad.row + j, a.vec, step, count, g);
+    if constexpr (MOM) {
       float *mp = const_cast<float *>(static_cast<const float *>(a.momentum.p)) + z * a.momentum.batch + i * a.momentum.row + j;
-      const float mom = __fmaf_rn(a.beta, *mp, u);
-      *mp = mom;
-      u = update_of(a, u, mom);
+      float mom[8];
+      load_eight<F32>(mp, a.vec, step, count, mom);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        mom[e] = __fmaf_rn(a.beta, mom[e], g[e]);
+        g[e] = update_of(a, g[e], mom[e]);
+      }
+      if (a.vec) {
+        if (count > 0) {
+          reinterpret_cast<float4 *>(mp)[0] = make_float4(mom[0], mom[1], mom[2], mom[3]);
+          reinterpret_cast<float4 *>(mp)[1] = make_float4(mom[4], mom[5], mom[6], mom[7]);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (e < count) mp[e * step] = mom[e];
+      }
     }
-    sum += double(u) * double(u);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum = fma(double(g[e]), double(g[e]), sum);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -105,12 +144,29 @@ k_muon_momentum(UpdateArgs a, double *__restrict__ parts) {
   }
 }
 
-// X_0 = S U / (|U| + eps) as hi + lo, s x w (transposed where m > n): 32 x 32
-// tiles through shared memory, so that both sides are read and written by rows.
+// Eight values of X as hi + lo, 16 bytes each.
+__device__ __forceinline__ void put_eight(__half *hi, __half *lo, const float (&f)[8]) {
+  uint4 h, l;
+  __half2 *hh = reinterpret_cast<__half2 *>(&h), *ll = reinterpret_cast<__half2 *>(&l);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    hh[e] = __floats2half2_rn(f[2 * e], f[2 * e + 1]);
+    const float2 b = __half22float2(hh[e]);
+    ll[e] = __floats2half2_rn(f[2 * e] - b.x, f[2 * e + 1] - b.y);
+  }
+  *reinterpret_cast<uint4 *>(hi) = h;
+  *reinterpret_cast<uint4 *>(lo) = l;
+}
+
+// X_0 = S U / (|U| + eps) as hi + lo, s x w (transposed where m > n): tiles of
+// 64 x 64 values, 16 per thread, through shared memory where the sides are
+// exchanged, so that both are read and written by rows. X's storage reaches
+// to a multiple of 64 columns, so its rows are written in whole vectors.
+template <class V, bool MOM>
 __global__ void __launch_bounds__(256)
 k_muon_scale(UpdateArgs a, const double *__restrict__ parts, int nparts, float eps, bool transposed,
              __half *__restrict__ hi, __half *__restrict__ lo, int64_t ld, int64_t batch_stride) {
-  __shared__ float tile[32][33];
+  __shared__ float tile[64][65];
   __shared__ double factor;  // fp64: 1 / |U| of a tiny update passes fp32's range
   const int64_t z = blockIdx.z;
   pdl_wait();
@@ -122,33 +178,49 @@ k_muon_scale(UpdateArgs a, const double *__restrict__ parts, int nparts, float e
     if (threadIdx.x == 0) factor = double(kScale) / (sqrt(sum) + double(eps));
   }
   __syncthreads();
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int64_t tiles_j = (a.n + 31) / 32, tiles = tiles_j * ((a.m + 31) / 32);
+  const double k = factor;
+  const int row = threadIdx.x >> 3, at = threadIdx.x & 7;  // 8 threads of 8 values per row, rows `row` and `row` + 32
+  const int step = a.vec ? 1 : 8, first = a.vec ? at * 8 : at;
+  const int64_t tiles_j = (a.n + 63) / 64, tiles = tiles_j * ((a.m + 63) / 64);
   for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
-    const int64_t i0 = t / tiles_j * 32, j0 = (t - t / tiles_j * tiles_j) * 32;
+    const int64_t i0 = t / tiles_j * 64, j0 = (t - t / tiles_j * tiles_j) * 64;
+    float u[2][8];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int64_t i = i0 + ty + 8 * k, j = j0 + tx;
-      if (i < a.m && j < a.n) {
-        float u = strided_at(a.grad, a.grad_type, z, i, j);
-        if (a.momentum.p)
-          u = update_of(a, u, static_cast<const float *>(a.momentum.p)[z * a.momentum.batch + i * a.momentum.row + j]);
-        tile[ty + 8 * k][tx] = float(double(u) * factor);
-      }
-    }
-    __syncthreads();
+    for (int q = 0; q < 2; ++q) {
+      const int64_t i = i0 + row + 32 * q, j = j0 + first;
+      const int count = i >= a.m || j >= a.n ? 0 : int(min(int64_t(8), (a.n - j + step - 1) / step));
+      load_eight<V>(static_cast<const typename V::T *>(a.grad.p) + z * a.grad.batch + i * a.grad.row + j, a.vec, step, count,
+                    u[q]);
+      if constexpr (MOM) {
+        float mom[8];
+        load_eight<F32>(static_cast<const float *>(a.momentum.p) + z * a.momentum.batch + i * a.momentum.row + j, a.vec, step,
+                        count, mom);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int64_t r = (transposed ? j0 : i0) + ty + 8 * k, c = (transposed ? i0 : j0) + tx;
-      if (r < (transposed ? a.n : a.m) && c < (transposed ? a.m : a.n)) {
-        const float v = transposed ? tile[tx][ty + 8 * k] : tile[ty + 8 * k][tx];
-        const __half h = __float2half_rn(v);
-        const int64_t at = z * batch_stride + r * ld + c;
-        hi[at] = h;
-        lo[at] = __float2half_rn(v - __half2float(h));
+        for (int e = 0; e < 8; ++e) u[q][e] = update_of(a, u[q][e], mom[e]);
       }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) u[q][e] = float(double(u[q][e]) * k);
     }
-    __syncthreads();
+    const bool through = transposed || !a.vec;
+    if (through) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) tile[row + 32 * q][first + e * step] = u[q][e];
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int r = row + 32 * q, c = at * 8;
+      if (through) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u[q][e] = transposed ? tile[c + e][r] : tile[r][c + e];
+      }
+      const int64_t rr = (transposed ? j0 : i0) + r, cc = (transposed ? i0 : j0) + c;
+      if (rr < (transposed ? a.n : a.m)) put_eight(hi + z * batch_stride + rr * ld + cc, lo + z * batch_stride + rr * ld + cc, u[q]);
+    }
+    if (through) __syncthreads();
   }
 }
 
@@ -176,19 +248,30 @@ struct FinishArgs {
   float keep, rate;
 };
 
-struct ProductArgs {
-  CUtensorMap a_hi, a_lo, b_hi, b_lo;  // the operands
-  int rows, cols, kblocks, batch;
-  int tiles_i, tiles_j, tiles;         // of one matrix
-  Pair in;                             // kSquare: A, kApply and kFinish: X
-  Pair out;
-  const float *diag_in;                // kSquare: A's diagonal, kApply and kFinish: B's
-  float *diag_out;                     // kGram: A's (scaled by S), kSquare: B's (not scaled)
+// How one kind of product is cut up: tiles of the result, each over `parts`
+// parts of the k-values.
+struct Cut {
+  int rows, cols, kblocks;
+  int tiles_j, tiles;  // of one matrix
+  int parts;
+};
+
+struct NsArgs {
+  CUtensorMap x_hi[2], x_lo[2], a_hi, a_lo, b_hi, b_lo;  // boxes of 64 x 64
+  Cut gram, square, apply;
+  int batch, steps;
+  Pair x[2], a, b;
+  float *diag_a, *diag_b;  // A's diagonal (scaled by S), B's (not scaled)
+  int64_t diag_ld;         // of the next matrix's
+  float *partial;          // gram.parts > 1: partial sums of its blocks, [block][part][32][32]
+  uint32_t *arrived;       // and how many parts of a block are there
+  uint32_t *barrier;       // blocks that finished a product
   FinishArgs fin;
   uint32_t *status;
 };
 
 constexpr int kEpilogueWarps = 8;
+constexpr int kThreads = 128 + 32 * kEpilogueWarps;
 constexpr int kFlush = 4;  // k-blocks of a SPLIT accumulation between two flushes
 
 template <int CG, int BN>
@@ -196,42 +279,54 @@ struct Layout {
   static constexpr int kA = 128 * 128;             // bytes of a CTA's A tile: 128 rows of 64 values
   static constexpr int kB = (BN / CG) * 128;       // and of its part of the B tile
   static constexpr int kStage = kA + kB;
-  static constexpr int kStages = CG == 2 ? 6 : BN == 256 ? 4 : BN == 128 ? 6 : 8;
-  static constexpr int kStaging = 32 * 33;         // floats of an epilogue warp's staging tile
+  static constexpr int kStages = 196608 / kStage;  // 192 KB: 4 to 8 stages
+  static constexpr int kStaging = 32 * 32;         // floats of an epilogue warp's staging tile
   static constexpr int kBytes = kStages * kStage + kEpilogueWarps * kStaging * 4 + 1024;  // 1,024: tile alignment
 };
 
-// Tile t: matrix, first row, first column. The symmetric products list only
-// tiles that reach the lower triangle, row of tiles by row of tiles.
+// Tile t of a matrix: its first row and column. The symmetric products list
+// only tiles that reach the lower triangle, row of tiles by row of tiles.
 template <int MODE, int TM, int BN>
-__device__ __forceinline__ void tile_at(const ProductArgs &g, int t, int &z, int &row, int &col) {
-  z = t / g.tiles;
-  t -= z * g.tiles;
+__device__ __forceinline__ void tile_at(const Cut &c, int t, int &row, int &col) {
   if constexpr (MODE == kGram || MODE == kSquare) {
     int i = 0;
     for (;; ++i) {
-      const int in_row = min((i * TM + TM - 1) / BN + 1, g.tiles_j);
+      const int in_row = min((i * TM + TM - 1) / BN + 1, c.tiles_j);
       if (t < in_row) break;
       t -= in_row;
     }
     row = i * TM;
     col = t * BN;
   } else {
-    const int i = t / g.tiles_j;
+    const int i = t / c.tiles_j;
     row = i * TM;
-    col = (t - i * g.tiles_j) * BN;
+    col = (t - i * c.tiles_j) * BN;
   }
 }
 
-__device__ __forceinline__ __half2 half2_at(const __half *p, int64_t at) {
-  return *reinterpret_cast<const __half2 *>(p + at);
+// Place of (r, c) in a staging tile: groups of four values of a row are moved
+// about by the row, so that a warp's 16-byte accesses along rows and its 4-byte
+// accesses down four rows at a time meet no bank twice.
+__device__ __forceinline__ int tile_place(int r, int c) {
+  return r * 32 + ((((c >> 2) ^ r ^ (r >> 2)) & 7) << 2) + (c & 3);
 }
-__device__ __forceinline__ void put_half2(const Pair &p, int64_t at, float f0, float f1, bool split) {
-  const __half2 h = __floats2half2_rn(f0, f1);
-  *reinterpret_cast<__half2 *>(p.hi + at) = h;
+
+// Four f16 values that other blocks may have written during the launch: from L2.
+__device__ __forceinline__ uint2 load_four(const __half *p) { return __ldcg(reinterpret_cast<const uint2 *>(p)); }
+__device__ __forceinline__ float4 open_four(uint2 v) {
+  const float2 a = __half22float2(*reinterpret_cast<__half2 *>(&v.x)), b = __half22float2(*reinterpret_cast<__half2 *>(&v.y));
+  return make_float4(a.x, a.y, b.x, b.y);
+}
+// Four values as hi, and with `split` lo, at the same offset of both.
+__device__ __forceinline__ void put_four(__half *hi, __half *lo, const float4 &f, bool split) {
+  const __half2 a = __floats2half2_rn(f.x, f.y), b = __floats2half2_rn(f.z, f.w);
+  *reinterpret_cast<uint2 *>(hi) =
+      make_uint2(*reinterpret_cast<const unsigned *>(&a), *reinterpret_cast<const unsigned *>(&b));
   if (split) {
-    const float2 b = __half22float2(h);
-    *reinterpret_cast<__half2 *>(p.lo + at) = __floats2half2_rn(f0 - b.x, f1 - b.y);
+    const float2 ra = __half22float2(a), rb = __half22float2(b);
+    const __half2 c = __floats2half2_rn(f.x - ra.x, f.y - ra.y), d = __floats2half2_rn(f.z - rb.x, f.w - rb.y);
+    *reinterpret_cast<uint2 *>(lo) =
+        make_uint2(*reinterpret_cast<const unsigned *>(&c), *reinterpret_cast<const unsigned *>(&d));
   }
 }
 __device__ __forceinline__ float load_typed(const void *p, int type, int64_t at) {
@@ -246,235 +341,275 @@ __device__ __forceinline__ void store_typed(void *p, int type, int64_t at, float
 }
 
 // The epilogue of a 32 x 32 block of the accumulator, staged by the warp in
-// `tile` (row stride 33). Everything else of the block is read and written two
-// rows at a time, 16 lanes of two values each, so that global accesses are
-// whole 32-byte sectors and shared-memory ones free of conflicts. All loads
-// of a block are issued before its first store. Rows are r0 .. r0 + 31,
-// columns c0 .. c0 + 31, both multiples of 32; storage reaches past the last
-// column to a multiple of 64, so columns need no guard.
+// `tile`. A turn handles four rows, eight lanes of four values each: global
+// accesses are whole 32-byte sectors, and the code is short (a block's
+// instructions run once, so that their fetches would cost more than the work:
+// an unrolled first version took 4,300 to 8,000 clocks a block). All loads
+// precede the first store. Rows are r0 .. r0 + 31, columns c0 .. c0 + 31, both
+// multiples of 32; storage reaches past the last column to a multiple of 64,
+// so columns need no guard.
 template <int MODE, bool SPLIT>
-__device__ __forceinline__ void finish_block(const ProductArgs &g, float *tile, int z, int r0, int c0, float dr_lane) {
-  const int lane = int(threadIdx.x) & 31, up = lane >> 4, pair = (lane & 15) * 2;
-  constexpr bool kReadsIn = MODE != kGram, kInLo = MODE == kApply || MODE == kFinish || SPLIT;
-  constexpr int kAtOnce = SPLIT ? 8 : 16;  // loads in flight; SPLIT needs registers for its sums
-  __half2 xh[kReadsIn ? kAtOnce : 1], xl[kReadsIn && kInLo ? kAtOnce : 1];
-  auto load = [&](int i0) {
-    if constexpr (kReadsIn) {
+__device__ __forceinline__ void finish_block(const NsArgs &g, int step, float *tile, int z, int r0, int c0,
+                                             float dr_lane) {
+  constexpr bool kSym = MODE == kGram || MODE == kSquare;
+  constexpr bool kInLo = !kSym || SPLIT;
+  const int lane = int(threadIdx.x) & 31, up = lane >> 3, four = (lane & 7) * 4;
+  const int rows = kSym ? g.square.rows : g.apply.rows;
+  const Pair &in = MODE == kSquare ? g.a : g.x[step & 1];
+  const Pair &out = MODE == kGram ? g.a : MODE == kSquare ? g.b : g.x[(step & 1) ^ 1];
+  const int turns = (min(32, rows - r0) - up + 3) >> 2;  // this lane's rows: r0 + up, r0 + up + 4, ...
+  uint2 xh[8], xl[8];
+  float4 dc;
+  if constexpr (MODE != kGram) {
+    const int64_t from = int64_t(z) * in.batch + int64_t(r0 + up) * in.ld + c0 + four;
+    const __half *h = in.hi + from, *l = in.lo + from;
 #pragma unroll
-      for (int i = 0; i < kAtOnce; ++i) {
-        const int r = r0 + 2 * (i0 + i) + up;
-        const int64_t at = int64_t(z) * g.in.batch + int64_t(r) * g.in.ld + c0 + pair;
-        const bool in = r < g.rows;
-        xh[i] = in ? half2_at(g.in.hi, at) : __half2();
-        if constexpr (kInLo) xl[i] = in ? half2_at(g.in.lo, at) : __half2();
+    for (int i = 0; i < 8; ++i) {
+      xh[i] = i < turns ? load_four(h) : make_uint2(0u, 0u);
+      if constexpr (kInLo) xl[i] = i < turns ? load_four(l) : make_uint2(0u, 0u);
+      h += 4 * in.ld;
+      l += 4 * in.ld;
+    }
+  }
+  if constexpr (MODE == kSquare) {
+    const float *d = g.diag_a + int64_t(z) * g.diag_ld + c0 + four;  // padded like the columns
+    dc = __ldcg(reinterpret_cast<const float4 *>(d));
+  }
+  const bool diagonal = kSym && r0 == c0;
+  if (diagonal) {
+    // The diagonal's value goes to its vector: (A A)_rr = acc + D_r^2. (Both
+    // triangles of the block are written as they were summed; they differ by
+    // the order of fp32 additions at most.)
+    const float acc = tile[tile_place(lane, lane)];
+    if (r0 + lane < rows) {
+      const int64_t at = int64_t(z) * g.diag_ld + r0 + lane;
+      if constexpr (MODE == kGram) g.diag_a[at] = acc * (1.0f / kScale);
+      else g.diag_b[at] = __fmaf_rn(kNsC / kScale, __fmaf_rn(dr_lane, dr_lane, acc), kNsB * dr_lane) * (1.0f / kScale);
+    }
+    __syncwarp();
+  }
+  const int64_t to = int64_t(z) * out.batch + int64_t(r0 + up) * out.ld + c0 + four;
+  __half *oh = out.hi + to, *ol = out.lo + to;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int rr = 4 * i + up;
+    float *at = tile + tile_place(rr, four);
+    float4 f = *reinterpret_cast<float4 *>(at);
+    if constexpr (MODE == kGram) {
+      f.x *= 1.0f / kScale;
+      f.y *= 1.0f / kScale;
+      f.z *= 1.0f / kScale;
+      f.w *= 1.0f / kScale;
+    } else {
+      float4 x = open_four(xh[i]);
+      if constexpr (kInLo) {
+        const float4 l = open_four(xl[i]);
+        x.x += l.x;
+        x.y += l.y;
+        x.z += l.z;
+        x.w += l.w;
       }
-    }
-  };
-  if constexpr (MODE == kGram || MODE == kSquare) {
-    const bool diagonal = r0 == c0;
-    float dc0 = 0.0f, dc1 = 0.0f;
-    if constexpr (MODE == kSquare) {
-      const float *d = g.diag_in + int64_t(z) * g.rows;
-      dc0 = c0 + pair < g.cols ? d[c0 + pair] : 0.0f;
-      dc1 = c0 + pair + 1 < g.cols ? d[c0 + pair + 1] : 0.0f;
-    }
-#pragma unroll 1
-    for (int i0 = 0; i0 < 16; i0 += kAtOnce) {
-    load(i0);
-#pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) {
-      const int rr = 2 * (i0 + i) + up, r = r0 + rr;
-      // a diagonal block takes its lower triangle on both sides
-      const bool swap0 = diagonal && pair > rr, swap1 = diagonal && pair + 1 > rr;
-      float f0 = tile[swap0 ? pair * 33 + rr : rr * 33 + pair];
-      float f1 = tile[swap1 ? (pair + 1) * 33 + rr : rr * 33 + pair + 1];
-      const bool d0 = diagonal && pair == rr, d1 = diagonal && pair + 1 == rr;
-      if constexpr (MODE == kGram) {
-        f0 *= 1.0f / kScale;
-        f1 *= 1.0f / kScale;
+      const float dr = __shfl_sync(0xffffffffu, dr_lane, rr);
+      if constexpr (MODE == kSquare) {  // off the diagonal (A A)_rc = acc + (D_r + D_c) O_rc
+        f.x = __fmaf_rn(kNsC / kScale, __fmaf_rn(dr + dc.x, x.x, f.x), kNsB * x.x);
+        f.y = __fmaf_rn(kNsC / kScale, __fmaf_rn(dr + dc.y, x.y, f.y), kNsB * x.y);
+        f.z = __fmaf_rn(kNsC / kScale, __fmaf_rn(dr + dc.z, x.z, f.z), kNsB * x.z);
+        f.w = __fmaf_rn(kNsC / kScale, __fmaf_rn(dr + dc.w, x.w, f.w), kNsB * x.w);
       } else {
-        const float dr = __shfl_sync(0xffffffffu, dr_lane, rr);
-        float2 x = __half22float2(xh[i]);
-        if constexpr (SPLIT) {
-          const float2 l = __half22float2(xl[i]);
-          x.x += l.x;
-          x.y += l.y;
-        }
-        // off the diagonal (A A)_rc = acc + (D_r + D_c) O_rc, on it acc + D_r^2
-        const float a0 = d0 ? dr : x.x, a1 = d1 ? dr : x.y;
-        f0 = __fmaf_rn(kNsC / kScale, __fmaf_rn(d0 ? dr : dr + dc0, a0, f0), kNsB * a0);
-        f1 = __fmaf_rn(kNsC / kScale, __fmaf_rn(d1 ? dr : dr + dc1, a1, f1), kNsB * a1);
-      }
-      if (d0 || d1) {
-        if (r < g.rows) g.diag_out[int64_t(z) * g.rows + r] = (d0 ? f0 : f1) * (MODE == kSquare ? 1.0f / kScale : 1.0f);
-        if (d0) f0 = 0.0f;
-        else f1 = 0.0f;
-      }
-      if (r < g.rows) put_half2(g.out, int64_t(z) * g.out.batch + int64_t(r) * g.out.ld + c0 + pair, f0, f1, SPLIT);
-      if (!diagonal) {
-        tile[rr * 33 + pair] = f0;
-        tile[rr * 33 + pair + 1] = f1;
+        const float k = kNsA + dr;
+        f.x = __fmaf_rn(k, x.x, f.x * (1.0f / kScale));
+        f.y = __fmaf_rn(k, x.y, f.y * (1.0f / kScale));
+        f.z = __fmaf_rn(k, x.z, f.z * (1.0f / kScale));
+        f.w = __fmaf_rn(k, x.w, f.w * (1.0f / kScale));
       }
     }
+    if (diagonal) {
+      if (rr == four) f.x = 0.0f;
+      if (rr == four + 1) f.y = 0.0f;
+      if (rr == four + 2) f.z = 0.0f;
+      if (rr == four + 3) f.w = 0.0f;
     }
+    if constexpr (MODE != kFinish) {
+      if (i < turns) put_four(oh, ol, f, kInLo);
+      oh += 4 * out.ld;
+      ol += 4 * out.ld;
+    }
+    if constexpr (kSym || MODE == kFinish) *reinterpret_cast<float4 *>(at) = f;
+  }
+  if constexpr (kSym) {
     if (!diagonal) {  // the mirror: rows c0 .., columns r0 ..
       __syncwarp();
+      const int64_t mirror = int64_t(z) * out.batch + int64_t(c0 + up) * out.ld + r0 + four;
+      oh = out.hi + mirror;
+      ol = out.lo + mirror;
 #pragma unroll 4
-      for (int i = 0; i < 16; ++i) {
-        const int cc = 2 * i + up;
-        put_half2(g.out, int64_t(z) * g.out.batch + int64_t(c0 + cc) * g.out.ld + r0 + pair, tile[pair * 33 + cc],
-                  tile[(pair + 1) * 33 + cc], SPLIT);
+      for (int i = 0; i < 8; ++i) {
+        const int cc = 4 * i + up;
+        put_four(oh, ol,
+                 make_float4(tile[tile_place(four, cc)], tile[tile_place(four + 1, cc)], tile[tile_place(four + 2, cc)],
+                             tile[tile_place(four + 3, cc)]),
+                 SPLIT);
+        oh += 4 * out.ld;
+        ol += 4 * out.ld;
       }
     }
-  } else {
+  }
+  if constexpr (MODE == kFinish) {
+    // by rows of the result, whichever way it lies: lane = its column
+    __syncwarp();
+    const FinishArgs &f = g.fin;
+    const int across = f.transposed ? r0 : c0, along = f.transposed ? c0 : r0;
+    const bool inside = across + lane < (f.transposed ? rows : g.apply.cols);
+    const int most = min(32, (f.transposed ? g.apply.cols : rows) - along);
+    const int64_t base = int64_t(z) * f.batch + int64_t(along) * f.row + across + lane;
 #pragma unroll 1
-    for (int i0 = 0; i0 < 16; i0 += kAtOnce) {
-    load(i0);
+    for (int e0 = 0; e0 < most; e0 += 8) {
+      float w[8];
+      if (f.update) {
 #pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) {
-      const int rr = 2 * (i0 + i) + up, r = r0 + rr;
-      const float f = kNsA + __shfl_sync(0xffffffffu, dr_lane, rr);
-      const float2 h = __half22float2(xh[i]), l = __half22float2(xl[i]);
-      const float f0 = __fmaf_rn(f, h.x + l.x, tile[rr * 33 + pair] * (1.0f / kScale));
-      const float f1 = __fmaf_rn(f, h.y + l.y, tile[rr * 33 + pair + 1] * (1.0f / kScale));
-      if constexpr (MODE == kApply) {
-        if (r < g.rows) put_half2(g.out, int64_t(z) * g.out.batch + int64_t(r) * g.out.ld + c0 + pair, f0, f1, true);
-      } else {
-        tile[rr * 33 + pair] = f0;
-        tile[rr * 33 + pair + 1] = f1;
+        for (int e = 0; e < 8; ++e)
+          w[e] = inside && e0 + e < most ? load_typed(f.out, f.type, base + (e0 + e) * f.row) : 0.0f;
       }
-    }
-    }
-    if constexpr (MODE == kFinish) {
-      // by rows of the result, whichever way it lies: lane = its column
-      __syncwarp();
-      const FinishArgs &f = g.fin;
-      const int across = f.transposed ? r0 : c0, along = f.transposed ? c0 : r0;
-      const bool in = across + lane < (f.transposed ? g.rows : g.cols);
-      const int most = min(32, (f.transposed ? g.cols : g.rows) - along);
-      const int64_t base = int64_t(z) * f.batch + int64_t(along) * f.row + across + lane;
-#pragma unroll 1
-      for (int e0 = 0; e0 < most; e0 += 8) {
-        float w[8];
-        if (f.update) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) w[e] = in && e0 + e < most ? load_typed(f.out, f.type, base + (e0 + e) * f.row) : 0.0f;
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float o = tile[f.transposed ? lane * 33 + e0 + e : (e0 + e) * 33 + lane] * (1.0f / kScale);
-          if (f.update) o = __fmaf_rn(-f.rate, o, f.keep * w[e]);
-          if (in && e0 + e < most) store_typed(f.out, f.type, base + (e0 + e) * f.row, o);
-        }
+      for (int e = 0; e < 8; ++e) {
+        float o = tile[f.transposed ? tile_place(lane, e0 + e) : tile_place(e0 + e, lane)] * (1.0f / kScale);
+        if (f.update) o = __fmaf_rn(-f.rate, o, f.keep * w[e]);
+        if (inside && e0 + e < most) store_typed(f.out, f.type, base + (e0 + e) * f.row, o);
       }
     }
   }
 }
 
-// One product over persistent tiles of (128 CG) x BN. Warp 0 loads operand
-// stages by TMA, warp 1 issues the matrix instructions, warps 4-11 turn finished
-// accumulators into the result while the next tile is computed (two
-// accumulators of BN columns in tensor memory; each epilogue warp has 32 rows
-// and every second block of 32 columns). Bound by the tensor cores for large
-// sides (each stage is 4 instructions of M x BN x 16).
+// A block's sum over its parts: each part leaves its own in `partial`, the one
+// that arrives last adds all of them in their order into `tile`. False: not last.
+__device__ __forceinline__ bool join_parts(const NsArgs &g, float *tile, int64_t block, int part) {
+  const int lane = int(threadIdx.x) & 31, parts = g.gram.parts;
+  auto at = [&](int i) { return reinterpret_cast<float4 *>(tile + tile_place(4 * i + (lane >> 3), (lane & 7) * 4)); };
+  float4 *mine = reinterpret_cast<float4 *>(g.partial + (block * parts + part) * 1024) + lane;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) __stcg(mine + 32 * i, *at(i));
+  __threadfence();
+  __syncwarp();
+  uint32_t before = 0;
+  if (lane == 0) before = atomicAdd(g.arrived + block, 1u);
+  before = __shfl_sync(0xffffffffu, before, 0);
+  if (before != uint32_t(parts - 1)) return false;
+  __threadfence();
+  if (lane == 0) g.arrived[block] = 0u;  // for the next step
+  const float4 *all = reinterpret_cast<const float4 *>(g.partial + block * parts * 1024) + lane;
+  float4 sum[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 2
+  for (int p = 0; p < parts; ++p) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float4 f = __ldcg(all + p * 256 + 32 * i);
+      sum[i].x += f.x;
+      sum[i].y += f.y;
+      sum[i].z += f.z;
+      sum[i].w += f.w;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) *at(i) = sum[i];
+  __syncwarp();
+  return true;
+}
+
+// What a thread carries from product to product: how often its role has used
+// the stages and the accumulators.
+struct Progress {
+  uint32_t stages = 0, sums = 0;
+};
+
+struct Shared {  // of a CTA
+  uint64_t full[8], empty[8], acc_full[2], acc_empty[2], drained;
+  uint32_t tmem;
+  volatile uint32_t given_up;
+};
+
+// One product, all tiles of this unit (a CTA, or with CG = 2 a pair of them).
+// Warp 0 loads operand stages by TMA, warp 1 issues the matrix instructions,
+// warps 4-11 turn finished accumulators into the result while the next one is
+// computed (two accumulators of BN columns in tensor memory; each epilogue
+// warp has 32 rows and every second block of 32 columns).
 //
 // SPLIT: the three products of hi and lo parts. The tensor core cuts its fp32
 // sums off instead of rounding them, which over thousands of k-values costs
 // more than the lo parts bring (measured: 3e-5 at 4,096), so a sum runs over
 // kFlush k-blocks only and the epilogue warps add those up in registers.
 template <int MODE, int CG, int BN, bool SPLIT>
-__global__ void __launch_bounds__(128 + 32 * kEpilogueWarps, 1) k_ns_product(const __grid_constant__ ProductArgs g) {
+__device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int step, Shared &sh, uint8_t *smem,
+                                            uint32_t rank, Progress &at) {
   using L = Layout<CG, BN>;
-  constexpr int kStages = L::kStages, kTM = 128 * CG, kBlocks = BN / 64;  // kBlocks: column blocks of an epilogue warp
-  constexpr bool kBMN = MODE == kApply || MODE == kFinish;                // B operand is X itself: n-contiguous
-  extern __shared__ uint8_t raw[];
-  __shared__ uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2], drained;
-  __shared__ uint32_t tmem_base;
-  __shared__ volatile uint32_t given_up;
-  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = CG == 2 ? cluster_rank() : 0u;
+  constexpr int kTM = 128 * CG, kBlocks = BN / 64;          // kBlocks: column blocks of an epilogue warp
+  constexpr bool kBMN = MODE == kApply || MODE == kFinish;  // the B operand is X itself: n-contiguous
+  constexpr uint32_t kStages = L::kStages;
+  const int warp = int(threadIdx.x) >> 5, lane = int(threadIdx.x) & 31;
   const int unit = int(blockIdx.x) / CG, units = int(gridDim.x) / CG;
-  const int total = g.tiles * g.batch;
-  const int kb = g.kblocks * (SPLIT ? 3 : 1);
-  const int per_sum = SPLIT ? kFlush : kb, sums = (kb + per_sum - 1) / per_sum;
+  const int parts = MODE == kGram ? c.parts : 1;
+  const int total = c.tiles * parts * g.batch;
+  const int kall = c.kblocks * (SPLIT ? 3 : 1);
+  // the k-blocks of part p: [kall p / parts, kall (p + 1) / parts)
+  auto k_from = [&](int p) { return MODE == kGram ? int(int64_t(kall) * p / parts) : p * kall; };
+  auto sum_end = [&](int k, int last) { return SPLIT ? min(last, k + kFlush) : last; };
 
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
-    }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], kEpilogueWarps * CG);
-    }
-    mbar_init(&drained, 1);
-    given_up = 0u;
-    prefetch_map(&g.a_hi);
-    prefetch_map(&g.b_hi);
-  }
-  if (warp == 2) tmem_alloc<CG>(&tmem_base, 2 * BN);
-  tmem_fence_before();
-  __syncthreads();
-  if constexpr (CG == 2) cluster_sync_all();
-  tmem_fence_after();
-  const uint32_t tmem = tmem_base;
-  pdl_trigger();
-  pdl_wait();
-
-  uint32_t issued = 0;  // stages loaded (warp 0)
   if (warp == 0) {
-    if (elect_one()) {
+    if (lane == 0) {
+      const CUtensorMap *xh = &g.x_hi[step & 1], *xl = &g.x_lo[step & 1];
+      const CUtensorMap *ah = MODE == kGram ? xh : MODE == kSquare ? &g.a_hi : &g.b_hi;
+      const CUtensorMap *al = MODE == kGram ? xl : MODE == kSquare ? &g.a_lo : &g.b_lo;
+      const CUtensorMap *bh = MODE == kSquare ? &g.a_hi : xh, *bl = MODE == kSquare ? &g.a_lo : xl;
       bool go = true;
       for (int t = unit; go && t < total; t += units) {
-        int z, row, col;
-        tile_at<MODE, kTM, BN>(g, t, z, row, col);
+        const int zt = t / parts, z = zt / c.tiles, part = t - zt * parts;
+        int row, col;
+        tile_at<MODE, kTM, BN>(c, zt - z * c.tiles, row, col);
         row += int(rank) * 128;
         col += int(rank) * (BN / CG);
-        for (int k = 0; k < kb; ++k) {
-          const uint32_t st = issued % kStages, use = issued / kStages;
-          if (!wait_or_give_up(&empty[st], (use & 1u) ^ 1u, &given_up)) {
+        for (int k = k_from(part), last = k_from(part + 1); k < last; ++k) {
+          const uint32_t st = at.stages % kStages, use = at.stages / kStages;
+          if (!wait_or_give_up(&sh.empty[st], (use & 1u) ^ 1u, &sh.given_up)) {
             go = false;
             break;
           }
-          // hi lo, lo hi, hi hi
-          const int seg = SPLIT ? k / g.kblocks : 2, k0 = (SPLIT ? k - seg * g.kblocks : k) * kTileK;
-          const CUtensorMap *ma = seg == 1 ? &g.a_lo : &g.a_hi, *mb = seg == 0 ? &g.b_lo : &g.b_hi;
+          const int seg = SPLIT ? k / c.kblocks : 2;  // hi lo, lo hi, hi hi
+          const int k0 = (SPLIT ? k - seg * c.kblocks : k) * kTileK;
+          const CUtensorMap *ma = seg == 1 ? al : ah, *mb = seg == 0 ? bl : bh;
           uint8_t *a = smem + st * L::kStage, *b = a + L::kA;
-          uint32_t bar = smem_u32(&full[st]);
+          uint32_t bar = smem_u32(&sh.full[st]);
           if constexpr (CG == 2) bar = mapa(bar, 0);
-          if (rank == 0) mbar_arrive_expect_tx(&full[st], CG * L::kStage);
-          tma_load<CG>(a, ma, k0, row, z, bar);
-          if constexpr (kBMN) {
+          if (rank == 0) mbar_arrive_expect_tx(&sh.full[st], CG * L::kStage);
 #pragma unroll
-            for (int q = 0; q < BN / CG / 64; ++q) tma_load<CG>(b + q * 8192, mb, col + q * 64, k0, z, bar);
-          } else {
-            tma_load<CG>(b, mb, k0, col, z, bar);
+          for (int q = 0; q < 2; ++q) tma_load<CG>(a + q * 8192, ma, k0, row + q * 64, z, bar);
+#pragma unroll
+          for (int q = 0; q < BN / CG / 64; ++q) {
+            if constexpr (kBMN) tma_load<CG>(b + q * 8192, mb, col + q * 64, k0, z, bar);
+            else tma_load<CG>(b + q * 8192, mb, k0, col + q * 64, z, bar);
           }
-          ++issued;
+          ++at.stages;
         }
       }
-      // the stages' last uses: no arrival is outstanding when the CTA ends
-      for (uint32_t i = issued > kStages ? issued - kStages : 0; go && i < issued; ++i)
-        go = wait_or_give_up(&empty[i % kStages], (i / kStages) & 1u, &given_up);
     }
+    __syncwarp();
   } else if (warp == 1 && rank == 0) {
-    if (elect_one()) {
+    if (lane == 0) {
       constexpr uint32_t kDesc = mma_desc(kTM, BN, kBMN);
-      uint32_t used = 0, filled = 0;
       bool go = true;
       for (int t = unit; go && t < total; t += units) {
-        for (int k = 0; go && k < kb; ++filled) {
-          const uint32_t acc = filled & 1u;
-          if (!wait_or_give_up(&acc_empty[acc], ((filled >> 1) & 1u) ^ 1u, &given_up)) {
+        const int part = t % parts, last = k_from(part + 1);
+        for (int k = k_from(part); go && k < last; ++at.sums) {
+          const uint32_t acc = at.sums & 1u;
+          if (!wait_or_give_up(&sh.acc_empty[acc], ((at.sums >> 1) & 1u) ^ 1u, &sh.given_up)) {
             go = false;
             break;
           }
           tmem_fence_after();
-          const int first = k, last = min(kb, k + per_sum);
-          for (; k < last; ++k, ++used) {
-            const uint32_t st = used % kStages;
-            if (!wait_or_give_up(&full[st], (used / kStages) & 1u, &given_up)) {
+          const int first = k, end = sum_end(k, last);
+          for (; k < end; ++k, ++at.stages) {
+            const uint32_t st = at.stages % kStages;
+            if (!wait_or_give_up(&sh.full[st], (at.stages / kStages) & 1u, &sh.given_up)) {
               go = false;
               break;
             }
@@ -483,104 +618,189 @@ __global__ void __launch_bounds__(128 + 32 * kEpilogueWarps, 1) k_ns_product(con
             const uint64_t da = operand_desc(a, 16), db = operand_desc(b, kBMN ? 8192 : 16);
 #pragma unroll
             for (int q = 0; q < kTileK / 16; ++q)  // 16 k-values: 32 bytes along a K-major row, 16 rows when MN-major
-              mma_f16<CG>(tmem + acc * BN, da + q * (32 >> 4), db + q * ((kBMN ? 2048 : 32) >> 4), kDesc,
+              mma_f16<CG>(sh.tmem + acc * BN, da + q * (32 >> 4), db + q * ((kBMN ? 2048 : 32) >> 4), kDesc,
                           k > first || q > 0);
-            mma_commit<CG>(&empty[st]);
+            mma_commit<CG>(&sh.empty[st]);
           }
-          if (go) mma_commit<CG>(&acc_full[acc]);
+          if (go) mma_commit<CG>(&sh.acc_full[acc]);
         }
       }
     }
+    __syncwarp();
   } else if (warp >= 4) {
     const int quad = warp & 3, side = (warp - 4) >> 2;
     float *tile = reinterpret_cast<float *>(smem + kStages * L::kStage) + (warp - 4) * L::kStaging;
-    uint32_t filled = 0;
+    const uint32_t tmem = sh.tmem + (uint32_t(quad * 32) << 16) + uint32_t(side * 32);
     bool go = true;
-    for (int t = unit; t < total; t += units) {
-      int z, row, col;
-      tile_at<MODE, kTM, BN>(g, t, z, row, col);
+    auto take = [&](uint32_t acc) {  // the accumulator is full; false: gave up
+      go = __all_sync(0xffffffffu, wait_or_give_up(&sh.acc_full[acc], (at.sums >> 1) & 1u, &sh.given_up));
+      tmem_fence_after();
+      return go;
+    };
+    auto give = [&](uint32_t acc) {
+      tmem_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        uint32_t bar = smem_u32(&sh.acc_empty[acc]);
+        if constexpr (CG == 2) bar = mapa(bar, 0);
+        mbar_arrive_cluster(bar);
+      }
+      ++at.sums;
+    };
+    for (int t = unit; go && t < total; t += units) {
+      const int zt = t / parts, z = zt / c.tiles, part = t - zt * parts;
+      int row, col;
+      tile_at<MODE, kTM, BN>(c, zt - z * c.tiles, row, col);
       const int r0 = row + int(rank) * 128 + quad * 32;
       float dr = 0.0f;
-      if (MODE != kGram && r0 + lane < g.rows) dr = g.diag_in[int64_t(z) * g.rows + r0 + lane];
-      auto block = [&](int b) { return col + (2 * b + side) * 32; };
-      auto wanted = [&](int c0) {
-        return r0 < g.rows && c0 < g.cols && (MODE == kApply || MODE == kFinish || c0 <= r0);
+      if (MODE != kGram && r0 + lane < c.rows)
+        dr = __ldcg((MODE == kSquare ? g.diag_a : g.diag_b) + int64_t(z) * g.diag_ld + r0 + lane);
+      auto wanted = [&](int b) {
+        const int c0 = col + (2 * b + side) * 32;
+        return r0 < c.rows && c0 < c.cols && (kBMN || c0 <= r0);
       };
-      auto address = [&](uint32_t acc, int b) {
-        return tmem + acc * BN + uint32_t((2 * b + side) * 32) + (uint32_t(quad * 32) << 16);
-      };
-      auto stage = [&](const float (&v)[32]) {
+      auto finish = [&](int b, const float(&v)[32]) {
+        const int c0 = col + (2 * b + side) * 32;
         __syncwarp();
 #pragma unroll
-        for (int e = 0; e < 32; ++e) tile[lane * 33 + e] = v[e];
+        for (int e = 0; e < 32; e += 4)
+          *reinterpret_cast<float4 *>(tile + tile_place(lane, e)) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
         __syncwarp();
-      };
-      auto take = [&](uint32_t acc) {  // an accumulator is full; false: gave up
-        const bool ok = wait_or_give_up(&acc_full[acc], (filled >> 1) & 1u, &given_up);
-        go = __all_sync(0xffffffffu, ok);
-        tmem_fence_after();
-        return go;
-      };
-      auto give = [&](uint32_t acc) {
-        tmem_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          uint32_t bar = smem_u32(&acc_empty[acc]);
-          if constexpr (CG == 2) bar = mapa(bar, 0);
-          mbar_arrive_cluster(bar);
+        if (MODE == kGram && parts > 1) {
+          constexpr int kPerTile = (kTM / 32) * (BN / 32);
+          const int64_t block = int64_t(zt) * kPerTile + (int(rank) * 4 + quad) * (BN / 32) + 2 * b + side;
+          if (!join_parts(g, tile, block, part)) return;
         }
-        ++filled;
+        finish_block<MODE, SPLIT>(g, step, tile, z, r0, c0, dr);
       };
       if constexpr (SPLIT) {
+        static_assert(kBlocks <= 2, "the sums stay in registers");
         float v[kBlocks][32];
-        for (int s = 0; s < sums; ++s) {
-          const uint32_t acc = filled & 1u;
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[b][e] = 0.0f;
+        }
+        for (int k = k_from(part), last = k_from(part + 1); k < last; k = sum_end(k, last)) {
+          const uint32_t acc = at.sums & 1u;
           if (!take(acc)) break;
 #pragma unroll
           for (int b = 0; b < kBlocks; ++b) {
             float f[32];
-            tmem_load32(address(acc, b), f);
+            tmem_load32(tmem + acc * BN + uint32_t(b * 64), f);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) v[b][e] = s == 0 ? f[e] : v[b][e] + f[e];
+            for (int e = 0; e < 32; ++e) v[b][e] += f[e];
           }
           give(acc);
         }
         if (!go) break;
-#pragma unroll
+#pragma unroll 1
         for (int b = 0; b < kBlocks; ++b) {
-          if (!wanted(block(b))) continue;
-          stage(v[b]);
-          finish_block<MODE, SPLIT>(g, tile, z, r0, block(b), dr);
+          if (!wanted(b)) break;
+          float f[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) f[e] = kBlocks > 1 && b > 0 ? v[kBlocks - 1][e] : v[0][e];
+          finish(b, f);
         }
       } else {
-        const uint32_t acc = filled & 1u;
+        const uint32_t acc = at.sums & 1u;
         if (!take(acc)) break;
 #pragma unroll 1
         for (int b = 0; b < kBlocks; ++b) {
-          if (!wanted(block(b))) break;
+          if (!wanted(b)) break;
           float v[32];
           __syncwarp();
-          tmem_load32(address(acc, b), v);
-          stage(v);
-          finish_block<MODE, SPLIT>(g, tile, z, r0, block(b), dr);
+          tmem_load32(tmem + acc * BN + uint32_t(b * 64), v);
+          finish(b, v);
         }
         give(acc);
       }
     }
+    asm volatile("fence.proxy.async.global;" ::: "memory");  // what this thread stored, for every block's TMA
+  }
+}
+
+// All blocks have finished the product (their stores are visible to every
+// block's loads); false: a wait gave up somewhere.
+__device__ __forceinline__ bool grid_wait(uint32_t *barrier, uint32_t target, Shared &sh) {
+  __syncthreads();
+  if (gridDim.x > 1) {
+    if (threadIdx.x == 0) {
+      asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(barrier) : "memory");
+      const long long start = clock64();
+      for (uint32_t n = 0;; ++n) {
+        uint32_t seen;
+        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(barrier) : "memory");
+        if (seen >= target) break;
+        if (sh.given_up || n >= kWaitTries || clock64() - start > kWaitClocks) {
+          sh.given_up = 1u;
+          break;
+        }
+      }
+    }
+    __syncthreads();
+  }
+  return sh.given_up == 0u;
+}
+
+// The whole iteration in one cooperative launch: 3 products a step, a barrier
+// over the grid after each. Launches cost more than the products of small
+// matrices, and for large ones the tensor cores are the bound either way.
+template <int CG, int BN, bool SPLIT>
+__global__ void __launch_bounds__(kThreads, 1) k_newton_schulz(const __grid_constant__ NsArgs g) {
+  using L = Layout<CG, BN>;
+  extern __shared__ uint8_t raw[];
+  __shared__ Shared sh;
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  const int warp = int(threadIdx.x) >> 5;
+  const uint32_t rank = CG == 2 ? cluster_rank() : 0u;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < L::kStages; ++i) {
+      mbar_init(&sh.full[i], 1);
+      mbar_init(&sh.empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.acc_full[i], 1);
+      mbar_init(&sh.acc_empty[i], kEpilogueWarps * CG);
+    }
+    mbar_init(&sh.drained, 1);
+    sh.given_up = 0u;
+  }
+  if (warp == 2) tmem_alloc<CG>(&sh.tmem, 2 * BN);
+  tmem_fence_before();
+  __syncthreads();
+  if constexpr (CG == 2) cluster_sync_all();
+  tmem_fence_after();
+
+  Progress at;
+  uint32_t target = 0;
+  for (int step = 0; step < g.steps; ++step) {
+    run_product<kGram, CG, BN, SPLIT>(g, g.gram, step, sh, smem, rank, at);
+    if (!grid_wait(g.barrier, target += gridDim.x, sh)) break;
+    run_product<kSquare, CG, BN, SPLIT>(g, g.square, step, sh, smem, rank, at);
+    if (!grid_wait(g.barrier, target += gridDim.x, sh)) break;
+    if (step + 1 == g.steps) {
+      run_product<kFinish, CG, BN, SPLIT>(g, g.apply, step, sh, smem, rank, at);
+      break;
+    }
+    run_product<kApply, CG, BN, SPLIT>(g, g.apply, step, sh, smem, rank, at);
+    if (!grid_wait(g.barrier, target += gridDim.x, sh)) break;
   }
 
-  __syncwarp();
-  if (given_up) {
-    // Leave nothing in flight: the loads that warp 0 issued and the matrix
-    // instructions of warp 1; then report.
-    if (warp == 1 && rank == 0 && elect_one()) {
-      mma_commit<CG>(&drained);
-      wait_for(&drained, 0u, nullptr);
-    }
-    if (warp == 0 && rank == 0) {
-      const uint32_t last = __reduce_max_sync(0xffffffffu, issued);
-      for (uint32_t i = last > kStages ? last - kStages : 0; i < last; ++i)
-        wait_for(&full[i % kStages], (i / kStages) & 1u, nullptr);
+  // No arrival or copy is outstanding when the CTA ends: the stages' last uses
+  // have been read, or, where a wait gave up, the copies have landed and the
+  // matrix instructions are done. Then that is reported.
+  __syncthreads();
+  const bool failed = sh.given_up != 0u;
+  const uint32_t issued = __reduce_max_sync(0xffffffffu, at.stages);
+  if (warp == 0 && (!failed || rank == 0)) {
+    for (uint32_t i = issued > L::kStages ? issued - L::kStages : 0; i < issued; ++i)
+      wait_for(failed ? &sh.full[i % L::kStages] : &sh.empty[i % L::kStages], (i / L::kStages) & 1u, nullptr);
+  }
+  if (failed) {
+    if (threadIdx.x == 32 && rank == 0) {
+      mma_commit<CG>(&sh.drained);
+      wait_for(&sh.drained, 0u, nullptr);
     }
     if (threadIdx.x == 0) {
       *reinterpret_cast<volatile uint32_t *>(g.status) = 1u;
@@ -590,7 +810,7 @@ __global__ void __launch_bounds__(128 + 32 * kEpilogueWarps, 1) k_ns_product(con
   tmem_fence_before();
   __syncthreads();
   if constexpr (CG == 2) cluster_sync_all();
-  if (warp == 2) tmem_free<CG>(tmem, 2 * BN);
+  if (warp == 2) tmem_free<CG>(sh.tmem, 2 * BN);
 }
 
 // ---------------------------------------------------------------------------
@@ -630,12 +850,12 @@ EncodeTiled encode_tiled() {
   return fn;
 }
 
-// Boxes of 64 columns x `box` rows of a batch of rows x cols f16 matrices.
-CUtensorMap matrix_map(const __half *p, int64_t rows, int64_t cols, int64_t ld, int64_t batch, int box) {
+// Boxes of 64 x 64 of a batch of rows x cols f16 matrices.
+CUtensorMap matrix_map(const __half *p, int64_t rows, int64_t cols, int64_t ld, int64_t batch) {
   CUtensorMap map;
   const cuuint64_t dims[3] = {cuuint64_t(cols), cuuint64_t(rows), cuuint64_t(batch)};
   const cuuint64_t strides[2] = {cuuint64_t(ld) * 2, cuuint64_t(ld) * 2 * cuuint64_t(rows)};
-  const cuuint32_t boxes[3] = {64, cuuint32_t(box), 1}, steps[3] = {1, 1, 1};
+  const cuuint32_t boxes[3] = {64, 64, 1}, steps[3] = {1, 1, 1};
   const CUresult r = encode_tiled()(&map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<__half *>(p), dims, strides,
                                     boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -643,16 +863,47 @@ CUtensorMap matrix_map(const __half *p, int64_t rows, int64_t cols, int64_t ld, 
   return map;
 }
 
+bool split_products(int32_t out_type) { return out_type != SE_BFLOAT16; }
+
+int64_t tile_count(bool symmetric, int64_t rows, int64_t cols, int tm, int bn) {
+  const int64_t ti = (rows + tm - 1) / tm, tj = (cols + bn - 1) / bn;
+  if (!symmetric) return ti * tj;
+  int64_t n = 0;
+  for (int64_t i = 0; i < ti; ++i) n += std::min<int64_t>((i * tm + tm - 1) / bn + 1, tj);
+  return n;
+}
+
+// The tile of a call (the same for its three products), and in how many parts
+// the k-values of X X^T are cut.
+constexpr int kUnits = 148;  // blocks that are expected to run at once
+struct Plan {
+  int cg, bn, parts;
+};
+
+Plan plan_for(int64_t batch, int64_t s, int64_t w, bool split) {
+  Plan p{1, 64, 1};
+  if (!split && tile_count(true, s, s, 128, 256) * batch >= kUnits) p.bn = 256;
+  else if (tile_count(true, s, s, 128, 128) * batch >= kUnits / 4) p.bn = 128;
+  const int64_t tiles = tile_count(true, s, s, 128 * p.cg, p.bn) * batch;
+  const int64_t kall = (w + kTileK - 1) / kTileK * (split ? 3 : 1);
+  p.parts = int(std::max<int64_t>(1, std::min<int64_t>(kUnits / p.cg / std::max<int64_t>(tiles, 1), kall / 8)));
+  return p;
+}
+
 // The workspace of a call: X twice (a product reads one and writes the other),
-// A, B, their diagonals, and the partial norms.
+// A, B, their diagonals, the partial norms, the partial sums of X X^T, and the
+// counters (zeroed by the first kernel).
 struct Space {
-  double *parts;
+  double *norms;
   Pair x[2], a, b;
-  float *diag_a, *diag_b;
+  float *diag_a, *diag_b, *partial;
+  uint32_t *counters;  // the barrier, then one per block of X X^T
+  int64_t ncounters;
   size_t bytes;
 };
 
 Space muon_space(void *base, int64_t batch, int64_t s, int64_t w, bool split) {
+  const Plan p = plan_for(batch, s, w, split);
   Space sp{};
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -662,160 +913,142 @@ Space muon_space(void *base, int64_t batch, int64_t s, int64_t w, bool split) {
   };
   const int64_t ldx = (w + 63) / 64 * 64, lda = (s + 63) / 64 * 64;
   auto pair = [&](int64_t ld, bool lo) {
-    Pair p{};
-    p.ld = ld;
-    p.batch = s * ld;
-    p.hi = reinterpret_cast<__half *>(take(size_t(batch) * s * ld * 2));
-    p.lo = lo ? reinterpret_cast<__half *>(take(size_t(batch) * s * ld * 2)) : p.hi;
-    return p;
+    Pair q{};
+    q.ld = ld;
+    q.batch = s * ld;
+    q.hi = reinterpret_cast<__half *>(take(size_t(batch) * s * ld * 2));
+    q.lo = lo ? reinterpret_cast<__half *>(take(size_t(batch) * s * ld * 2)) : q.hi;
+    return q;
   };
-  sp.parts = reinterpret_cast<double *>(take(size_t(batch) * kNormParts * sizeof(double)));
+  sp.norms = reinterpret_cast<double *>(take(size_t(batch) * kNormParts * sizeof(double)));
   sp.x[0] = pair(ldx, true);
   sp.x[1] = pair(ldx, true);
   sp.a = pair(lda, split);
   sp.b = pair(lda, split);
-  sp.diag_a = reinterpret_cast<float *>(take(size_t(batch) * s * sizeof(float)));
-  sp.diag_b = reinterpret_cast<float *>(take(size_t(batch) * s * sizeof(float)));
+  sp.diag_a = reinterpret_cast<float *>(take(size_t(batch) * lda * sizeof(float)));
+  sp.diag_b = reinterpret_cast<float *>(take(size_t(batch) * lda * sizeof(float)));
+  const int64_t values = p.parts > 1 ? tile_count(true, s, s, 128 * p.cg, p.bn) * batch * 128 * p.cg * p.bn : 0;
+  sp.partial = reinterpret_cast<float *>(take(size_t(values) * p.parts * sizeof(float)));
+  sp.ncounters = 1 + values / 1024;
+  sp.counters = reinterpret_cast<uint32_t *>(take(size_t(sp.ncounters) * sizeof(uint32_t)));
   sp.bytes = at;
   return sp;
 }
 
-bool split_products(int32_t out_type) { return out_type != SE_BFLOAT16; }
-
-template <int MODE, int CG, int BN, bool SPLIT>
-void launch_product(ProductArgs &g, int sms, cudaStream_t st) {
+template <int CG, int BN, bool SPLIT>
+void launch_newton_schulz(const NsArgs &g, int64_t units, int sms, cudaStream_t st) {
   using L = Layout<CG, BN>;
-  auto *kernel = k_ns_product<MODE, CG, BN, SPLIT>;
+  auto *kernel = k_newton_schulz<CG, BN, SPLIT>;
   allow_dynamic_smem(kernel, L::kBytes);
-  const int64_t units = std::min<int64_t>(int64_t(g.tiles) * g.batch, sms / CG);
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(units * CG));
-  cfg.blockDim = dim3(128 + 32 * kEpilogueWarps);
+  cfg.gridDim = dim3(unsigned(std::min<int64_t>(units, sms / CG) * CG));
+  cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = L::kBytes;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[0].id = cudaLaunchAttributeCooperative;  // the blocks wait for one another
+  attr[0].val.cooperative = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = CG;
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = CG == 2 ? 2 : 1;
-  cuda_check(cudaLaunchKernelEx(&cfg, kernel, g), "k_ns_product");
-  launched("k_ns_product");
-}
-
-int64_t product_tiles(bool symmetric, int64_t rows, int64_t cols, int tm, int bn, int64_t &ti, int64_t &tj) {
-  ti = (rows + tm - 1) / tm;
-  tj = (cols + bn - 1) / bn;
-  if (!symmetric) return ti * tj;
-  int64_t n = 0;
-  for (int64_t i = 0; i < ti; ++i) n += std::min<int64_t>((i * tm + tm - 1) / bn + 1, tj);
-  return n;
-}
-
-// One product of `op_a` (rows x depth) and `op_b` (K-major: cols x depth;
-// for X itself depth x cols).
-template <int MODE>
-void product(ProductArgs &g, const Pair &op_a, const Pair &op_b, int64_t rows, int64_t cols, int64_t depth,
-             int64_t batch, bool split, int sms, cudaStream_t st) {
-  constexpr bool kSym = MODE == kGram || MODE == kSquare, kBMN = !kSym;
-  g.rows = int(rows);
-  g.cols = int(cols);
-  g.kblocks = int((depth + kTileK - 1) / kTileK);
-  g.batch = int(batch);
-  int64_t ti = 0, tj = 0;
-  auto go = [&](auto cg, auto bn, auto sp) {
-    constexpr int CG = decltype(cg)::value, BN = decltype(bn)::value;
-    constexpr bool kSplit = decltype(sp)::value;
-    const int64_t tiles = product_tiles(kSym, rows, cols, 128 * CG, BN, ti, tj);
-    if (tiles * batch > 0x7fffffff) throw std::invalid_argument("batch x m x n is too large");
-    g.tiles_i = int(ti);
-    g.tiles_j = int(tj);
-    g.tiles = int(tiles);
-    const int box_b = kBMN ? 64 : BN / CG;
-    auto map_b = [&](const __half *p) {
-      return kBMN ? matrix_map(p, depth, cols, op_b.ld, batch, box_b) : matrix_map(p, cols, depth, op_b.ld, batch, box_b);
-    };
-    g.a_hi = matrix_map(op_a.hi, rows, depth, op_a.ld, batch, 128);
-    g.b_hi = map_b(op_b.hi);
-    if (kSplit) {
-      g.a_lo = matrix_map(op_a.lo, rows, depth, op_a.ld, batch, 128);
-      g.b_lo = map_b(op_b.lo);
-    }
-    launch_product<MODE, CG, BN, kSplit>(g, sms, st);
-  };
-  using std::integral_constant;
-  const bool wide = product_tiles(kSym, rows, cols, 128, 256, ti, tj) * batch >= sms;
-  const bool medium = product_tiles(kSym, rows, cols, 128, 128, ti, tj) * batch >= sms / 2;
-  const integral_constant<int, 1> one{};
-  if (split) {
-    if (medium) go(one, integral_constant<int, 128>{}, std::true_type{});
-    else go(one, integral_constant<int, 64>{}, std::true_type{});
-  } else if (wide) {
-    go(one, integral_constant<int, 256>{}, std::false_type{});
-  } else if (medium) {
-    go(one, integral_constant<int, 128>{}, std::false_type{});
-  } else {
-    go(one, integral_constant<int, 64>{}, std::false_type{});
-  }
+  cuda_check(cudaLaunchKernelEx(&cfg, kernel, g), "k_newton_schulz");
+  launched("k_newton_schulz");
 }
 
 // The orthogonalised update of `u` into `fin`.
-void orthogonalise(const UpdateArgs &u, int64_t batch, int steps, float eps, bool split, FinishArgs fin, void *workspace,
+void orthogonalise(UpdateArgs u, int grad_type, int64_t batch, int steps, float eps, bool split, FinishArgs fin, void *workspace,
                    size_t workspace_bytes, int device, cudaStream_t st) {
+  const size_t gb = value_bytes(grad_type);
+  u.vec = u.n % 8 == 0 && aligned16(u.grad.p) && u.grad.row * gb % 16 == 0 && (batch == 1 || u.grad.batch * gb % 16 == 0) &&
+          (u.momentum.p == nullptr ||
+           (aligned16(u.momentum.p) && u.momentum.row % 4 == 0 && (batch == 1 || u.momentum.batch % 4 == 0)));
   const bool transposed = u.m > u.n;
   const int64_t s = std::min(u.m, u.n), w = std::max(u.m, u.n);
-  Space sp = muon_space(workspace, batch, s, w, split);
+  const Plan plan = plan_for(batch, s, w, split);
+  const Space sp = muon_space(workspace, batch, s, w, split);
   if (workspace_bytes < sp.bytes) throw std::invalid_argument("workspace is smaller than se_muon_workspace asks for");
+  const int tm = 128 * plan.cg;
+  auto cut = [&](bool symmetric, int64_t cols, int64_t depth, int parts) {
+    const int64_t tiles = tile_count(symmetric, s, cols, tm, plan.bn);
+    if (tiles * parts * batch > 0x7fffffff) throw std::invalid_argument("batch x m x n is too large");
+    return Cut{int(s), int(cols), int((depth + kTileK - 1) / kTileK), int((cols + plan.bn - 1) / plan.bn), int(tiles), parts};
+  };
+  NsArgs g{};
+  g.gram = cut(true, s, w, plan.parts);
+  g.square = cut(true, s, s, 1);
+  g.apply = cut(false, w, s, 1);
   const int sms = sm_count(device);
-  uint32_t *status = ns_status(device);
-  if (*static_cast<volatile uint32_t *>(status) != 0u) {
-    *static_cast<volatile uint32_t *>(status) = 0u;
+  g.status = ns_status(device);
+  if (*static_cast<volatile uint32_t *>(g.status) != 0u) {
+    *static_cast<volatile uint32_t *>(g.status) = 0u;
     throw Error(SE_ERR_RUNTIME, "an earlier orthogonalisation on cuda:" + std::to_string(device) +
                                     " gave up waiting for its copies; its results are not valid");
   }
-  const int64_t count = u.m * u.n;
-  const int nparts = int(std::min<int64_t>(kNormParts, (count + 1023) / 1024));
-  k_muon_momentum<<<dim3(unsigned(nparts), unsigned(batch)), 256, 0, st>>>(u, sp.parts);
-  launched("k_muon_momentum");
-  {
-    const int64_t tiles = ((u.m + 31) / 32) * ((u.n + 31) / 32);
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(unsigned(std::min<int64_t>(tiles, 1024)), 1, unsigned(batch));
-    cfg.blockDim = dim3(256);
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    cuda_check(cudaLaunchKernelEx(&cfg, k_muon_scale, u, static_cast<const double *>(sp.parts), nparts, eps, transposed,
-                                  sp.x[0].hi, sp.x[0].lo, sp.x[0].ld, sp.x[0].batch),
-               "k_muon_scale");
-    launched("k_muon_scale");
+  const bool dense = u.grad.row == u.n && (u.momentum.p == nullptr || u.momentum.row == u.n);
+  const int64_t spans = dense ? (u.m * u.n + kSpan - 1) / kSpan : u.m * ((u.n + kSpan - 1) / kSpan);
+  const int nparts = int(std::min<int64_t>(std::min<int64_t>(kNormParts, spans), std::max<int64_t>(1, 4 * sms / batch)));
+  const int64_t tiles64 = ((u.m + 63) / 64) * ((u.n + 63) / 64);
+  dispatch_value(grad_type, [&](auto tag) {
+    using V = decltype(tag);
+    auto go = [&](auto mom) {
+      constexpr bool kMom = decltype(mom)::value;
+      k_muon_momentum<V, kMom><<<dim3(unsigned(nparts), unsigned(batch)), 256, 0, st>>>(u, sp.norms, sp.counters, sp.ncounters);
+      launched("k_muon_momentum");
+      cudaLaunchConfig_t cfg{};
+      cfg.gridDim = dim3(unsigned(std::min<int64_t>(tiles64, 8 * sms)), 1, unsigned(batch));
+      cfg.blockDim = dim3(256);
+      cfg.stream = st;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      attr[0].val.programmaticStreamSerializationAllowed = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      cuda_check(cudaLaunchKernelEx(&cfg, k_muon_scale<V, kMom>, u, static_cast<const double *>(sp.norms), nparts, eps,
+                                    transposed, sp.x[0].hi, sp.x[0].lo, sp.x[0].ld, sp.x[0].batch),
+                 "k_muon_scale");
+      launched("k_muon_scale");
+    };
+    if (u.momentum.p) go(std::true_type{});
+    else go(std::false_type{});
+  });
+
+  for (int k = 0; k < 2; ++k) {
+    g.x[k] = sp.x[k];
+    g.x_hi[k] = matrix_map(sp.x[k].hi, s, w, sp.x[k].ld, batch);
+    if (split) g.x_lo[k] = matrix_map(sp.x[k].lo, s, w, sp.x[k].ld, batch);
   }
+  g.a = sp.a;
+  g.b = sp.b;
+  g.a_hi = matrix_map(sp.a.hi, s, s, sp.a.ld, batch);
+  g.b_hi = matrix_map(sp.b.hi, s, s, sp.b.ld, batch);
+  if (split) {
+    g.a_lo = matrix_map(sp.a.lo, s, s, sp.a.ld, batch);
+    g.b_lo = matrix_map(sp.b.lo, s, s, sp.b.ld, batch);
+  }
+  g.batch = int(batch);
+  g.steps = steps;
+  g.diag_a = sp.diag_a;
+  g.diag_b = sp.diag_b;
+  g.diag_ld = sp.a.ld;
+  g.partial = sp.partial;
+  g.barrier = sp.counters;
+  g.arrived = sp.counters + 1;
   fin.transposed = transposed;
-  for (int k = 0; k < steps; ++k) {
-    const Pair &x = sp.x[k & 1], &next = sp.x[(k & 1) ^ 1];
-    ProductArgs g{};
-    g.status = status;
-    g.out = sp.a;
-    g.diag_out = sp.diag_a;
-    product<kGram>(g, x, x, s, s, w, batch, split, sms, st);
-    g.in = sp.a;
-    g.out = sp.b;
-    g.diag_in = sp.diag_a;
-    g.diag_out = sp.diag_b;
-    product<kSquare>(g, sp.a, sp.a, s, s, s, batch, split, sms, st);
-    g.in = x;
-    g.out = next;
-    g.diag_in = sp.diag_b;
-    g.diag_out = nullptr;
-    g.fin = fin;
-    if (k + 1 < steps) product<kApply>(g, sp.b, x, s, w, s, batch, split, sms, st);
-    else product<kFinish>(g, sp.b, x, s, w, s, batch, split, sms, st);
+  g.fin = fin;
+  const int64_t units = std::max<int64_t>(int64_t(g.gram.tiles) * plan.parts, g.apply.tiles) * batch;
+  const int form = plan.cg * 1000 + plan.bn * 2 + (split ? 1 : 0);
+  switch (form) {
+    case 2512: launch_newton_schulz<2, 256, false>(g, units, sms, st); break;
+    case 2256: launch_newton_schulz<2, 128, false>(g, units, sms, st); break;
+    case 2257: launch_newton_schulz<2, 128, true>(g, units, sms, st); break;
+    case 1512: launch_newton_schulz<1, 256, false>(g, units, sms, st); break;
+    case 1256: launch_newton_schulz<1, 128, false>(g, units, sms, st); break;
+    case 1257: launch_newton_schulz<1, 128, true>(g, units, sms, st); break;
+    case 1128: launch_newton_schulz<1, 64, false>(g, units, sms, st); break;
+    default: launch_newton_schulz<1, 64, true>(g, units, sms, st); break;
   }
 }
 
@@ -863,7 +1096,6 @@ extern "C" int se_orthogonalize(int32_t dtype, const void *update, size_t batch,
     if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0) throw std::invalid_argument("workspace must be 256-byte aligned");
     UpdateArgs u{};
     u.grad = {update, batch_stride, row_stride};
-    u.grad_type = dtype;
     u.m = m;
     u.n = n;
     FinishArgs fin{};
@@ -871,7 +1103,7 @@ extern "C" int se_orthogonalize(int32_t dtype, const void *update, size_t batch,
     fin.type = dtype;
     fin.row = n;
     fin.batch = m * n;
-    orthogonalise(u, int64_t(batch), steps, eps, split_products(dtype), fin, workspace, workspace_bytes, device,
+    orthogonalise(u, dtype, int64_t(batch), steps, eps, split_products(dtype), fin, workspace, workspace_bytes, device,
                   static_cast<cudaStream_t>(stream));
   });
 }
@@ -901,7 +1133,6 @@ extern "C" int se_muon_step(int32_t weight_dtype, int32_t grad_dtype, void *weig
     if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0) throw std::invalid_argument("workspace must be 256-byte aligned");
     UpdateArgs u{};
     u.grad = {grad, grad_batch_stride, grad_row_stride};
-    u.grad_type = grad_dtype;
     u.momentum = {momentum, momentum_batch_stride, momentum_row_stride};
     u.beta = float(beta);
     u.nesterov = nesterov != 0;
@@ -915,7 +1146,7 @@ extern "C" int se_muon_step(int32_t weight_dtype, int32_t grad_dtype, void *weig
     fin.batch = weight_batch_stride;
     fin.keep = float(1.0 - lr * weight_decay);
     fin.rate = float(lr * scale);
-    orthogonalise(u, int64_t(batch), steps, eps, split_products(weight_dtype), fin, workspace, workspace_bytes, device,
+    orthogonalise(u, grad_dtype, int64_t(batch), steps, eps, split_products(weight_dtype), fin, workspace, workspace_bytes, device,
                   static_cast<cudaStream_t>(stream));
   });
 }

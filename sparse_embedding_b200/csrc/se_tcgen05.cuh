@@ -11,30 +11,21 @@
 
 namespace se_gpu {
 
-// A wait gives up after this time, or this many tries (each may suspend the
-// thread for a while). In a healthy launch a wait takes microseconds.
-constexpr uint64_t kWaitNanoseconds = 4000000000ull;
-constexpr uint32_t kWaitTries = 1u << 26;
+// A wait gives up after this many clocks (seconds), or this many tries (each
+// may suspend the thread for a while). In a healthy launch a wait takes
+// microseconds. (Clocks, since a read of the nanosecond timer is slow enough
+// to show in every wait.)
+constexpr long long kWaitClocks = 8000000000ll;
+constexpr uint32_t kWaitTries = 1u << 30;
 
-__device__ __forceinline__ uint64_t global_ns() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
 __device__ __forceinline__ bool wait_for(uint64_t *bar, uint32_t parity, const volatile uint32_t *given_up) {
   if (mbar_try_wait(bar, parity)) return true;
-  const uint64_t start = global_ns();
-  for (uint32_t n = 0; n < kWaitTries && global_ns() - start < kWaitNanoseconds; ++n) {
+  const long long start = clock64();
+  for (uint32_t n = 0; n < kWaitTries; ++n) {
     if (mbar_try_wait(bar, parity)) return true;
-    if (given_up != nullptr && *given_up) return false;
+    if ((given_up != nullptr && *given_up) || clock64() - start > kWaitClocks) return false;
   }
   return false;
-}
-
-__device__ __forceinline__ bool elect_one() {
-  uint32_t p;
-  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
-  return p != 0u;
 }
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
