@@ -340,41 +340,52 @@ __device__ __forceinline__ void store_typed(void *p, int type, int64_t at, float
   else static_cast<__nv_bfloat16 *>(p)[at] = __float2bfloat16_rn(v);
 }
 
+// What the epilogue of a 32 x 32 block reads besides the accumulator: A (kSquare)
+// or X (kApply, kFinish) and A's diagonal over the columns. A warp asks for it
+// before it waits for the accumulator, or while it still works on the block
+// before, so that the latency is hidden.
+template <int MODE, bool SPLIT>
+struct BlockInput {
+  static constexpr bool kLo = MODE == kApply || MODE == kFinish || SPLIT;
+  uint2 hi[8], lo[8];
+  float4 diag;
+  __device__ __forceinline__ void load(const NsArgs &g, int step, int z, int r0, int c0) {
+    if constexpr (MODE != kGram) {
+      const int lane = int(threadIdx.x) & 31, up = lane >> 3, four = (lane & 7) * 4;
+      const Pair &in = MODE == kSquare ? g.a : g.x[step & 1];
+      const int turns = (min(32, g.apply.rows - r0) - up + 3) >> 2;
+      const int64_t from = int64_t(z) * in.batch + int64_t(r0 + up) * in.ld + c0 + four;
+      const __half *h = in.hi + from, *l = in.lo + from;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        hi[i] = i < turns ? load_four(h) : make_uint2(0u, 0u);
+        if constexpr (kLo) lo[i] = i < turns ? load_four(l) : make_uint2(0u, 0u);
+        h += 4 * in.ld;
+        l += 4 * in.ld;
+      }
+      if constexpr (MODE == kSquare)  // padded like the columns
+        diag = __ldcg(reinterpret_cast<const float4 *>(g.diag_a + int64_t(z) * g.diag_ld + c0 + four));
+    }
+  }
+};
+
 // The epilogue of a 32 x 32 block of the accumulator, staged by the warp in
 // `tile`. A turn handles four rows, eight lanes of four values each: global
 // accesses are whole 32-byte sectors, and the code is short (a block's
 // instructions run once, so that their fetches would cost more than the work:
-// an unrolled first version took 4,300 to 8,000 clocks a block). All loads
-// precede the first store. Rows are r0 .. r0 + 31, columns c0 .. c0 + 31, both
-// multiples of 32; storage reaches past the last column to a multiple of 64,
-// so columns need no guard.
-template <int MODE, bool SPLIT>
+// an unrolled first version took 4,300 to 8,000 clocks a block). `next` is
+// called where the block's input has been used. Rows are r0 .. r0 + 31,
+// columns c0 .. c0 + 31, both multiples of 32; storage reaches past the last
+// column to a multiple of 64, so columns need no guard.
+template <int MODE, bool SPLIT, class Next>
 __device__ __forceinline__ void finish_block(const NsArgs &g, int step, float *tile, int z, int r0, int c0,
-                                             float dr_lane) {
+                                             float dr_lane, const BlockInput<MODE, SPLIT> &input, Next &&next) {
   constexpr bool kSym = MODE == kGram || MODE == kSquare;
-  constexpr bool kInLo = !kSym || SPLIT;
+  constexpr bool kInLo = BlockInput<MODE, SPLIT>::kLo;
   const int lane = int(threadIdx.x) & 31, up = lane >> 3, four = (lane & 7) * 4;
-  const int rows = kSym ? g.square.rows : g.apply.rows;
-  const Pair &in = MODE == kSquare ? g.a : g.x[step & 1];
+  const int rows = g.apply.rows;
   const Pair &out = MODE == kGram ? g.a : MODE == kSquare ? g.b : g.x[(step & 1) ^ 1];
   const int turns = (min(32, rows - r0) - up + 3) >> 2;  // this lane's rows: r0 + up, r0 + up + 4, ...
-  uint2 xh[8], xl[8];
-  float4 dc;
-  if constexpr (MODE != kGram) {
-    const int64_t from = int64_t(z) * in.batch + int64_t(r0 + up) * in.ld + c0 + four;
-    const __half *h = in.hi + from, *l = in.lo + from;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      xh[i] = i < turns ? load_four(h) : make_uint2(0u, 0u);
-      if constexpr (kInLo) xl[i] = i < turns ? load_four(l) : make_uint2(0u, 0u);
-      h += 4 * in.ld;
-      l += 4 * in.ld;
-    }
-  }
-  if constexpr (MODE == kSquare) {
-    const float *d = g.diag_a + int64_t(z) * g.diag_ld + c0 + four;  // padded like the columns
-    dc = __ldcg(reinterpret_cast<const float4 *>(d));
-  }
   const bool diagonal = kSym && r0 == c0;
   if (diagonal) {
     // The diagonal's value goes to its vector: (A A)_rr = acc + D_r^2. (Both
@@ -401,9 +412,9 @@ __device__ __forceinline__ void finish_block(const NsArgs &g, int step, float *t
       f.z *= 1.0f / kScale;
       f.w *= 1.0f / kScale;
     } else {
-      float4 x = open_four(xh[i]);
+      float4 x = open_four(input.hi[i]);
       if constexpr (kInLo) {
-        const float4 l = open_four(xl[i]);
+        const float4 l = open_four(input.lo[i]);
         x.x += l.x;
         x.y += l.y;
         x.z += l.z;
@@ -411,10 +422,10 @@ __device__ __forceinline__ void finish_block(const NsArgs &g, int step, float *t
       }
       const float dr = __shfl_sync(0xffffffffu, dr_lane, rr);
       if constexpr (MODE == kSquare) {  // off the diagonal (A A)_rc = acc + (D_r + D_c) O_rc
-        f.x = __fmaf_rn(kNsC / kScale, __fmaf_rn(dr + dc.x, x.x, f.x), kNsB * x.x);
-        f.y = __fmaf_rn(kNsC / kScale, __fmaf_rn(dr + dc.y, x.y, f.y), kNsB * x.y);
-        f.z = __fmaf_rn(kNsC / kScale, __fmaf_rn(dr + dc.z, x.z, f.z), kNsB * x.z);
-        f.w = __fmaf_rn(kNsC / kScale, __fmaf_rn(dr + dc.w, x.w, f.w), kNsB * x.w);
+        f.x = __fmaf_rn(kNsC / kScale, __fmaf_rn(dr + input.diag.x, x.x, f.x), kNsB * x.x);
+        f.y = __fmaf_rn(kNsC / kScale, __fmaf_rn(dr + input.diag.y, x.y, f.y), kNsB * x.y);
+        f.z = __fmaf_rn(kNsC / kScale, __fmaf_rn(dr + input.diag.z, x.z, f.z), kNsB * x.z);
+        f.w = __fmaf_rn(kNsC / kScale, __fmaf_rn(dr + input.diag.w, x.w, f.w), kNsB * x.w);
       } else {
         const float k = kNsA + dr;
         f.x = __fmaf_rn(k, x.x, f.x * (1.0f / kScale));
@@ -436,6 +447,7 @@ __device__ __forceinline__ void finish_block(const NsArgs &g, int step, float *t
     }
     if constexpr (kSym || MODE == kFinish) *reinterpret_cast<float4 *>(at) = f;
   }
+  next();
   if constexpr (kSym) {
     if (!diagonal) {  // the mirror: rows c0 .., columns r0 ..
       __syncwarp();
@@ -517,10 +529,26 @@ __device__ __forceinline__ bool join_parts(const NsArgs &g, float *tile, int64_t
   return true;
 }
 
-// What a thread carries from product to product: how often its role has used
-// the stages and the accumulators.
+// A ring of N buffers: the one in turn and how often the ring went round (its
+// parity is the phase to wait for).
+template <uint32_t N>
+struct Ring {
+  uint32_t at = 0, parity = 0;
+  __device__ __forceinline__ void advance() {
+    if (++at == N) {
+      at = 0;
+      parity ^= 1u;
+    }
+  }
+};
+
+// What a thread carries from product to product: where its role stands in the
+// operand stages and in the accumulators, and the stages it has loaded.
+template <uint32_t STAGES>
 struct Progress {
-  uint32_t stages = 0, sums = 0;
+  Ring<STAGES> stage;
+  Ring<2> sum;
+  uint32_t loaded = 0;
 };
 
 struct Shared {  // of a CTA
@@ -541,7 +569,7 @@ struct Shared {  // of a CTA
 // kFlush k-blocks only and the epilogue warps add those up in registers.
 template <int MODE, int CG, int BN, bool SPLIT>
 __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int step, Shared &sh, uint8_t *smem,
-                                            uint32_t rank, Progress &at) {
+                                            uint32_t rank, Progress<Layout<CG, BN>::kStages> &at) {
   using L = Layout<CG, BN>;
   constexpr int kTM = 128 * CG, kBlocks = BN / 64;          // kBlocks: column blocks of an epilogue warp
   constexpr bool kBMN = MODE == kApply || MODE == kFinish;  // the B operand is X itself: n-contiguous
@@ -556,7 +584,7 @@ __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int s
   auto sum_end = [&](int k, int last) { return SPLIT ? min(last, k + kFlush) : last; };
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       const CUtensorMap *xh = &g.x_hi[step & 1], *xl = &g.x_lo[step & 1];
       const CUtensorMap *ah = MODE == kGram ? xh : MODE == kSquare ? &g.a_hi : &g.b_hi;
       const CUtensorMap *al = MODE == kGram ? xl : MODE == kSquare ? &g.a_lo : &g.b_lo;
@@ -569,12 +597,12 @@ __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int s
         row += int(rank) * 128;
         col += int(rank) * (BN / CG);
         for (int k = k_from(part), last = k_from(part + 1); k < last; ++k) {
-          const uint32_t st = at.stages % kStages, use = at.stages / kStages;
-          if (!wait_or_give_up(&sh.empty[st], (use & 1u) ^ 1u, &sh.given_up)) {
+          const uint32_t st = at.stage.at;
+          if (!wait_or_give_up(&sh.empty[st], at.stage.parity ^ 1u, &sh.given_up)) {
             go = false;
             break;
           }
-          const int seg = SPLIT ? k / c.kblocks : 2;  // hi lo, lo hi, hi hi
+          const int seg = SPLIT ? (k >= c.kblocks) + (k >= 2 * c.kblocks) : 2;  // hi lo, lo hi, hi hi
           const int k0 = (SPLIT ? k - seg * c.kblocks : k) * kTileK;
           const CUtensorMap *ma = seg == 1 ? al : ah, *mb = seg == 0 ? bl : bh;
           uint8_t *a = smem + st * L::kStage, *b = a + L::kA;
@@ -588,41 +616,51 @@ __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int s
             if constexpr (kBMN) tma_load<CG>(b + q * 8192, mb, col + q * 64, k0, z, bar);
             else tma_load<CG>(b + q * 8192, mb, k0, col + q * 64, z, bar);
           }
-          ++at.stages;
+          at.stage.advance();
+          ++at.loaded;
         }
       }
     }
     __syncwarp();
   } else if (warp == 1 && rank == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
+      // One elected thread, so that operands of the matrix instructions are known
+      // to be uniform: chosen as lane 0, with the descriptors computed for each
+      // instruction, the thread needed 560 to 620 clocks a stage whatever the
+      // tile (now 515 at 128 x 256, 305 at 128 x 128; the arithmetic takes 512
+      // and 256).
       constexpr uint32_t kDesc = mma_desc(kTM, BN, kBMN);
+      constexpr uint32_t kStepA = 32 >> 4, kStepB = (kBMN ? 2048 : 32) >> 4;  // 16 k-values: along a row, or 16 rows
+      const uint32_t first_a = smem_u32(smem), tmem = sh.tmem;
+      const uint64_t desc_a = operand_desc(first_a, 16), desc_b = operand_desc(first_a + L::kA, kBMN ? 8192 : 16);
       bool go = true;
       for (int t = unit; go && t < total; t += units) {
-        const int part = t % parts, last = k_from(part + 1);
-        for (int k = k_from(part); go && k < last; ++at.sums) {
-          const uint32_t acc = at.sums & 1u;
-          if (!wait_or_give_up(&sh.acc_empty[acc], ((at.sums >> 1) & 1u) ^ 1u, &sh.given_up)) {
+        const int part = parts > 1 ? t % parts : 0, last = k_from(part + 1);
+        for (int k = k_from(part); go && k < last; at.sum.advance()) {
+          const uint32_t acc = tmem + at.sum.at * BN;
+          if (!wait_or_give_up(&sh.acc_empty[at.sum.at], at.sum.parity ^ 1u, &sh.given_up)) {
             go = false;
             break;
           }
           tmem_fence_after();
-          const int first = k, end = sum_end(k, last);
-          for (; k < end; ++k, ++at.stages) {
-            const uint32_t st = at.stages % kStages;
-            if (!wait_or_give_up(&sh.full[st], (at.stages / kStages) & 1u, &sh.given_up)) {
+          const int end = sum_end(k, last);
+          bool add = false;
+          for (; k < end; ++k) {
+            const uint32_t st = at.stage.at;
+            if (!wait_or_give_up(&sh.full[st], at.stage.parity, &sh.given_up)) {
               go = false;
               break;
             }
             tmem_fence_after();
-            const uint32_t a = smem_u32(smem + st * L::kStage), b = a + L::kA;
-            const uint64_t da = operand_desc(a, 16), db = operand_desc(b, kBMN ? 8192 : 16);
+            const uint64_t da = desc_a + st * (L::kStage >> 4), db = desc_b + st * (L::kStage >> 4);
+            mma_f16<CG>(acc, da, db, kDesc, add);
+            add = true;
 #pragma unroll
-            for (int q = 0; q < kTileK / 16; ++q)  // 16 k-values: 32 bytes along a K-major row, 16 rows when MN-major
-              mma_f16<CG>(sh.tmem + acc * BN, da + q * (32 >> 4), db + q * ((kBMN ? 2048 : 32) >> 4), kDesc,
-                          k > first || q > 0);
+            for (int q = 1; q < kTileK / 16; ++q) mma_f16<CG>(acc, da + q * kStepA, db + q * kStepB, kDesc, true);
             mma_commit<CG>(&sh.empty[st]);
+            at.stage.advance();
           }
-          if (go) mma_commit<CG>(&sh.acc_full[acc]);
+          if (go) mma_commit<CG>(&sh.acc_full[at.sum.at]);
         }
       }
     }
@@ -632,20 +670,20 @@ __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int s
     float *tile = reinterpret_cast<float *>(smem + kStages * L::kStage) + (warp - 4) * L::kStaging;
     const uint32_t tmem = sh.tmem + (uint32_t(quad * 32) << 16) + uint32_t(side * 32);
     bool go = true;
-    auto take = [&](uint32_t acc) {  // the accumulator is full; false: gave up
-      go = __all_sync(0xffffffffu, wait_or_give_up(&sh.acc_full[acc], (at.sums >> 1) & 1u, &sh.given_up));
+    auto take = [&] {  // the accumulator in turn is full; false: gave up
+      go = __all_sync(0xffffffffu, wait_or_give_up(&sh.acc_full[at.sum.at], at.sum.parity, &sh.given_up));
       tmem_fence_after();
       return go;
     };
-    auto give = [&](uint32_t acc) {
+    auto give = [&] {
       tmem_fence_before();
       __syncwarp();
       if (lane == 0) {
-        uint32_t bar = smem_u32(&sh.acc_empty[acc]);
+        uint32_t bar = smem_u32(&sh.acc_empty[at.sum.at]);
         if constexpr (CG == 2) bar = mapa(bar, 0);
         mbar_arrive_cluster(bar);
       }
-      ++at.sums;
+      at.sum.advance();
     };
     for (int t = unit; go && t < total; t += units) {
       const int zt = t / parts, z = zt / c.tiles, part = t - zt * parts;
@@ -655,12 +693,16 @@ __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int s
       float dr = 0.0f;
       if (MODE != kGram && r0 + lane < c.rows)
         dr = __ldcg((MODE == kSquare ? g.diag_a : g.diag_b) + int64_t(z) * g.diag_ld + r0 + lane);
+      auto column = [&](int b) { return col + (2 * b + side) * 32; };
       auto wanted = [&](int b) {
-        const int c0 = col + (2 * b + side) * 32;
-        return r0 < c.rows && c0 < c.cols && (kBMN || c0 <= r0);
+        return b < kBlocks && r0 < c.rows && column(b) < c.cols && (kBMN || column(b) <= r0);
       };
+      BlockInput<MODE, SPLIT> input;
+      auto ask = [&](int b) {
+        if (wanted(b)) input.load(g, step, z, r0, column(b));
+      };
+      ask(0);
       auto finish = [&](int b, const float(&v)[32]) {
-        const int c0 = col + (2 * b + side) * 32;
         __syncwarp();
 #pragma unroll
         for (int e = 0; e < 32; e += 4)
@@ -671,7 +713,7 @@ __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int s
           const int64_t block = int64_t(zt) * kPerTile + (int(rank) * 4 + quad) * (BN / 32) + 2 * b + side;
           if (!join_parts(g, tile, block, part)) return;
         }
-        finish_block<MODE, SPLIT>(g, step, tile, z, r0, c0, dr);
+        finish_block<MODE, SPLIT>(g, step, tile, z, r0, column(b), dr, input, [&] { ask(b + 1); });
       };
       if constexpr (SPLIT) {
         static_assert(kBlocks <= 2, "the sums stay in registers");
@@ -682,16 +724,15 @@ __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int s
           for (int e = 0; e < 32; ++e) v[b][e] = 0.0f;
         }
         for (int k = k_from(part), last = k_from(part + 1); k < last; k = sum_end(k, last)) {
-          const uint32_t acc = at.sums & 1u;
-          if (!take(acc)) break;
+          if (!take()) break;
 #pragma unroll
           for (int b = 0; b < kBlocks; ++b) {
             float f[32];
-            tmem_load32(tmem + acc * BN + uint32_t(b * 64), f);
+            tmem_load32(tmem + at.sum.at * BN + uint32_t(b * 64), f);
 #pragma unroll
             for (int e = 0; e < 32; ++e) v[b][e] += f[e];
           }
-          give(acc);
+          give();
         }
         if (!go) break;
 #pragma unroll 1
@@ -703,17 +744,16 @@ __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int s
           finish(b, f);
         }
       } else {
-        const uint32_t acc = at.sums & 1u;
-        if (!take(acc)) break;
+        if (!take()) break;
 #pragma unroll 1
         for (int b = 0; b < kBlocks; ++b) {
           if (!wanted(b)) break;
           float v[32];
           __syncwarp();
-          tmem_load32(tmem + acc * BN + uint32_t(b * 64), v);
+          tmem_load32(tmem + at.sum.at * BN + uint32_t(b * 64), v);
           finish(b, v);
         }
-        give(acc);
+        give();
       }
     }
     asm volatile("fence.proxy.async.global;" ::: "memory");  // what this thread stored, for every block's TMA
@@ -772,7 +812,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_newton_schulz(const __grid_cons
   if constexpr (CG == 2) cluster_sync_all();
   tmem_fence_after();
 
-  Progress at;
+  Progress<L::kStages> at;
   uint32_t target = 0;
   for (int step = 0; step < g.steps; ++step) {
     run_product<kGram, CG, BN, SPLIT>(g, g.gram, step, sh, smem, rank, at);
@@ -792,7 +832,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_newton_schulz(const __grid_cons
   // matrix instructions are done. Then that is reported.
   __syncthreads();
   const bool failed = sh.given_up != 0u;
-  const uint32_t issued = __reduce_max_sync(0xffffffffu, at.stages);
+  const uint32_t issued = __reduce_max_sync(0xffffffffu, at.loaded);
   if (warp == 0 && (!failed || rank == 0)) {
     for (uint32_t i = issued > L::kStages ? issued - L::kStages : 0; i < issued; ++i)
       wait_for(failed ? &sh.full[i % L::kStages] : &sh.empty[i % L::kStages], (i / L::kStages) & 1u, nullptr);

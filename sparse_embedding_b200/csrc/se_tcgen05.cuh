@@ -27,6 +27,12 @@ __device__ __forceinline__ bool wait_for(uint64_t *bar, uint32_t parity, const v
   }
   return false;
 }
+// One lane of the converged warp, the same one every time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+  return p != 0u;
+}
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -89,13 +95,11 @@ __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint
   if constexpr (CG == 1) {
     asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
                  " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(desc),
-                 "r"(uint32_t(add))
-                 : "memory");
+                 "r"(uint32_t(add)));
   } else {
     asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
                  " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(desc),
-                 "r"(uint32_t(add))
-                 : "memory");
+                 "r"(uint32_t(add)));
   }
 }
 // Arrives on the barrier (in both CTAs with CG = 2) when the thread's matrix instructions are done.
