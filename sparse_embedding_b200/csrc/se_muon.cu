@@ -274,14 +274,19 @@ constexpr int kEpilogueWarps = 8;
 constexpr int kThreads = 128 + 32 * kEpilogueWarps;
 constexpr int kFlush = 4;  // k-blocks of a SPLIT accumulation between two flushes
 
-template <int CG, int BN>
+// Shared memory of a CTA: operand stages, then the epilogue warps' staging
+// tiles (SPLIT stages all blocks of an accumulator at once: its sums would not
+// leave registers for the epilogue).
+template <int CG, int BN, bool SPLIT>
 struct Layout {
-  static constexpr int kA = 128 * 128;             // bytes of a CTA's A tile: 128 rows of 64 values
-  static constexpr int kB = (BN / CG) * 128;       // and of its part of the B tile
+  static constexpr int kA = 128 * 128;        // bytes of a CTA's A tile: 128 rows of 64 values
+  static constexpr int kB = (BN / CG) * 128;  // and of its part of the B tile
   static constexpr int kStage = kA + kB;
-  static constexpr int kStages = 196608 / kStage;  // 192 KB: 4 to 8 stages
-  static constexpr int kStaging = 32 * 32;         // floats of an epilogue warp's staging tile
-  static constexpr int kBytes = kStages * kStage + kEpilogueWarps * kStaging * 4 + 1024;  // 1,024: tile alignment
+  static constexpr int kStaging = (SPLIT ? BN / 64 : 1) * 32 * 32;  // floats of a warp
+  static constexpr int kStagingBytes = kEpilogueWarps * kStaging * 4;
+  static constexpr int kRoom = 232448 - 1024 - 512 - kStagingBytes;  // 1,024: tile alignment; 512: static variables
+  static constexpr int kStages = kRoom / kStage < 8 ? kRoom / kStage : 8;
+  static constexpr int kBytes = kStages * kStage + kStagingBytes + 1024;
 };
 
 // Tile t of a matrix: its first row and column. The symmetric products list
@@ -399,13 +404,14 @@ __device__ __forceinline__ void finish_block(const NsArgs &g, int step, float *t
     }
     __syncwarp();
   }
-  const int64_t to = int64_t(z) * out.batch + int64_t(r0 + up) * out.ld + c0 + four;
-  __half *oh = out.hi + to, *ol = out.lo + to;
+  // Reads of the staged block before its writes: in turn, each would wait for the other.
+  float4 v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = *reinterpret_cast<const float4 *>(tile + tile_place(4 * i + up, four));
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int rr = 4 * i + up;
-    float *at = tile + tile_place(rr, four);
-    float4 f = *reinterpret_cast<float4 *>(at);
+    float4 &f = v[i];
     if constexpr (MODE == kGram) {
       f.x *= 1.0f / kScale;
       f.y *= 1.0f / kScale;
@@ -440,27 +446,37 @@ __device__ __forceinline__ void finish_block(const NsArgs &g, int step, float *t
       if (rr == four + 2) f.z = 0.0f;
       if (rr == four + 3) f.w = 0.0f;
     }
-    if constexpr (MODE != kFinish) {
-      if (i < turns) put_four(oh, ol, f, kInLo);
+  }
+  next();
+  if constexpr (MODE != kFinish) {
+    const int64_t to = int64_t(z) * out.batch + int64_t(r0 + up) * out.ld + c0 + four;
+    __half *oh = out.hi + to, *ol = out.lo + to;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i < turns) put_four(oh, ol, v[i], kInLo);
       oh += 4 * out.ld;
       ol += 4 * out.ld;
     }
-    if constexpr (kSym || MODE == kFinish) *reinterpret_cast<float4 *>(at) = f;
   }
-  next();
+  if ((kSym && !diagonal) || MODE == kFinish) {
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) *reinterpret_cast<float4 *>(tile + tile_place(4 * i + up, four)) = v[i];
+    __syncwarp();
+  }
   if constexpr (kSym) {
     if (!diagonal) {  // the mirror: rows c0 .., columns r0 ..
-      __syncwarp();
-      const int64_t mirror = int64_t(z) * out.batch + int64_t(c0 + up) * out.ld + r0 + four;
-      oh = out.hi + mirror;
-      ol = out.lo + mirror;
-#pragma unroll 4
+#pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int cc = 4 * i + up;
-        put_four(oh, ol,
-                 make_float4(tile[tile_place(four, cc)], tile[tile_place(four + 1, cc)], tile[tile_place(four + 2, cc)],
-                             tile[tile_place(four + 3, cc)]),
-                 SPLIT);
+        v[i] = make_float4(tile[tile_place(four, cc)], tile[tile_place(four + 1, cc)], tile[tile_place(four + 2, cc)],
+                           tile[tile_place(four + 3, cc)]);
+      }
+      const int64_t to = int64_t(z) * out.batch + int64_t(c0 + up) * out.ld + r0 + four;
+      __half *oh = out.hi + to, *ol = out.lo + to;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        put_four(oh, ol, v[i], SPLIT);
         oh += 4 * out.ld;
         ol += 4 * out.ld;
       }
@@ -468,7 +484,6 @@ __device__ __forceinline__ void finish_block(const NsArgs &g, int step, float *t
   }
   if constexpr (MODE == kFinish) {
     // by rows of the result, whichever way it lies: lane = its column
-    __syncwarp();
     const FinishArgs &f = g.fin;
     const int across = f.transposed ? r0 : c0, along = f.transposed ? c0 : r0;
     const bool inside = across + lane < (f.transposed ? rows : g.apply.cols);
@@ -569,8 +584,8 @@ struct Shared {  // of a CTA
 // kFlush k-blocks only and the epilogue warps add those up in registers.
 template <int MODE, int CG, int BN, bool SPLIT>
 __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int step, Shared &sh, uint8_t *smem,
-                                            uint32_t rank, Progress<Layout<CG, BN>::kStages> &at) {
-  using L = Layout<CG, BN>;
+                                            uint32_t rank, Progress<Layout<CG, BN, SPLIT>::kStages> &at) {
+  using L = Layout<CG, BN, SPLIT>;
   constexpr int kTM = 128 * CG, kBlocks = BN / 64;          // kBlocks: column blocks of an epilogue warp
   constexpr bool kBMN = MODE == kApply || MODE == kFinish;  // the B operand is X itself: n-contiguous
   constexpr uint32_t kStages = L::kStages;
@@ -701,19 +716,19 @@ __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int s
       auto ask = [&](int b) {
         if (wanted(b)) input.load(g, step, z, r0, column(b));
       };
-      ask(0);
-      auto finish = [&](int b, const float(&v)[32]) {
-        __syncwarp();
+      if constexpr (!SPLIT) ask(0);
+      auto stage = [&](float *to, const float(&v)[32]) {
 #pragma unroll
         for (int e = 0; e < 32; e += 4)
-          *reinterpret_cast<float4 *>(tile + tile_place(lane, e)) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-        __syncwarp();
+          *reinterpret_cast<float4 *>(to + tile_place(lane, e)) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+      };
+      auto finish = [&](int b, float *staged) {
         if (MODE == kGram && parts > 1) {
           constexpr int kPerTile = (kTM / 32) * (BN / 32);
           const int64_t block = int64_t(zt) * kPerTile + (int(rank) * 4 + quad) * (BN / 32) + 2 * b + side;
-          if (!join_parts(g, tile, block, part)) return;
+          if (!join_parts(g, staged, block, part)) return;
         }
-        finish_block<MODE, SPLIT>(g, step, tile, z, r0, column(b), dr, input, [&] { ask(b + 1); });
+        finish_block<MODE, SPLIT>(g, step, staged, z, r0, column(b), dr, input, [&] { ask(b + 1); });
       };
       if constexpr (SPLIT) {
         static_assert(kBlocks <= 2, "the sums stay in registers");
@@ -735,14 +750,13 @@ __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int s
           give();
         }
         if (!go) break;
-#pragma unroll 1
-        for (int b = 0; b < kBlocks; ++b) {
-          if (!wanted(b)) break;
-          float f[32];
+        __syncwarp();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) f[e] = kBlocks > 1 && b > 0 ? v[kBlocks - 1][e] : v[0][e];
-          finish(b, f);
-        }
+        for (int b = 0; b < kBlocks; ++b) stage(tile + b * 1024, v[b]);
+        __syncwarp();
+        ask(0);  // not earlier: the sums fill the registers
+#pragma unroll 1
+        for (int b = 0; b < kBlocks && wanted(b); ++b) finish(b, tile + b * 1024);
       } else {
         if (!take()) break;
 #pragma unroll 1
@@ -751,7 +765,9 @@ __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int s
           float v[32];
           __syncwarp();
           tmem_load32(tmem + at.sum.at * BN + uint32_t(b * 64), v);
-          finish(b, v);
+          stage(tile, v);
+          __syncwarp();
+          finish(b, tile);
         }
         give();
       }
@@ -788,7 +804,7 @@ __device__ __forceinline__ bool grid_wait(uint32_t *barrier, uint32_t target, Sh
 // matrices, and for large ones the tensor cores are the bound either way.
 template <int CG, int BN, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1) k_newton_schulz(const __grid_constant__ NsArgs g) {
-  using L = Layout<CG, BN>;
+  using L = Layout<CG, BN, SPLIT>;
   extern __shared__ uint8_t raw[];
   __shared__ Shared sh;
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
@@ -913,21 +929,48 @@ int64_t tile_count(bool symmetric, int64_t rows, int64_t cols, int tm, int bn) {
   return n;
 }
 
-// The tile of a call (the same for its three products), and in how many parts
-// the k-values of X X^T are cut.
-constexpr int kUnits = 148;  // blocks that are expected to run at once
+// The tile of a call (the same for its three products): 128 cg x bn, cg = 2 by
+// a pair of blocks; and in how many parts the k-values of X X^T are cut.
+constexpr int kUnits = 148;  // blocks that run at once
 struct Plan {
   int cg, bn, parts;
 };
 
+// The form with the least estimated time of a step. A product takes, for each
+// round of tiles over the units, its k-blocks times the clocks of a stage, and
+// at its end the last epilogue and the barrier. Both were measured for each
+// form (clocks; with SPLIT the flushes come on top) and are rounded here; the
+// estimate orders the forms as their times do, e.g. at 4096 x 4096 bf16 (us)
+// 1x64 1944, 1x128 1416, 1x256 1512, 2x128 1506, 2x256 1336; at 2048 x 2048
+// 334, 258, 366, 248, 363; at 1024 x 1024 134, 182, 283, 178, 283; 2048 x 2048
+// fp32 1048, 672, -, 638, -.
 Plan plan_for(int64_t batch, int64_t s, int64_t w, bool split) {
-  Plan p{1, 64, 1};
-  if (!split && tile_count(true, s, s, 128, 256) * batch >= kUnits) p.bn = 256;
-  else if (tile_count(true, s, s, 128, 128) * batch >= kUnits / 4) p.bn = 128;
-  const int64_t tiles = tile_count(true, s, s, 128 * p.cg, p.bn) * batch;
-  const int64_t kall = (w + kTileK - 1) / kTileK * (split ? 3 : 1);
-  p.parts = int(std::max<int64_t>(1, std::min<int64_t>(kUnits / p.cg / std::max<int64_t>(tiles, 1), kall / 8)));
-  return p;
+  struct Form {
+    int cg, bn, stage, end, stage_split, end_split;
+  };
+  constexpr Form forms[] = {{1, 64, 330, 8000, 330, 12000}, {1, 128, 420, 11000, 450, 16000}, {2, 128, 400, 11000, 430, 16000},
+                            {1, 256, 600, 20000, 0, 0},     {2, 256, 560, 20000, 0, 0}};
+  auto blocks = [&](int64_t values) { return (values + kTileK - 1) / kTileK * (split ? 3 : 1); };
+  Plan best{};
+  int64_t least = 0;
+  for (const Form &f : forms) {
+    if (split && f.stage_split == 0) continue;
+    const int64_t units = kUnits / f.cg;
+    auto rounds = [&](int64_t tiles) { return (tiles + units - 1) / units; };
+    const int64_t sym = tile_count(true, s, s, 128 * f.cg, f.bn) * batch;
+    const int64_t app = tile_count(false, s, w, 128 * f.cg, f.bn) * batch;
+    // joining parts costs about as much as 24 stages
+    const int64_t kall = blocks(w);
+    const int64_t parts = kall < 48 ? 1 : std::max<int64_t>(1, std::min<int64_t>(units / sym, kall / 16));
+    const int64_t stages = rounds(sym * parts) * ((kall + parts - 1) / parts) + (parts > 1 ? 24 : 0) +
+                           rounds(sym) * blocks(s) + rounds(app) * blocks(s);
+    const int64_t clocks = stages * (split ? f.stage_split : f.stage) + 3 * (split ? f.end_split : f.end);
+    if (least == 0 || clocks < least) {
+      least = clocks;
+      best = Plan{f.cg, f.bn, int(parts)};
+    }
+  }
+  return best;
 }
 
 // The workspace of a call: X twice (a product reads one and writes the other),
@@ -977,7 +1020,7 @@ Space muon_space(void *base, int64_t batch, int64_t s, int64_t w, bool split) {
 
 template <int CG, int BN, bool SPLIT>
 void launch_newton_schulz(const NsArgs &g, int64_t units, int sms, cudaStream_t st) {
-  using L = Layout<CG, BN>;
+  using L = Layout<CG, BN, SPLIT>;
   auto *kernel = k_newton_schulz<CG, BN, SPLIT>;
   allow_dynamic_smem(kernel, L::kBytes);
   cudaLaunchConfig_t cfg{};
