@@ -870,6 +870,305 @@ __global__ void __launch_bounds__(kThreads, 1) k_newton_schulz(const __grid_cons
 }
 
 // ---------------------------------------------------------------------------
+// Small matrices: one CTA each, everything on chip
+// ---------------------------------------------------------------------------
+
+constexpr int kSmallSide = 128, kSmallWide = 256;  // the largest s and w of the kernel below
+constexpr int kSmallTile = 128 * 128;              // bytes: 128 rows of 64 values
+
+// Place (in values) of (r, c) in a matrix of 64-column tiles of 128 rows with
+// 128-byte swizzle: what the matrix instructions read, K-major as rows of
+// columns, or MN-major as rows of k.
+__device__ __forceinline__ int small_place(int r, int c) {
+  return (c >> 6) * (kSmallTile / 2) + r * 64 + ((((c >> 3) ^ r) & 7) << 3) + (c & 7);
+}
+
+__device__ __forceinline__ void open_eight(const uint4 &v, float (&f)[8]) {
+  const __half2 *h = reinterpret_cast<const __half2 *>(&v);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float2 t = __half22float2(h[e]);
+    f[2 * e] = t.x;
+    f[2 * e + 1] = t.y;
+  }
+}
+
+// The whole call for a matrix with s <= 128 and w <= 256: momentum, norm, all
+// products and the result in one CTA, X as hi + lo and A / B in shared memory
+// in the layout of the matrix instructions (X serves as a K-major operand of
+// X X^T and, the same bytes, as the MN-major one of B X). A product is a few
+// instructions by one thread; its epilogue reads and writes a thread's own
+// row in place. Bound by latency: between two products only a barrier of the
+// CTA, where the kernel for large matrices passes through L2 and a barrier of
+// the grid (128 x 64 bf16: 64 us there with its three launches).
+//
+// SPLIT: hi hi into one accumulator (at most 16 instructions, as between two
+// flushes there), the lo products into another, 2^-11 of it in size, whose cut
+// sums do not matter.
+template <class V, bool MOM, bool SPLIT>
+__global__ void __launch_bounds__(256)
+k_newton_schulz_small(UpdateArgs a, int s, int w, int transposed, int steps, float eps, FinishArgs fin,
+                      uint32_t tmem_columns, uint32_t *status) {
+  extern __shared__ uint8_t raw[];
+  __shared__ float diag_a[kSmallSide], diag_b[kSmallSide];
+  __shared__ double red[8];
+  __shared__ double factor;
+  __shared__ uint64_t done;
+  __shared__ uint32_t tmem_base;
+  __shared__ volatile uint32_t given_up;
+  __half *xh = reinterpret_cast<__half *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  const int xtiles = (w + 63) >> 6, stiles = (s + 63) >> 6;
+  __half *xl = xh + xtiles * (kSmallTile / 2), *ah = xl + xtiles * (kSmallTile / 2), *al = ah + stiles * (kSmallTile / 2);
+  const int tid = int(threadIdx.x), warp = tid >> 5, lane = tid & 31;
+  const int64_t z = blockIdx.x;
+
+  if (tid == 0) {
+    mbar_init(&done, 1);
+    given_up = 0u;
+  }
+  if (warp == 0) tmem_alloc<1>(&tmem_base, tmem_columns);
+  {
+    const int n16 = (2 * xtiles + (SPLIT ? 2 : 1) * stiles) * (kSmallTile / 16);
+    for (int i = tid; i < n16; i += 256) reinterpret_cast<uint4 *>(xh)[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
+
+  // U, its norm, X_0: items of 8 values of a row
+  const int m = int(a.m), n = int(a.n), groups = (n + 7) >> 3, items = m * groups;
+  auto load_item = [&](int t, int &i, int &j, int &count, float (&u)[8], float (&mom)[8]) {
+    i = t / groups;
+    j = (t - i * groups) * 8;
+    count = t < items ? min(8, n - j) : 0;
+    load_eight<V>(static_cast<const typename V::T *>(a.grad.p) + z * a.grad.batch + i * a.grad.row + j, a.vec, 1, count, u);
+    if constexpr (MOM)
+      load_eight<F32>(static_cast<const float *>(a.momentum.p) + z * a.momentum.batch + i * a.momentum.row + j, a.vec, 1,
+                      count, mom);
+  };
+  double sum = 0.0;
+#pragma unroll 2
+  for (int t = tid; t < items; t += 256) {
+    int i, j, count;
+    float u[8], mom[8];
+    load_item(t, i, j, count, u, mom);
+    if constexpr (MOM) {
+      float *mp = const_cast<float *>(static_cast<const float *>(a.momentum.p)) + z * a.momentum.batch + i * a.momentum.row + j;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        mom[e] = __fmaf_rn(a.beta, mom[e], u[e]);
+        if (e < count) mp[e] = mom[e];
+        u[e] = update_of(a, u[e], mom[e]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum = fma(double(u[e]), double(u[e]), sum);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) red[warp] = sum;
+  __syncthreads();
+  if (tid == 0) {
+    sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += red[i];
+    factor = double(kScale) / (sqrt(sum) + double(eps));
+  }
+  tmem_fence_before();
+  __syncthreads();
+  tmem_fence_after();
+  const uint32_t tmem = tmem_base;
+#pragma unroll 2
+  for (int t = tid; t < items; t += 256) {
+    int i, j, count;
+    float u[8], mom[8];
+    load_item(t, i, j, count, u, mom);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (MOM) u[e] = update_of(a, u[e], mom[e]);
+      u[e] = e < count ? float(double(u[e]) * factor) : 0.0f;
+    }
+    if (!transposed) {
+      put_eight(xh + small_place(i, j), xl + small_place(i, j), u);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (e < count) {
+          const __half h = __float2half_rn(u[e]);
+          xh[small_place(j + e, i)] = h;
+          xl[small_place(j + e, i)] = __float2half_rn(u[e] - __half2float(h));
+        }
+      }
+    }
+  }
+
+  // operands of a product are written: make them visible to the tensor core, let one thread issue, wait for it
+  const uint32_t sx = smem_u32(xh), sxl = smem_u32(xl), sa = smem_u32(ah), sal = smem_u32(al);
+  uint32_t parity = 0;
+  auto multiply = [&](uint32_t pa, uint32_t pal, uint32_t pb, uint32_t pbl, bool b_mn, int width, int depth) {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    tmem_fence_before();
+    __syncthreads();
+    if (warp == 0 && elect_one()) {
+      tmem_fence_after();
+      const int wide = (width + 15) & ~15, chunks = (depth + 15) >> 4;
+      const uint32_t desc = mma_desc(128, wide, b_mn);
+      const uint32_t extra = tmem + tmem_columns / 2;  // the lo products' accumulator
+      auto go = [&](uint32_t acc, uint32_t x, uint32_t y, bool add) {
+        const uint64_t da = operand_desc(x, 16), db = operand_desc(y, b_mn ? kSmallTile : 16);
+        for (int q = 0; q < chunks; ++q) {
+          const uint32_t along = (q >> 2) * (kSmallTile >> 4) + (q & 3) * (32 >> 4);
+          mma_f16<1>(acc, da + along, db + (b_mn ? q * (2048 >> 4) : along), desc, add || q > 0);
+        }
+      };
+      go(tmem, pa, pb, false);
+      if constexpr (SPLIT) {
+        go(extra, pa, pbl, false);
+        go(extra, pal, pb, true);
+      }
+      mma_commit<1>(&done);
+    }
+    __syncwarp();
+    const bool ok = wait_or_give_up(&done, parity, &given_up);
+    parity ^= 1u;
+    tmem_fence_after();
+    return __syncthreads_and(ok) != 0;
+  };
+  const int quad = warp & 3, side = warp >> 2, r = quad * 32 + lane;
+  const bool mine = quad * 32 < s;  // warps of rows beyond s have nothing to do (their rows are zeros throughout)
+  auto sums = [&](int c0, float (&v)[32]) {
+    __syncwarp();
+    tmem_load32(tmem + (uint32_t(quad * 32) << 16) + uint32_t(c0), v);
+    if constexpr (SPLIT) {
+      float l[32];
+      tmem_load32(tmem + (uint32_t(quad * 32) << 16) + tmem_columns / 2 + uint32_t(c0), l);
+#pragma unroll
+      for (int e = 0; e < 32; ++e) v[e] += l[e];
+    }
+  };
+  auto give = [&](__half *hi, __half *lo, bool both, int c, const float (&f)[8]) {
+    const int at = small_place(r, c);
+    uint4 h, l;
+    __half2 *hh = reinterpret_cast<__half2 *>(&h), *ll = reinterpret_cast<__half2 *>(&l);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      hh[e] = __floats2half2_rn(f[2 * e], f[2 * e + 1]);
+      const float2 b = __half22float2(hh[e]);
+      ll[e] = __floats2half2_rn(f[2 * e] - b.x, f[2 * e + 1] - b.y);
+    }
+    *reinterpret_cast<uint4 *>(hi + at) = h;
+    if (both) *reinterpret_cast<uint4 *>(lo + at) = l;
+  };
+  auto take = [&](const __half *hi, const __half *lo, bool both, int c, float (&f)[8]) {
+    const int at = small_place(r, c);
+    open_eight(*reinterpret_cast<const uint4 *>(hi + at), f);
+    if (both) {
+      float l[8];
+      open_eight(*reinterpret_cast<const uint4 *>(lo + at), l);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] += l[e];
+    }
+  };
+
+  for (int step = 0; step < steps; ++step) {
+    // A = X X^T, its diagonal apart
+    if (!multiply(sx, sxl, sx, sxl, false, s, w)) break;
+    if (mine) {
+#pragma unroll 1
+      for (int c0 = side * 32; c0 < s; c0 += 64) {
+        float v[32];
+        sums(c0, v);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float f[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            f[e] = c0 + 8 * q + e < s ? v[8 * q + e] * (1.0f / kScale) : 0.0f;
+            if (c0 + 8 * q + e == r) {
+              diag_a[r] = f[e];
+              f[e] = 0.0f;
+            }
+          }
+          give(ah, al, SPLIT, c0 + 8 * q, f);
+        }
+      }
+    }
+    // B = b A + c A A, in A's place
+    if (!multiply(sa, sal, sa, sal, false, s, s)) break;
+    if (mine) {
+      const float dr = diag_a[r < s ? r : 0];
+#pragma unroll 1
+      for (int c0 = side * 32; c0 < s; c0 += 64) {
+        float v[32];
+        sums(c0, v);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float x[8], f[8];
+          take(ah, al, SPLIT, c0 + 8 * q, x);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int c = c0 + 8 * q + e;
+            const bool on = c == r;
+            const float o = on ? dr : x[e];
+            const float aa = __fmaf_rn(on ? dr : dr + diag_a[c], o, v[8 * q + e]);
+            f[e] = c < s ? __fmaf_rn(kNsC / kScale, aa, kNsB * o) : 0.0f;
+            if (on) {
+              diag_b[r] = f[e] * (1.0f / kScale);
+              f[e] = 0.0f;
+            }
+          }
+          give(ah, al, SPLIT, c0 + 8 * q, f);
+        }
+      }
+    }
+    // X = (a + diag) X + B X, in place
+    if (!multiply(sa, sal, sx, sxl, true, w, s)) break;
+    if (mine) {
+      const float k = kNsA + diag_b[r < s ? r : 0];
+#pragma unroll 1
+      for (int c0 = side * 32; c0 < w; c0 += 64) {
+        float v[32];
+        sums(c0, v);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float x[8], f[8];
+          take(xh, xl, true, c0 + 8 * q, x);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            f[e] = c0 + 8 * q + e < w && r < s ? __fmaf_rn(k, x[e], v[8 * q + e] * (1.0f / kScale)) : 0.0f;
+          give(xh, xl, true, c0 + 8 * q, f);
+        }
+      }
+    }
+  }
+  __syncthreads();
+  if (given_up) {
+    if (tid == 0) {
+      wait_for(&done, parity ^ 1u, nullptr);
+      *reinterpret_cast<volatile uint32_t *>(status) = 1u;
+      __threadfence_system();
+    }
+  } else {
+    // the result, in the call's own order
+    for (int t = tid; t < items; t += 256) {
+      const int i = t / groups, j = (t - i * groups) * 8, count = min(8, n - j);
+      const int64_t at = z * fin.batch + int64_t(i) * fin.row + j;
+      float o[8], old[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        old[e] = fin.update && e < count ? load_typed(fin.out, fin.type, at + e) : 0.0f;
+        const int p = e < count ? (transposed ? small_place(j + e, i) : small_place(i, j + e)) : 0;
+        o[e] = (__half2float(xh[p]) + __half2float(xl[p])) * (1.0f / kScale);
+        if (fin.update) o[e] = __fmaf_rn(-fin.rate, o[e], fin.keep * old[e]);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < count) store_typed(fin.out, fin.type, at + e, o[e]);
+    }
+  }
+  tmem_fence_before();
+  __syncthreads();
+  if (warp == 0) tmem_free<1>(tmem, tmem_columns);
+}
+
+// ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
 
@@ -1070,6 +1369,26 @@ void orthogonalise(UpdateArgs u, int grad_type, int64_t batch, int steps, float 
     throw Error(SE_ERR_RUNTIME, "an earlier orthogonalisation on cuda:" + std::to_string(device) +
                                     " gave up waiting for its copies; its results are not valid");
   }
+  fin.transposed = transposed;
+  if (s <= kSmallSide && w <= kSmallWide) {
+    const int xtiles = int((w + 63) / 64), stiles = int((s + 63) / 64);
+    const size_t smem = size_t(2 * xtiles + (split ? 2 : 1) * stiles) * kSmallTile + 1024;
+    const uint32_t columns = (w > 128 ? 256 : 128) * (split ? 2 : 1);
+    dispatch_value(grad_type, [&](auto tag) {
+      using V = decltype(tag);
+      auto go = [&](auto mom, auto sp) {
+        auto *kernel = k_newton_schulz_small<V, decltype(mom)::value, decltype(sp)::value>;
+        allow_dynamic_smem(kernel, smem);
+        kernel<<<unsigned(batch), 256, smem, st>>>(u, int(s), int(w), int(transposed), steps, eps, fin, columns, g.status);
+      };
+      if (u.momentum.p && split) go(std::true_type{}, std::true_type{});
+      else if (u.momentum.p) go(std::true_type{}, std::false_type{});
+      else if (split) go(std::false_type{}, std::true_type{});
+      else go(std::false_type{}, std::false_type{});
+    });
+    launched("k_newton_schulz_small");
+    return;
+  }
   const bool dense = u.grad.row == u.n && (u.momentum.p == nullptr || u.momentum.row == u.n);
   const int64_t spans = dense ? (u.m * u.n + kSpan - 1) / kSpan : u.m * ((u.n + kSpan - 1) / kSpan);
   const int nparts = int(std::min<int64_t>(std::min<int64_t>(kNormParts, spans), std::max<int64_t>(1, 4 * sms / batch)));
@@ -1119,7 +1438,6 @@ void orthogonalise(UpdateArgs u, int grad_type, int64_t batch, int steps, float 
   g.partial = sp.partial;
   g.barrier = sp.counters;
   g.arrived = sp.counters + 1;
-  fin.transposed = transposed;
   g.fin = fin;
   const int64_t units = std::max<int64_t>(int64_t(g.gram.tiles) * plan.parts, g.apply.tiles) * batch;
   const int form = plan.cg * 1000 + plan.bn * 2 + (split ? 1 : 0);
