@@ -325,7 +325,8 @@ int se_orthogonalize(int32_t dtype, const void *update, size_t batch, int64_t m,
  *   momentum = beta momentum + grad                        (fp32)
  *   U = grad + beta momentum if nesterov, else momentum
  *   weight = (1 - lr weight_decay) weight - lr scale orthogonalize(U)
- * Weight, gradient and momentum overlap nowhere. */
+ * grad_dtype is weight_dtype or SE_FLOAT32. Weight, gradient and momentum
+ * overlap nowhere. */
 int se_muon_step(int32_t weight_dtype, int32_t grad_dtype, void *weight, int64_t weight_batch_stride,
                  int64_t weight_row_stride, const void *grad, int64_t grad_batch_stride, int64_t grad_row_stride,
                  float *momentum, int64_t momentum_batch_stride, int64_t momentum_row_stride, size_t batch,

@@ -29,7 +29,7 @@
 // thread that holds it.
 
 #include <algorithm>
-#include <cstring>
+#include <type_traits>
 
 #include "se_dense.hpp"
 #include "se_tcgen05.cuh"
@@ -86,9 +86,49 @@ __device__ __forceinline__ float update_of(const UpdateArgs &a, float g, float m
   return a.nesterov ? __fmaf_rn(a.beta, mom, g) : mom;
 }
 
-// M <- beta M + G, and this block's part of |U|^2 (fp64: squares of fp32
-// values neither overflow nor vanish there). Zeroes the counters of the launch
-// that follows. Bound by HBM: a matrix without gaps is taken as one row, and
+// Adds eight squares to `sum` through an fp32 sum (a conversion to fp64 per value
+// would take longer than the loads). True where that was not safe: fp32 squares
+// may have overflowed or vanished, and the caller takes its sum again with
+// wide_square_sum.
+__device__ __forceinline__ bool square_sum(const float (&u)[8], double &sum) {
+  float f = 0.0f, most = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    f = __fmaf_rn(u[e], u[e], f);
+    most = fmaxf(most, fabsf(u[e]));
+  }
+  sum += double(f);
+  return !(f > 1e-24f && f < 1e36f) && !(most == 0.0f && f == 0.0f);
+}
+__device__ __forceinline__ void wide_square_sum(const float (&u)[8], double &sum) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sum = fma(double(u[e]), double(u[e]), sum);
+}
+
+// S / (|U| + eps) as a fraction and two powers of two: the factor itself may lie
+// outside fp32's range.
+struct Factor {
+  float fraction, power0, power1;
+  __device__ __forceinline__ float times(float u) const { return u * power0 * power1 * fraction; }
+};
+__device__ __forceinline__ Factor update_factor(double sum, float eps) {
+  const double f = double(kScale) / (sqrt(sum) + double(eps));
+  Factor r;
+  if (!(f > 0.0) || f > 1.7e308) {  // a sum that is infinite, no number, or zero with eps = 0
+    r.fraction = float(f);
+    r.power0 = r.power1 = 1.0f;
+    return r;
+  }
+  int k;
+  r.fraction = float(frexp(f, &k));  // [0.5, 1]
+  const int half = k / 2;
+  r.power0 = ldexpf(1.0f, half);
+  r.power1 = ldexpf(1.0f, k - half);
+  return r;
+}
+
+// M <- beta M + G, and this block's part of |U|^2. Zeroes the counters of the
+// launch that follows. Bound by HBM: a matrix without gaps is taken as one row, and
 // every thread has 8 values of each array in flight.
 template <class V, bool MOM>
 __global__ void __launch_bounds__(256)
@@ -104,9 +144,15 @@ k_muon_momentum(UpdateArgs a, double *__restrict__ parts, uint32_t *__restrict__
   const int64_t spans = (len + kSpan - 1) / kSpan;
   const int step = a.vec ? 1 : 256;
   double sum = 0.0;
+  bool unsafe = false;
+  auto place = [&](int64_t t, int64_t &i, int64_t &j) {
+    i = t / spans;
+    j = (t - i * spans) * kSpan + threadIdx.x * (a.vec ? 8 : 1);
+    return j >= len ? 0 : int(min(int64_t(8), (len - j + step - 1) / step));
+  };
   for (int64_t t = blockIdx.x; t < rows * spans; t += gridDim.x) {
-    const int64_t i = t / spans, j = (t - i * spans) * kSpan + threadIdx.x * (a.vec ? 8 : 1);
-    const int count = j >= len ? 0 : int(min(int64_t(8), (len - j + step - 1) / step));
+    int64_t i, j;
+    const int count = place(t, i, j);
     float g[8];
     load_eight<V>(static_cast<const typename V::T *>(a.grad.p) + z * a.grad.batch + i * a.grad.row + j, a.vec, step, count, g);
     if constexpr (MOM) {
@@ -129,8 +175,23 @@ k_muon_momentum(UpdateArgs a, double *__restrict__ parts, uint32_t *__restrict__
           if (e < count) mp[e * step] = mom[e];
       }
     }
+    unsafe |= square_sum(g, sum);
+  }
+  if (__syncthreads_or(unsafe)) {
+    sum = 0.0;
+    for (int64_t t = blockIdx.x; t < rows * spans; t += gridDim.x) {
+      int64_t i, j;
+      const int count = place(t, i, j);
+      float g[8], mom[8];
+      load_eight<V>(static_cast<const typename V::T *>(a.grad.p) + z * a.grad.batch + i * a.grad.row + j, a.vec, step, count, g);
+      if constexpr (MOM) {
+        load_eight<F32>(static_cast<const float *>(a.momentum.p) + z * a.momentum.batch + i * a.momentum.row + j, a.vec, step,
+                        count, mom);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sum = fma(double(g[e]), double(g[e]), sum);
+        for (int e = 0; e < 8; ++e) g[e] = update_of(a, g[e], mom[e]);
+      }
+      wide_square_sum(g, sum);
+    }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -167,7 +228,7 @@ __global__ void __launch_bounds__(256)
 k_muon_scale(UpdateArgs a, const double *__restrict__ parts, int nparts, float eps, bool transposed,
              __half *__restrict__ hi, __half *__restrict__ lo, int64_t ld, int64_t batch_stride) {
   __shared__ float tile[64][65];
-  __shared__ double factor;  // fp64: 1 / |U| of a tiny update passes fp32's range
+  __shared__ Factor factor;
   const int64_t z = blockIdx.z;
   pdl_wait();
   if (threadIdx.x < 32) {
@@ -175,10 +236,10 @@ k_muon_scale(UpdateArgs a, const double *__restrict__ parts, int nparts, float e
     for (int k = threadIdx.x; k < nparts; k += 32) sum += parts[z * kNormParts + k];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (threadIdx.x == 0) factor = double(kScale) / (sqrt(sum) + double(eps));
+    if (threadIdx.x == 0) factor = update_factor(sum, eps);
   }
   __syncthreads();
-  const double k = factor;
+  const Factor k = factor;
   const int row = threadIdx.x >> 3, at = threadIdx.x & 7;  // 8 threads of 8 values per row, rows `row` and `row` + 32
   const int step = a.vec ? 1 : 8, first = a.vec ? at * 8 : at;
   const int64_t tiles_j = (a.n + 63) / 64, tiles = tiles_j * ((a.m + 63) / 64);
@@ -199,7 +260,7 @@ k_muon_scale(UpdateArgs a, const double *__restrict__ parts, int nparts, float e
         for (int e = 0; e < 8; ++e) u[q][e] = update_of(a, u[q][e], mom[e]);
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) u[q][e] = float(double(u[q][e]) * k);
+      for (int e = 0; e < 8; ++e) u[q][e] = k.times(u[q][e]);
     }
     const bool through = transposed || !a.vec;
     if (through) {
@@ -893,26 +954,32 @@ __device__ __forceinline__ void open_eight(const uint4 &v, float (&f)[8]) {
   }
 }
 
-// The whole call for a matrix with s <= 128 and w <= 256: momentum, norm, all
-// products and the result in one CTA, X as hi + lo and A / B in shared memory
-// in the layout of the matrix instructions (X serves as a K-major operand of
-// X X^T and, the same bytes, as the MN-major one of B X). A product is a few
-// instructions by one thread; its epilogue reads and writes a thread's own
-// row in place. Bound by latency: between two products only a barrier of the
-// CTA, where the kernel for large matrices passes through L2 and a barrier of
-// the grid (128 x 64 bf16: 64 us there with its three launches).
+// The whole call for a matrix with s <= 128 and w <= 128 (SIDES = 4) or 256
+// (SIDES = 2): momentum, norm, all products and the result in one CTA. A thread
+// owns every SIDES-th block of 32 columns of a row: its values of X and of A
+// stay in its registers in fp32, and only their f16 operand parts go to shared
+// memory, in the layout of the matrix instructions (X serves as a K-major
+// operand of X X^T and, the same bytes, as the MN-major one of B X). Between two products there is only a
+// barrier of the CTA, where the kernel for large matrices passes through L2
+// and a barrier of the grid (128 x 64 bf16: 64 us there with its launches).
+// Bound by the instructions of one SM and the latency of 3 products a step;
+// with X and A in shared memory as f16 pairs, unpacked and packed again in
+// every epilogue, it took 33 us at 128 x 64 and 70 at 128 x 256.
 //
 // SPLIT: hi hi into one accumulator (at most 16 instructions, as between two
 // flushes there), the lo products into another, 2^-11 of it in size, whose cut
 // sums do not matter.
-template <class V, bool MOM, bool SPLIT>
-__global__ void __launch_bounds__(256)
+template <class V, class W, bool MOM, int SIDES>
+__global__ void __launch_bounds__(128 * SIDES)
 k_newton_schulz_small(UpdateArgs a, int s, int w, int transposed, int steps, float eps, FinishArgs fin,
                       uint32_t tmem_columns, uint32_t *status) {
+  constexpr bool SPLIT = !std::is_same_v<W, BF16>;  // as split_products says
+  constexpr int kThreads = 128 * SIDES, kWarps = 4 * SIDES;
+  constexpr int kX = SIDES == 2 ? 4 : 1, kA = 4 / SIDES;  // blocks of X and of A that a thread owns
   extern __shared__ uint8_t raw[];
-  __shared__ float diag_a[kSmallSide], diag_b[kSmallSide];
-  __shared__ double red[8];
-  __shared__ double factor;
+  __shared__ __align__(16) float diag[kSmallSide];
+  __shared__ double red[kWarps];
+  __shared__ Factor factor;
   __shared__ uint64_t done;
   __shared__ uint32_t tmem_base;
   __shared__ volatile uint32_t given_up;
@@ -929,37 +996,57 @@ k_newton_schulz_small(UpdateArgs a, int s, int w, int transposed, int steps, flo
   if (warp == 0) tmem_alloc<1>(&tmem_base, tmem_columns);
   {
     const int n16 = (2 * xtiles + (SPLIT ? 2 : 1) * stiles) * (kSmallTile / 16);
-    for (int i = tid; i < n16; i += 256) reinterpret_cast<uint4 *>(xh)[i] = make_uint4(0u, 0u, 0u, 0u);
+    for (int i = tid; i < n16; i += kThreads) reinterpret_cast<uint4 *>(xh)[i] = make_uint4(0u, 0u, 0u, 0u);
   }
+  if (tid < kSmallSide) diag[tid] = 0.0f;
 
-  // U, its norm, X_0: items of 8 values of a row
-  const int m = int(a.m), n = int(a.n), groups = (n + 7) >> 3, items = m * groups;
-  auto load_item = [&](int t, int &i, int &j, int &count, float (&u)[8], float (&mom)[8]) {
-    i = t / groups;
-    j = (t - i * groups) * 8;
-    count = t < items ? min(8, n - j) : 0;
+  // U, its norm, X_0: eight values of a row per thread, a power of two of threads per row
+  const int m = int(a.m), n = int(a.n);
+  int shift = 0;
+  while ((8 << shift) < n) ++shift;
+  const int i0 = tid >> shift, rows = kThreads >> shift, j = (tid & ((1 << shift) - 1)) * 8, count = max(0, min(8, n - j));
+  auto load_update = [&](int i, float (&u)[8], float (&mom)[8]) {
     load_eight<V>(static_cast<const typename V::T *>(a.grad.p) + z * a.grad.batch + i * a.grad.row + j, a.vec, 1, count, u);
     if constexpr (MOM)
       load_eight<F32>(static_cast<const float *>(a.momentum.p) + z * a.momentum.batch + i * a.momentum.row + j, a.vec, 1,
                       count, mom);
   };
   double sum = 0.0;
+  bool unsafe = false;
 #pragma unroll 2
-  for (int t = tid; t < items; t += 256) {
-    int i, j, count;
+  for (int i = i0; i < m; i += rows) {
     float u[8], mom[8];
-    load_item(t, i, j, count, u, mom);
+    load_update(i, u, mom);
     if constexpr (MOM) {
       float *mp = const_cast<float *>(static_cast<const float *>(a.momentum.p)) + z * a.momentum.batch + i * a.momentum.row + j;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         mom[e] = __fmaf_rn(a.beta, mom[e], u[e]);
-        if (e < count) mp[e] = mom[e];
         u[e] = update_of(a, u[e], mom[e]);
       }
-    }
+      if (a.vec) {
+        if (count > 0) {
+          reinterpret_cast<float4 *>(mp)[0] = make_float4(mom[0], mom[1], mom[2], mom[3]);
+          reinterpret_cast<float4 *>(mp)[1] = make_float4(mom[4], mom[5], mom[6], mom[7]);
+        }
+      } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sum = fma(double(u[e]), double(u[e]), sum);
+        for (int e = 0; e < 8; ++e)
+          if (e < count) mp[e] = mom[e];
+      }
+    }
+    unsafe |= square_sum(u, sum);
+  }
+  if (__syncthreads_or(unsafe)) {
+    sum = 0.0;
+    for (int i = i0; i < m; i += rows) {
+      float u[8], mom[8];
+      load_update(i, u, mom);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if constexpr (MOM) u[e] = update_of(a, u[e], mom[e]);
+      wide_square_sum(u, sum);
+    }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -968,25 +1055,25 @@ k_newton_schulz_small(UpdateArgs a, int s, int w, int transposed, int steps, flo
   if (tid == 0) {
     sum = 0.0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum += red[i];
-    factor = double(kScale) / (sqrt(sum) + double(eps));
+    for (int i = 0; i < kWarps; ++i) sum += red[i];
+    factor = update_factor(sum, eps);
   }
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
   const uint32_t tmem = tmem_base;
+  const Factor k0 = factor;
 #pragma unroll 2
-  for (int t = tid; t < items; t += 256) {
-    int i, j, count;
+  for (int i = i0; i < m; i += rows) {
     float u[8], mom[8];
-    load_item(t, i, j, count, u, mom);
+    load_update(i, u, mom);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       if constexpr (MOM) u[e] = update_of(a, u[e], mom[e]);
-      u[e] = e < count ? float(double(u[e]) * factor) : 0.0f;
+      u[e] = e < count ? k0.times(u[e]) : 0.0f;
     }
     if (!transposed) {
-      put_eight(xh + small_place(i, j), xl + small_place(i, j), u);
+      if (count > 0) put_eight(xh + small_place(i, j), xl + small_place(i, j), u);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -999,7 +1086,8 @@ k_newton_schulz_small(UpdateArgs a, int s, int w, int transposed, int steps, flo
     }
   }
 
-  // operands of a product are written: make them visible to the tensor core, let one thread issue, wait for it
+  // A product: the operands written so far become visible to the tensor core,
+  // one thread issues its instructions, all wait. False: gave up.
   const uint32_t sx = smem_u32(xh), sxl = smem_u32(xl), sa = smem_u32(ah), sal = smem_u32(al);
   uint32_t parity = 0;
   auto multiply = [&](uint32_t pa, uint32_t pal, uint32_t pb, uint32_t pbl, bool b_mn, int width, int depth) {
@@ -1028,11 +1116,14 @@ k_newton_schulz_small(UpdateArgs a, int s, int w, int transposed, int steps, flo
     __syncwarp();
     const bool ok = wait_or_give_up(&done, parity, &given_up);
     parity ^= 1u;
+    const bool all = __syncthreads_and(ok) != 0;
     tmem_fence_after();
-    return __syncthreads_and(ok) != 0;
+    return all;
   };
   const int quad = warp & 3, side = warp >> 2, r = quad * 32 + lane;
-  const bool mine = quad * 32 < s;  // warps of rows beyond s have nothing to do (their rows are zeros throughout)
+  const bool mine = quad * 32 < s;  // rows beyond s hold zeros throughout
+  const int s16 = (s + 15) & ~15, w16 = (w + 15) & ~15;
+  auto column = [&](int b) { return (b * SIDES + side) * 32; };
   auto sums = [&](int c0, float (&v)[32]) {
     __syncwarp();
     tmem_load32(tmem + (uint32_t(quad * 32) << 16) + uint32_t(c0), v);
@@ -1043,124 +1134,153 @@ k_newton_schulz_small(UpdateArgs a, int s, int w, int transposed, int steps, flo
       for (int e = 0; e < 32; ++e) v[e] += l[e];
     }
   };
-  auto give = [&](__half *hi, __half *lo, bool both, int c, const float (&f)[8]) {
-    const int at = small_place(r, c);
-    uint4 h, l;
-    __half2 *hh = reinterpret_cast<__half2 *>(&h), *ll = reinterpret_cast<__half2 *>(&l);
+  // a block of the thread's row as operand parts, as far as the products' widths reach
+  auto put_block = [&](__half *hi, __half *lo, int c0, int end, const float (&f)[32]) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      hh[e] = __floats2half2_rn(f[2 * e], f[2 * e + 1]);
-      const float2 b = __half22float2(hh[e]);
-      ll[e] = __floats2half2_rn(f[2 * e] - b.x, f[2 * e + 1] - b.y);
-    }
-    *reinterpret_cast<uint4 *>(hi + at) = h;
-    if (both) *reinterpret_cast<uint4 *>(lo + at) = l;
-  };
-  auto take = [&](const __half *hi, const __half *lo, bool both, int c, float (&f)[8]) {
-    const int at = small_place(r, c);
-    open_eight(*reinterpret_cast<const uint4 *>(hi + at), f);
-    if (both) {
-      float l[8];
-      open_eight(*reinterpret_cast<const uint4 *>(lo + at), l);
+    for (int q = 0; q < 4; ++q) {
+      if (c0 + 8 * q < end) {
+        const int at = small_place(r, c0 + 8 * q);
+        uint4 h;
+        __half2 *hh = reinterpret_cast<__half2 *>(&h);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] += l[e];
+        for (int e = 0; e < 4; ++e) hh[e] = __floats2half2_rn(f[8 * q + 2 * e], f[8 * q + 2 * e + 1]);
+        *reinterpret_cast<uint4 *>(hi + at) = h;
+        if constexpr (SPLIT) {
+          uint4 l;
+          __half2 *ll = reinterpret_cast<__half2 *>(&l);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 back = __half22float2(hh[e]);
+            ll[e] = __floats2half2_rn(f[8 * q + 2 * e] - back.x, f[8 * q + 2 * e + 1] - back.y);
+          }
+          *reinterpret_cast<uint4 *>(lo + at) = l;
+        }
+      }
     }
   };
 
+  // this lane's element of a diagonal block, which becomes zero
+  auto on_diagonal = [&](float (&f)[32]) {
+    float d = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 32; ++e) {
+      d = e == lane ? f[e] : d;
+      f[e] = e == lane ? 0.0f : f[e];
+    }
+    return d;
+  };
+
+  float x[kX][32], o[kA][32];
+  __syncthreads();
+#pragma unroll
+  for (int b = 0; b < kX; ++b) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      float h[8] = {}, l[8] = {};
+      if (mine && column(b) + 8 * q < w16) {
+        const int at = small_place(r, column(b) + 8 * q);
+        open_eight(*reinterpret_cast<const uint4 *>(xh + at), h);
+        open_eight(*reinterpret_cast<const uint4 *>(xl + at), l);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[b][8 * q + e] = h[e] + l[e];
+    }
+  }
+
+  bool ok = true;
   for (int step = 0; step < steps; ++step) {
-    // A = X X^T, its diagonal apart
-    if (!multiply(sx, sxl, sx, sxl, false, s, w)) break;
+    // A = X X^T, its diagonal D apart: off it, O
+    if (!(ok = multiply(sx, sxl, sx, sxl, false, s, w))) break;
     if (mine) {
-#pragma unroll 1
-      for (int c0 = side * 32; c0 < s; c0 += 64) {
-        float v[32];
-        sums(c0, v);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float f[8];
+      for (int b = 0; b < kA; ++b) {
+        const int c0 = column(b);
+        if (c0 >= s) break;
+        sums(c0, o[b]);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            f[e] = c0 + 8 * q + e < s ? v[8 * q + e] * (1.0f / kScale) : 0.0f;
-            if (c0 + 8 * q + e == r) {
-              diag_a[r] = f[e];
-              f[e] = 0.0f;
-            }
-          }
-          give(ah, al, SPLIT, c0 + 8 * q, f);
+        for (int e = 0; e < 32; ++e) o[b][e] *= 1.0f / kScale;
+        if (c0 == quad * 32) {
+          const float d = on_diagonal(o[b]);
+          if (r < s) diag[r] = d;
         }
+        put_block(ah, al, c0, s16, o[b]);
       }
     }
-    // B = b A + c A A, in A's place
-    if (!multiply(sa, sal, sa, sal, false, s, s)) break;
+    // B = b A + c A A, in A's place: (A A)_rc = (O O)_rc + (D_r + D_c) O_rc, on the diagonal (O O)_rr + D_r^2
+    if (!(ok = multiply(sa, sal, sa, sal, false, s, s))) break;
+    float k = kNsA;
     if (mine) {
-      const float dr = diag_a[r < s ? r : 0];
-#pragma unroll 1
-      for (int c0 = side * 32; c0 < s; c0 += 64) {
+      const float dr = diag[r];
+#pragma unroll
+      for (int b = 0; b < kA; ++b) {
+        const int c0 = column(b);
+        if (c0 >= s) break;
         float v[32];
         sums(c0, v);
+        if (c0 == quad * 32)
+          k = __fmaf_rn(kNsC / kScale, __fmaf_rn(dr, dr, on_diagonal(v)), kNsB * dr) * (1.0f / kScale);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float x[8], f[8];
-          take(ah, al, SPLIT, c0 + 8 * q, x);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int c = c0 + 8 * q + e;
-            const bool on = c == r;
-            const float o = on ? dr : x[e];
-            const float aa = __fmaf_rn(on ? dr : dr + diag_a[c], o, v[8 * q + e]);
-            f[e] = c < s ? __fmaf_rn(kNsC / kScale, aa, kNsB * o) : 0.0f;
-            if (on) {
-              diag_b[r] = f[e] * (1.0f / kScale);
-              f[e] = 0.0f;
-            }
-          }
-          give(ah, al, SPLIT, c0 + 8 * q, f);
+        for (int e = 0; e < 32; e += 4) {
+          const float4 dc = *reinterpret_cast<const float4 *>(diag + c0 + e);
+          v[e] = __fmaf_rn(kNsC / kScale, __fmaf_rn(dr + dc.x, o[b][e], v[e]), kNsB * o[b][e]);
+          v[e + 1] = __fmaf_rn(kNsC / kScale, __fmaf_rn(dr + dc.y, o[b][e + 1], v[e + 1]), kNsB * o[b][e + 1]);
+          v[e + 2] = __fmaf_rn(kNsC / kScale, __fmaf_rn(dr + dc.z, o[b][e + 2], v[e + 2]), kNsB * o[b][e + 2]);
+          v[e + 3] = __fmaf_rn(kNsC / kScale, __fmaf_rn(dr + dc.w, o[b][e + 3], v[e + 3]), kNsB * o[b][e + 3]);
         }
+        if (c0 == quad * 32) on_diagonal(v);
+        put_block(ah, al, c0, s16, v);
       }
     }
-    // X = (a + diag) X + B X, in place
-    if (!multiply(sa, sal, sx, sxl, true, w, s)) break;
+    __syncthreads();  // every thread has read D: B's diagonal takes its place
+    if (mine && quad % SIDES == side && r < s) diag[r] = k;  // the warp whose block holds these rows' diagonal
+    // X = (a + diag B) X + B X
+    if (!(ok = multiply(sa, sal, sx, sxl, true, w, s))) break;
     if (mine) {
-      const float k = kNsA + diag_b[r < s ? r : 0];
-#pragma unroll 1
-      for (int c0 = side * 32; c0 < w; c0 += 64) {
+      k = kNsA + diag[r];
+#pragma unroll
+      for (int b = 0; b < kX; ++b) {
+        const int c0 = column(b);
+        if (c0 >= w) break;
         float v[32];
         sums(c0, v);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float x[8], f[8];
-          take(xh, xl, true, c0 + 8 * q, x);
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            f[e] = c0 + 8 * q + e < w && r < s ? __fmaf_rn(k, x[e], v[8 * q + e] * (1.0f / kScale)) : 0.0f;
-          give(xh, xl, true, c0 + 8 * q, f);
-        }
+        for (int e = 0; e < 32; ++e) x[b][e] = __fmaf_rn(k, x[b][e], v[e] * (1.0f / kScale));
+        put_block(xh, xl, c0, w16, x[b]);
       }
     }
   }
   __syncthreads();
-  if (given_up) {
+  if (!ok) {
     if (tid == 0) {
       wait_for(&done, parity ^ 1u, nullptr);
       *reinterpret_cast<volatile uint32_t *>(status) = 1u;
       __threadfence_system();
     }
   } else {
-    // the result, in the call's own order
-    for (int t = tid; t < items; t += 256) {
-      const int i = t / groups, j = (t - i * groups) * 8, count = min(8, n - j);
-      const int64_t at = z * fin.batch + int64_t(i) * fin.row + j;
-      float o[8], old[8];
+    // O through shared memory (X's operands are no longer needed), then in the call's own order
+    float *out = reinterpret_cast<float *>(xh);
+    const int ld = xtiles * 64;
+    auto place = [&](int rr, int c) { return rr * ld + ((((c >> 2) ^ rr) & 7) << 2 | (c & 3)) + (c & ~31); };
+    if (mine) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        old[e] = fin.update && e < count ? load_typed(fin.out, fin.type, at + e) : 0.0f;
-        const int p = e < count ? (transposed ? small_place(j + e, i) : small_place(i, j + e)) : 0;
-        o[e] = (__half2float(xh[p]) + __half2float(xl[p])) * (1.0f / kScale);
-        if (fin.update) o[e] = __fmaf_rn(-fin.rate, o[e], fin.keep * old[e]);
+      for (int b = 0; b < kX; ++b) {
+        if (column(b) >= w) break;
+#pragma unroll
+        for (int e = 0; e < 32; e += 4)
+          *reinterpret_cast<float4 *>(out + place(r, column(b) + e)) =
+              make_float4(x[b][e], x[b][e + 1], x[b][e + 2], x[b][e + 3]);
       }
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e < count) store_typed(fin.out, fin.type, at + e, o[e]);
+    }
+    __syncthreads();
+    typename W::T *to = static_cast<typename W::T *>(fin.out) + z * fin.batch;
+    for (int i = warp; i < m; i += kWarps) {
+#pragma unroll 2
+      for (int c = lane; c < n; c += 32) {
+        typename W::T *at = to + int64_t(i) * fin.row + c;
+        float f = out[transposed ? place(c, i) : place(i, c)] * (1.0f / kScale);
+        if constexpr (MOM) f = __fmaf_rn(-fin.rate, f, fin.keep * W::load(*at));
+        *at = W::store(f);
+      }
     }
   }
   tmem_fence_before();
@@ -1374,17 +1494,20 @@ void orthogonalise(UpdateArgs u, int grad_type, int64_t batch, int steps, float 
     const int xtiles = int((w + 63) / 64), stiles = int((s + 63) / 64);
     const size_t smem = size_t(2 * xtiles + (split ? 2 : 1) * stiles) * kSmallTile + 1024;
     const uint32_t columns = (w > 128 ? 256 : 128) * (split ? 2 : 1);
-    dispatch_value(grad_type, [&](auto tag) {
-      using V = decltype(tag);
-      auto go = [&](auto mom, auto sp) {
-        auto *kernel = k_newton_schulz_small<V, decltype(mom)::value, decltype(sp)::value>;
+    auto launch = [&](auto grad, auto out, auto mom) {
+      auto start = [&](auto sides) {
+        auto *kernel = k_newton_schulz_small<decltype(grad), decltype(out), decltype(mom)::value, decltype(sides)::value>;
         allow_dynamic_smem(kernel, smem);
-        kernel<<<unsigned(batch), 256, smem, st>>>(u, int(s), int(w), int(transposed), steps, eps, fin, columns, g.status);
+        kernel<<<unsigned(batch), 128 * decltype(sides)::value, smem, st>>>(u, int(s), int(w), int(transposed), steps, eps,
+                                                                            fin, columns, g.status);
       };
-      if (u.momentum.p && split) go(std::true_type{}, std::true_type{});
-      else if (u.momentum.p) go(std::true_type{}, std::false_type{});
-      else if (split) go(std::false_type{}, std::true_type{});
-      else go(std::false_type{}, std::false_type{});
+      if (w > 128) start(std::integral_constant<int, 2>{});
+      else start(std::integral_constant<int, 4>{});
+    };
+    dispatch_value(fin.type, [&](auto out) {
+      if (!fin.update) launch(out, out, std::false_type{});  // an update and its result have one type
+      else if (grad_type == fin.type) launch(out, out, std::true_type{});
+      else launch(F32{}, out, std::true_type{});
     });
     launched("k_newton_schulz_small");
     return;
@@ -1518,6 +1641,8 @@ extern "C" int se_muon_step(int32_t weight_dtype, int32_t grad_dtype, void *weig
   return guarded([&] {
     check_value_dtype(weight_dtype, "weight_dtype");
     check_value_dtype(grad_dtype, "grad_dtype");
+    if (grad_dtype != weight_dtype && grad_dtype != SE_FLOAT32)
+      throw std::invalid_argument("grad_dtype must be weight_dtype or float32");
     check_matrices(batch, m, n, steps, eps);
     if (!std::isfinite(lr) || !std::isfinite(beta) || !std::isfinite(weight_decay) || !std::isfinite(scale))
       throw std::invalid_argument("lr, beta, weight_decay and scale must be finite");
