@@ -14,6 +14,7 @@ be captured into CUDA graphs. `torch_ops` has the autograd forms.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 
 from . import _native as N
@@ -27,6 +28,19 @@ def _code(dtype) -> int:
         torch = torch_mod()
         _FLOATS.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
     return _FLOATS.get(dtype, -1)
+
+
+@functools.lru_cache(maxsize=None)
+def _entry(name: str):
+    """An entry point of the library (looked up once)."""
+    return getattr(N.lib(), name)
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(name: str, *args) -> int:
+    size = C.c_size_t()
+    N.check(_entry(name)(*args, C.byref(size)))
+    return size.value
 
 
 def _cuda_tensor(x, what: str):
@@ -79,24 +93,27 @@ def _same_device(a, b, what: str) -> None:
         raise ValueError(f"{what} is on {b.device}, the call on {a.device}")
 
 
+def _param(x, dim: int, p, what: str):
+    p = _cuda_tensor(p, what)
+    _same_device(x, p, what)
+    if p.dim() != 1 or p.shape[0] != dim or not p.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous 1D tensor of dim values")
+    if p.dtype != x.dtype and p.dtype != torch_mod().float32:
+        raise ValueError(f"{what} must have x's dtype or float32")
+    return p
+
+
 def _affine(x, dim: int, weight, bias):
     if weight is None:
         if bias is not None:
             raise ValueError("bias needs a weight")
         return None, None, 0
-    out = []
-    for p, what in ((weight, "weight"), (bias, "bias")):
-        if p is not None:
-            p = _cuda_tensor(p, what)
-            _same_device(x, p, what)
-            if p.dim() != 1 or p.shape[0] != dim or not p.is_contiguous():
-                raise ValueError(f"{what} must be a contiguous 1D tensor of dim values")
-            if p.dtype != x.dtype and p.dtype != torch_mod().float32:
-                raise ValueError(f"{what} must have x's dtype or float32")
-        out.append(p)
-    if out[1] is not None and out[1].dtype != out[0].dtype:
-        raise ValueError("weight and bias must have the same dtype")
-    return out[0], out[1], _code(out[0].dtype)
+    weight = _param(x, dim, weight, "weight")
+    if bias is not None:
+        bias = _param(x, dim, bias, "bias")
+        if bias.dtype != weight.dtype:
+            raise ValueError("weight and bias must have the same dtype")
+    return weight, bias, _code(weight.dtype)
 
 
 def _ptr(t):
@@ -104,7 +121,8 @@ def _ptr(t):
 
 
 def _stream(t) -> int:
-    return torch_mod().cuda.current_stream(t.device).cuda_stream
+    # what torch.cuda.current_stream(t.device).cuda_stream gives, without building a Stream object
+    return torch_mod()._C._cuda_getCurrentRawStream(t.device.index)
 
 
 def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, return_stats: bool = False):
@@ -119,13 +137,12 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, return_stats: bool 
     eps = float(eps)
     if not math.isfinite(eps) or eps < 0.0:
         raise ValueError("eps must be finite and non-negative")
-    torch = torch_mod()
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = x.new_empty(x.shape)
     mean = rstd = None
     if return_stats:
-        mean, rstd = (torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) for _ in range(2))
-    N.check(N.lib().se_layer_norm(_code(x.dtype), pcode, x.data_ptr(), rows, dim, stride, _ptr(weight), _ptr(bias), eps,
-                                  y.data_ptr(), _ptr(mean), _ptr(rstd), x.device.index, _stream(x)))
+        mean, rstd = (x.new_empty(x.shape[:-1], dtype=torch_mod().float32) for _ in range(2))
+    N.check(_entry("se_layer_norm")(_code(x.dtype), pcode, x.data_ptr(), rows, dim, stride, _ptr(weight), _ptr(bias), eps,
+                                    y.data_ptr(), _ptr(mean), _ptr(rstd), x.device.index, _stream(x)))
     return (y, mean, rstd) if return_stats else y
 
 
@@ -143,25 +160,21 @@ def layer_norm_backward(grad, x, mean, rstd, weight=None, with_bias: bool = True
     rows, dim, stride = _rows(x, "x")
     _, _, gstride = _rows(grad, "grad")
     weight, _, pcode = _affine(x, dim, weight, None)
-    torch = torch_mod()
     for t, what in ((mean, "mean"), (rstd, "rstd")):
-        if not is_torch_tensor(t) or t.dtype != torch.float32 or t.numel() != rows or not t.is_contiguous():
+        if not is_torch_tensor(t) or t.dtype != torch_mod().float32 or t.numel() != rows or not t.is_contiguous():
             raise ValueError(f"{what} must be a contiguous float32 tensor with a value per row")
         _same_device(x, t, what)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dx = x.new_empty(x.shape)
     dw = db = work = None
     nbytes = 0
-    L = N.lib()
     if weight is not None:
-        dw = torch.empty_like(weight)
-        db = torch.empty_like(weight) if with_bias else None
-        size = C.c_size_t()
-        N.check(L.se_layer_norm_backward_workspace(rows, dim, x.device.index, C.byref(size)))
-        nbytes = size.value
-        work = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-    N.check(L.se_layer_norm_backward(_code(x.dtype), pcode, grad.data_ptr(), gstride, x.data_ptr(), stride, rows, dim,
-                                     mean.data_ptr(), rstd.data_ptr(), _ptr(weight), dx.data_ptr(), _ptr(dw), _ptr(db),
-                                     _ptr(work), nbytes, x.device.index, _stream(x)))
+        dw = weight.new_empty(weight.shape)
+        db = weight.new_empty(weight.shape) if with_bias else None
+        nbytes = _workspace_bytes("se_layer_norm_backward_workspace", rows, dim, x.device.index)
+        work = x.new_empty(nbytes, dtype=torch_mod().uint8)
+    N.check(_entry("se_layer_norm_backward")(_code(x.dtype), pcode, grad.data_ptr(), gstride, x.data_ptr(), stride, rows,
+                                             dim, mean.data_ptr(), rstd.data_ptr(), _ptr(weight), dx.data_ptr(),
+                                             _ptr(dw), _ptr(db), _ptr(work), nbytes, x.device.index, _stream(x)))
     return dx, dw, db
 
 
@@ -182,11 +195,9 @@ def _matrices(x, what: str):
     return batch, m, n, (bs if batch > 1 else m * rs), rs
 
 
-def _muon_work(code: int, batch: int, m: int, n: int, device):
-    size = C.c_size_t()
-    N.check(N.lib().se_muon_workspace(code, batch, m, n, C.byref(size)))
-    # torch's allocations are aligned to 512 bytes
-    return torch_mod().empty(size.value, dtype=torch_mod().uint8, device=device), size.value
+def _muon_work(x, batch: int, m: int, n: int):
+    nbytes = _workspace_bytes("se_muon_workspace", _code(x.dtype), batch, m, n)
+    return x.new_empty(nbytes, dtype=torch_mod().uint8), nbytes  # torch's allocations are aligned to 512 bytes
 
 
 def orthogonalize(update, steps: int = 5, eps: float = 1e-7):
@@ -197,12 +208,10 @@ def orthogonalize(update, steps: int = 5, eps: float = 1e-7):
     Returns a new tensor of update's shape and dtype."""
     u = _cuda_tensor(update, "update")
     batch, m, n, bs, rs = _matrices(u, "update")
-    torch = torch_mod()
-    out = torch.empty(u.shape, dtype=u.dtype, device=u.device)
-    code = _code(u.dtype)
-    work, nbytes = _muon_work(code, batch, m, n, u.device)
-    N.check(N.lib().se_orthogonalize(code, u.data_ptr(), batch, m, n, bs, rs, int(steps), float(eps), out.data_ptr(),
-                                     work.data_ptr(), nbytes, u.device.index, _stream(u)))
+    out = u.new_empty(u.shape)
+    work, nbytes = _muon_work(u, batch, m, n)
+    N.check(_entry("se_orthogonalize")(_code(u.dtype), u.data_ptr(), batch, m, n, bs, rs, int(steps), float(eps),
+                                       out.data_ptr(), work.data_ptr(), nbytes, u.device.index, _stream(u)))
     return out
 
 
@@ -241,9 +250,8 @@ def muon_step(weight, grad, momentum, lr: float = 0.02, beta: float = 0.95, weig
             raise ValueError("weight, grad and momentum must not share memory")
     if scale is None:
         scale = math.sqrt(max(1.0, m / n)) if n else 1.0
-    code = _code(w.dtype)
-    work, nbytes = _muon_work(code, batch, m, n, w.device)
-    N.check(N.lib().se_muon_step(code, _code(g.dtype), w.data_ptr(), wbs, wrs, g.data_ptr(), gbs, grs, mom.data_ptr(),
-                                 mbs, mrs, batch, m, n, float(lr), float(beta), float(weight_decay), float(scale),
-                                 int(bool(nesterov)), int(steps), float(eps), work.data_ptr(), nbytes, w.device.index,
-                                 _stream(w)))
+    work, nbytes = _muon_work(w, batch, m, n)
+    N.check(_entry("se_muon_step")(_code(w.dtype), _code(g.dtype), w.data_ptr(), wbs, wrs, g.data_ptr(), gbs, grs,
+                                   mom.data_ptr(), mbs, mrs, batch, m, n, float(lr), float(beta), float(weight_decay),
+                                   float(scale), int(bool(nesterov)), int(steps), float(eps), work.data_ptr(), nbytes,
+                                   w.device.index, _stream(w)))
