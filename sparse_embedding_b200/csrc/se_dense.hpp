@@ -57,4 +57,48 @@ inline int sm_count(int device) {
   return known[device] = n;
 }
 
+// Blocks of a kernel that run on a multiprocessor at once (asked once per
+// device, block and shared memory).
+template <class... KArgs>
+inline int resident_blocks(void (*kernel)(KArgs...), int device, int threads, size_t smem) {
+  using Key = std::pair<std::pair<const void *, int>, std::pair<int, size_t>>;
+  static std::mutex mu;
+  static std::map<Key, int> known;
+  const Key key{{reinterpret_cast<const void *>(kernel), device}, {threads, smem}};
+  std::lock_guard<std::mutex> lock(mu);
+  auto it = known.find(key);
+  if (it != known.end()) return it->second;
+  int n = 0;
+  cuda_check(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem), "occupancy");
+  return known[key] = n < 1 ? 1 : n;
+}
+
+// A word in host memory that a kernel sets when one of its waits for a copy gave
+// up. The next call on the device reads it, without waiting for the GPU, and
+// reports it. (The word is allocated by the device's first call, which may be
+// under stream capture.)
+inline uint32_t *wait_status(int device) {
+  static std::mutex mu;
+  static std::map<int, uint32_t *> known;
+  std::lock_guard<std::mutex> lock(mu);
+  uint32_t *&word = known[device];
+  if (word == nullptr) {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cuda_check(cudaThreadExchangeStreamCaptureMode(&mode), "cudaThreadExchangeStreamCaptureMode");
+    void *p = nullptr;
+    const cudaError_t e = cudaHostAlloc(&p, sizeof(uint32_t), cudaHostAllocMapped | cudaHostAllocPortable);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    cuda_check(e, "cudaHostAlloc");
+    *static_cast<volatile uint32_t *>(p) = 0u;
+    word = static_cast<uint32_t *>(p);
+  }
+  volatile uint32_t *seen = word;
+  if (*seen != 0u) {
+    *seen = 0u;
+    throw Error(SE_ERR_RUNTIME, "an earlier layer normalisation or Muon update on cuda:" + std::to_string(device) +
+                                    " gave up waiting for its copies; its results are not valid");
+  }
+  return word;
+}
+
 }  // namespace se_gpu

@@ -1292,25 +1292,6 @@ k_newton_schulz_small(UpdateArgs a, int s, int w, int transposed, int steps, flo
 // Host side
 // ---------------------------------------------------------------------------
 
-// A word in host memory that a product sets when a wait gave up; the next call
-// on the device reads it without waiting for the GPU.
-uint32_t *ns_status(int device) {
-  static std::mutex mu;
-  static std::map<int, uint32_t *> known;
-  std::lock_guard<std::mutex> lock(mu);
-  auto it = known.find(device);
-  if (it != known.end()) return it->second;
-  // an allocation is allowed while another stream, or this one, is being captured
-  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-  cuda_check(cudaThreadExchangeStreamCaptureMode(&mode), "cudaThreadExchangeStreamCaptureMode");
-  void *p = nullptr;
-  const cudaError_t e = cudaHostAlloc(&p, sizeof(uint32_t), cudaHostAllocMapped | cudaHostAllocPortable);
-  cudaThreadExchangeStreamCaptureMode(&mode);
-  cuda_check(e, "cudaHostAlloc");
-  *static_cast<volatile uint32_t *>(p) = 0u;
-  return known[device] = static_cast<uint32_t *>(p);
-}
-
 using EncodeTiled = decltype(&cuTensorMapEncodeTiled);
 EncodeTiled encode_tiled() {
   static EncodeTiled fn = [] {
@@ -1483,12 +1464,7 @@ void orthogonalise(UpdateArgs u, int grad_type, int64_t batch, int steps, float 
   g.square = cut(true, s, s, 1);
   g.apply = cut(false, w, s, 1);
   const int sms = sm_count(device);
-  g.status = ns_status(device);
-  if (*static_cast<volatile uint32_t *>(g.status) != 0u) {
-    *static_cast<volatile uint32_t *>(g.status) = 0u;
-    throw Error(SE_ERR_RUNTIME, "an earlier orthogonalisation on cuda:" + std::to_string(device) +
-                                    " gave up waiting for its copies; its results are not valid");
-  }
+  g.status = wait_status(device);
   fin.transposed = transposed;
   if (s <= kSmallSide && w <= kSmallWide) {
     const int xtiles = int((w + 63) / 64), stiles = int((s + 63) / 64);

@@ -25,6 +25,7 @@
 
 #include "se_common.cuh"
 #include "se_dense.hpp"
+#include "se_tcgen05.cuh"
 
 namespace se_gpu {
 
@@ -36,6 +37,7 @@ constexpr int kNormNarrowThreads = 256;  // block of the kernels with several ro
 // values per column besides the row).
 constexpr __host__ __device__ int norm_wide_threads(int vec) { return vec == 1 ? 1024 : 512; }
 constexpr __host__ __device__ int norm_wide_loads(int vec) { return vec == 1 ? 8 : 16 / vec; }
+constexpr __host__ __device__ int norm_wide_rows(int vec) { return vec == 1 ? 1 : 2; }
 
 // VEC values of a row: one 16-byte load where the layout allows it, else one value.
 template <class V, int VEC>
@@ -86,39 +88,226 @@ __device__ __forceinline__ void param_put(void *p, int type, int64_t i, float f)
   else static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(f);
 }
 
-// Sums of N values over the threads of a row: xor shuffles within the warp's
-// part, and for a whole block (WIDE) one exchange through shared memory.
+// Two fp32 operations in one instruction, where a vector has pairs.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 z, x, y;\n mov.b64 {%0, %1}, z;\n}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 z, x, y;\n mov.b64 {%0, %1}, z;\n}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n .reg .b64 x, y, z, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
+      " fma.rn.f32x2 w, x, y, z;\n mov.b64 {%0, %1}, w;\n}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+// o = a + b, a b, a b + c on vectors; `all` is a value for every element.
+template <int N> __device__ __forceinline__ void vadd(float (&o)[N], const float (&a)[N], const float (&b)[N]) {
+  if constexpr (N == 1) o[0] = a[0] + b[0];
+  else
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const float2 r = add2({a[i], a[i + 1]}, {b[i], b[i + 1]});
+      o[i] = r.x;
+      o[i + 1] = r.y;
+    }
+}
+template <int N> __device__ __forceinline__ void vmul(float (&o)[N], const float (&a)[N], const float (&b)[N]) {
+  if constexpr (N == 1) o[0] = a[0] * b[0];
+  else
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const float2 r = mul2({a[i], a[i + 1]}, {b[i], b[i + 1]});
+      o[i] = r.x;
+      o[i + 1] = r.y;
+    }
+}
+template <int N>
+__device__ __forceinline__ void vfma(float (&o)[N], const float (&a)[N], const float (&b)[N], const float (&c)[N]) {
+  if constexpr (N == 1) o[0] = __fmaf_rn(a[0], b[0], c[0]);
+  else
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const float2 r = fma2({a[i], a[i + 1]}, {b[i], b[i + 1]}, {c[i], c[i + 1]});
+      o[i] = r.x;
+      o[i + 1] = r.y;
+    }
+}
+template <int N> struct All {
+  float v[N];
+  __device__ __forceinline__ explicit All(float f) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = f;
+  }
+};
+template <int N> __device__ __forceinline__ float vsum(const float (&a)[N]) {
+  if constexpr (N == 1) {
+    return a[0];
+  } else if constexpr (N == 2) {
+    return a[0] + a[1];
+  } else {
+    float h[N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; i += 2) {
+      const float2 r = add2({a[i], a[i + 1]}, {a[N / 2 + i], a[N / 2 + i + 1]});
+      h[i] = r.x;
+      h[i + 1] = r.y;
+    }
+    return vsum(h);
+  }
+}
+
+// Sums of N values over the threads of a row, in every one of them.
+//
+// Within a warp's part (`lanes` threads), N > 1 rows at a time: in the first
+// steps a thread gives away half of the values it holds and adds to the other
+// half, until it holds one; the rest are plain xor steps on that one, and the
+// sums go back by one shuffle each (N = 4 over 32 lanes: 10 shuffles for 20).
+// For a whole block (WIDE) an exchange through shared memory follows.
 // Successive exchanges alternate between two buffers, so one barrier each is
 // enough: a buffer is written again only after the next exchange's barrier.
 template <int N, bool WIDE>
 struct RowSum {
+  static_assert(N == 1 || N == 2 || N == 4, "a power of two");
   int lanes;
-  float (*buf)[32][2];  // [2][32][2]
+  float (*buf)[32][4];  // [2][32][4]
   int phase = 0;
   __device__ __forceinline__ void operator()(float (&v)[N]) {
+    const int lane = int(threadIdx.x) & 31, part = lanes < 32 ? lanes : 32;
+    constexpr unsigned kAll = 0xffffffffu;
+    if (N == 1 || part < N) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      if (o < lanes) {
+      for (int o = 16; o > 0; o >>= 1) {
+        if (o < part) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+          for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(kAll, v[i], o);
+        }
       }
+    } else {
+      const int half = part >> 1, quarter = part >> 2;
+      float one;
+      int rest;
+      if constexpr (N == 4) {
+        const bool up = lane & half, upper = lane & quarter;
+        const float a = (up ? v[2] : v[0]) + __shfl_xor_sync(kAll, up ? v[0] : v[2], half);
+        const float b = (up ? v[3] : v[1]) + __shfl_xor_sync(kAll, up ? v[1] : v[3], half);
+        one = (upper ? b : a) + __shfl_xor_sync(kAll, upper ? a : b, quarter);
+        rest = quarter;
+      } else {
+        const bool up = lane & half;
+        one = (up ? v[N - 1] : v[0]) + __shfl_xor_sync(kAll, up ? v[0] : v[N - 1], half);
+        rest = half;
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1)
+        if (o < rest) one += __shfl_xor_sync(kAll, one, o);
+      const int first = lane & ~(part - 1);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        v[i] = __shfl_sync(kAll, one, first + (N == 4 ? (i >> 1) * half + (i & 1) * quarter : i * half));
     }
     if constexpr (WIDE) {
-      static_assert(N <= 2, "two values per exchange");
-      const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+      const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
       if (lane == 0) {
 #pragma unroll
         for (int i = 0; i < N; ++i) buf[phase][warp][i] = v[i];
       }
       __syncthreads();
+      const bool whole = (warps & (warps - 1)) == 0;  // a power of two: every lane's steps see all warps
+      const int from = whole ? lane & (warps - 1) : lane;
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = lane < warps ? buf[phase][lane][i] : 0.0f;
+      for (int i = 0; i < N; ++i) v[i] = from < warps ? buf[phase][from][i] : 0.0f;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
+        if (o < warps) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+          for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(kAll, v[i], o);
+        }
+      }
+      if (!whole) {  // lane 0's saw all
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = __shfl_sync(kAll, v[i], 0);
       }
       phase ^= 1;
+    }
+  }
+};
+
+// Tiles of rows on their way through shared memory, by bulk copies (one per
+// tile where the rows have no gaps, else one per row) into STAGES buffers of
+// `rows` rows for each of N arrays. The loads of a block are so several tiles
+// deep, whatever registers its threads have left. Buffer k's tile is ready when
+// its barrier completes a phase; a wait that gives up makes the block leave.
+constexpr int kNormStages = 4;
+template <class T, int N>
+struct RowRing {
+  const T *src[N];
+  int64_t stride[N];
+  int64_t rows_total, step;  // rows of the matrix, rows between two tiles of this block
+  int rows, dim, stages;
+  T *buf;
+  uint64_t *bars;
+  volatile uint32_t *given_up;
+  int at = 0;
+  uint32_t parity = 0;
+
+  __device__ __forceinline__ T *tile(int stage, int n) const { return buf + (int64_t(stage) * N + n) * rows * dim; }
+  __device__ __forceinline__ void fill(int stage, int64_t base) const {  // one thread
+    const int64_t left = rows_total - base;
+    const int count = int(left < rows ? left : rows);
+    if (count <= 0) return;
+    const uint32_t row_bytes = uint32_t(dim * sizeof(T));
+    mbar_arrive_expect_tx(&bars[stage], uint32_t(count) * row_bytes * N);
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const T *from = src[n] + base * stride[n];
+      if (stride[n] == dim) {
+        bulk_copy_g2s(tile(stage, n), from, uint32_t(count) * row_bytes, &bars[stage]);
+      } else {
+        for (int r = 0; r < count; ++r)
+          bulk_copy_g2s(tile(stage, n) + int64_t(r) * dim, from + r * stride[n], row_bytes, &bars[stage]);
+      }
+    }
+  }
+  __device__ __forceinline__ void start(int64_t base) {
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < stages; ++i) mbar_init(&bars[i], 1);
+      *given_up = 0u;
+      for (int i = 0; i < stages; ++i) fill(i, base + i * step);
+    }
+    __syncthreads();
+  }
+  __device__ __forceinline__ bool ready() const { return wait_or_give_up(&bars[at], parity, given_up); }
+  // The tile has been read by all threads (a barrier lies between): refill its buffer.
+  __device__ __forceinline__ void next(int64_t base) {
+    if (threadIdx.x == 0) fill(at, base + stages * step);
+    if (++at == stages) {
+      at = 0;
+      parity ^= 1u;
+    }
+  }
+  // After a wait that gave up: the copies still in flight.
+  __device__ __forceinline__ void drain(int64_t base, uint32_t *status) {
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < stages; ++i) {
+        if (base + i * step < rows_total) wait_for(&bars[at], parity, nullptr);
+        if (++at == stages) {
+          at = 0;
+          parity ^= 1u;
+        }
+      }
+      *reinterpret_cast<volatile uint32_t *>(status) = 1u;
+      __threadfence_system();
     }
   }
 };
@@ -127,12 +316,18 @@ struct RowSum {
 // with WIDE the block), NV vectors of VEC values per thread, U rows at a time
 // (their loads are in flight together).
 template <class V, int VEC, int NV, int U, bool WIDE>
-__global__ void __launch_bounds__(WIDE ? norm_wide_threads(VEC) : kNormNarrowThreads)
+__global__ void __launch_bounds__(WIDE ? norm_wide_threads(VEC) : kNormNarrowThreads, !WIDE && NV == 1 ? 3 : 1)
 k_norm_forward(const typename V::T *__restrict__ x, int64_t x_stride, int64_t rows, int dim,
                const void *__restrict__ weight, const void *__restrict__ bias, int ptype, float eps,
-               typename V::T *__restrict__ y, float *__restrict__ mean_out, float *__restrict__ rstd_out, int lanes) {
+               typename V::T *__restrict__ y, float *__restrict__ mean_out, float *__restrict__ rstd_out, int lanes,
+               int stages, uint32_t *status) {
   using P = Pack<V, VEC>;
-  __shared__ float red[2][32][2];
+  using T = typename V::T;
+  constexpr bool kRing = VEC > 1;
+  __shared__ float red[2][32][4];
+  __shared__ uint64_t bars[kNormStages];
+  __shared__ volatile uint32_t given_up;
+  extern __shared__ __align__(128) uint8_t raw_smem[];
   const int lane = WIDE ? int(threadIdx.x) : int(threadIdx.x) & (lanes - 1);
   const int group = WIDE ? 0 : int(threadIdx.x) / lanes;
   const int groups = WIDE ? 1 : int(blockDim.x) / lanes;
@@ -148,65 +343,91 @@ k_norm_forward(const typename V::T *__restrict__ x, int64_t x_stride, int64_t ro
   }
   RowSum<U, WIDE> sum{lanes, red};
   const float inv = 1.0f / float(dim);
-  for (int64_t base = int64_t(blockIdx.x) * groups * U; base < rows; base += int64_t(gridDim.x) * groups * U) {
+  const int64_t first = int64_t(blockIdx.x) * groups * U, step = int64_t(gridDim.x) * groups * U;
+  RowRing<T, 1> ring{{x}, {x_stride}, rows, step, groups * U, dim, stages, reinterpret_cast<T *>(raw_smem), bars, &given_up};
+  if constexpr (kRing) ring.start(first);
+  for (int64_t base = first; base < rows; base += step) {
     typename P::Raw raw[U][NV];
+    const bool ok = kRing ? ring.ready() : true;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t row = base + group * U + u;
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
         const int c = (v * lanes + lane) * VEC;
-        raw[u][v] = row < rows && c < dim ? P::load(x + row * x_stride + c) : P::zero();
+        const bool in = row < rows && c < dim;
+        if constexpr (kRing) raw[u][v] = in ? P::load(ring.tile(ring.at, 0) + (group * U + u) * dim + c) : P::zero();
+        else raw[u][v] = in ? P::load(x + row * x_stride + c) : P::zero();
       }
     }
-    float m[U], s[U];
+    if constexpr (kRing) {
+      if (__syncthreads_or(!ok)) {
+        ring.drain(base, status);
+        return;
+      }
+      ring.next(base);
+    }
+    // values beyond the row are zeros, and zeros again after the mean is taken off
+    float f[U][NV][VEC], m[U], s[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      m[u] = 0.0f;
+      float t[VEC];
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
-        float f[VEC];
-        P::open(raw[u][v], f);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) m[u] += f[i];
+        P::open(raw[u][v], f[u][v]);
+        if (v == 0) P::open(raw[u][0], t);
+        else vadd(t, t, f[u][v]);
       }
+      m[u] = vsum(t);
     }
     sum(m);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       m[u] *= inv;
-      s[u] = 0.0f;
+      const All<VEC> minus(-m[u]);
+      float t[VEC];
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
-        float f[VEC];
-        P::open(raw[u][v], f);
-        if ((v * lanes + lane) * VEC < dim) {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            const float d = f[i] - m[u];
-            s[u] = __fmaf_rn(d, d, s[u]);
-          }
-        }
+        if ((v * lanes + lane) * VEC < dim) vadd(f[u][v], f[u][v], minus.v);
+        if (v == 0) vmul(t, f[u][v], f[u][v]);
+        else vfma(t, f[u][v], f[u][v], t);
       }
+      s[u] = vsum(t);
     }
     sum(s);
+#pragma unroll
+    for (int u = 0; u < U; ++u) s[u] = __fmaf_rn(s[u], inv, eps);
+    if constexpr (U == 1) {
+      s[0] = 1.0f / sqrtf(s[0]);
+    } else {  // a thread takes the root and the quotient of one of the rows (part of a row of `lanes` >= U threads)
+      if (lanes < U) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) s[u] = 1.0f / sqrtf(s[u]);
+      } else {
+        float one = s[0];
+#pragma unroll
+        for (int u = 1; u < U; ++u) one = (lane & (U - 1)) == u ? s[u] : one;
+        one = 1.0f / sqrtf(one);
+        const int from = (int(threadIdx.x) & 31) & ~(U - 1);
+#pragma unroll
+        for (int u = 0; u < U; ++u) s[u] = __shfl_sync(0xffffffffu, one, from + u);
+      }
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t row = base + group * U + u;
       if (row >= rows) continue;
-      const float r = 1.0f / sqrtf(s[u] * inv + eps);
       if (lane == 0) {
         if (mean_out) mean_out[row] = m[u];
-        if (rstd_out) rstd_out[row] = r;
+        if (rstd_out) rstd_out[row] = s[u];
       }
+      const All<VEC> r(s[u]);
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
         const int c = (v * lanes + lane) * VEC;
-        float f[VEC];
-        P::open(raw[u][v], f);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) f[i] = __fmaf_rn((f[i] - m[u]) * r, w[v][i], b[v][i]);
-        if (c < dim) P::store(y + row * dim + c, f);
+        vmul(f[u][v], f[u][v], r.v);
+        vfma(f[u][v], f[u][v], w[v], b[v]);
+        if (c < dim) P::store(y + row * dim + c, f[u][v]);
       }
     }
   }
@@ -219,7 +440,7 @@ __global__ void __launch_bounds__(512)
 k_norm_forward_long(const typename V::T *__restrict__ x, int64_t x_stride, int64_t rows, int64_t dim,
                     const void *__restrict__ weight, const void *__restrict__ bias, int ptype, float eps,
                     typename V::T *__restrict__ y, float *__restrict__ mean_out, float *__restrict__ rstd_out) {
-  __shared__ float red[2][32][2];
+  __shared__ float red[2][32][4];
   RowSum<1, true> sum{32, red};
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const typename V::T *xr = x + row * x_stride;
@@ -251,10 +472,15 @@ __global__ void __launch_bounds__(WIDE ? norm_wide_threads(VEC) : kNormNarrowThr
 k_norm_backward(const typename V::T *__restrict__ grad, int64_t g_stride, const typename V::T *__restrict__ x,
                 int64_t x_stride, int64_t rows, int dim, const float *__restrict__ mean,
                 const float *__restrict__ rstd, const void *__restrict__ weight, int ptype,
-                typename V::T *__restrict__ dx, float *__restrict__ partial, int lanes) {
+                typename V::T *__restrict__ dx, float *__restrict__ partial, int lanes, int stages,
+                uint32_t *status) {
   using P = Pack<V, VEC>;
-  __shared__ float red[2][32][2];
-  extern __shared__ float cols[];  // narrow: [warps][dim]
+  using T = typename V::T;
+  constexpr bool kRing = VEC > 1;
+  __shared__ float red[2][32][4];
+  __shared__ uint64_t bars[kNormStages];
+  __shared__ volatile uint32_t given_up;
+  extern __shared__ __align__(128) uint8_t raw_smem[];  // the ring; at the end, narrow: [warps][dim] fp32
   const int lane = WIDE ? int(threadIdx.x) : int(threadIdx.x) & (lanes - 1);
   const int group = WIDE ? 0 : int(threadIdx.x) / lanes;
   const int groups = WIDE ? 1 : int(blockDim.x) / lanes;
@@ -269,11 +495,16 @@ k_norm_backward(const typename V::T *__restrict__ grad, int64_t g_stride, const 
       db[v][i] = 0.0f;
     }
   }
-  RowSum<2, WIDE> sum{lanes, red};
+  RowSum<WIDE ? 2 * U : U, WIDE> sum{lanes, red};
   const float inv = 1.0f / float(dim);
-  for (int64_t base = int64_t(blockIdx.x) * groups * U; base < rows; base += int64_t(gridDim.x) * groups * U) {
+  const int64_t first = int64_t(blockIdx.x) * groups * U, step = int64_t(gridDim.x) * groups * U;
+  RowRing<T, 2> ring{{x, grad}, {x_stride, g_stride}, rows, step, groups * U, dim, stages,
+                     reinterpret_cast<T *>(raw_smem), bars, &given_up};
+  if constexpr (kRing) ring.start(first);
+  for (int64_t base = first; base < rows; base += step) {
     typename P::Raw xr[U][NV], gr[U][NV];
     float m[U], r[U];
+    const bool ok = kRing ? ring.ready() : true;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t row = base + group * U + u;
@@ -283,50 +514,85 @@ k_norm_backward(const typename V::T *__restrict__ grad, int64_t g_stride, const 
       for (int v = 0; v < NV; ++v) {
         const int c = (v * lanes + lane) * VEC;
         const bool in = row < rows && c < dim;
-        xr[u][v] = in ? P::load(x + row * x_stride + c) : P::zero();
-        gr[u][v] = in ? P::load(grad + row * g_stride + c) : P::zero();
+        if constexpr (kRing) {
+          const int at = (group * U + u) * dim + c;
+          xr[u][v] = in ? P::load(ring.tile(ring.at, 0) + at) : P::zero();
+          gr[u][v] = in ? P::load(ring.tile(ring.at, 1) + at) : P::zero();
+        } else {
+          xr[u][v] = in ? P::load(x + row * x_stride + c) : P::zero();
+          gr[u][v] = in ? P::load(grad + row * g_stride + c) : P::zero();
+        }
       }
+    }
+    if constexpr (kRing) {
+      if (__syncthreads_or(!ok)) {
+        ring.drain(base, status);
+        return;
+      }
+      ring.next(base);
+    }
+    // rows and columns beyond the matrix have r, g and w zero: they add nothing
+    float s0[U], s1[U], both[2 * U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const All<VEC> rr(r[u]), mr(-m[u] * r[u]);
+      float t0[VEC], t1[VEC];
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        float h[VEC], g[VEC], q[VEC];
+        P::open(xr[u][v], h);
+        P::open(gr[u][v], g);
+        vfma(h, h, rr.v, mr.v);
+        vmul(q, g, w[v]);
+        if (v == 0) {
+          vmul(t0, g, w[v]);
+          vmul(t1, q, h);
+        } else {
+          vadd(t0, t0, q);
+          vfma(t1, q, h, t1);
+        }
+        vfma(dw[v], g, h, dw[v]);
+        vadd(db[v], db[v], g);
+      }
+      s0[u] = vsum(t0);
+      s1[u] = vsum(t1);
+    }
+    if constexpr (WIDE) {  // one exchange for both
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        both[2 * u] = s0[u];
+        both[2 * u + 1] = s1[u];
+      }
+      sum(both);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        s0[u] = both[2 * u];
+        s1[u] = both[2 * u + 1];
+      }
+    } else {
+      sum(s0);
+      sum(s1);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t row = base + group * U + u;
-      float s[2] = {0.0f, 0.0f};
+      if (row >= rows) continue;
+      const All<VEC> rr(r[u]), mr(-m[u] * r[u]), c0(-r[u] * (s0[u] * inv)), c1(-r[u] * (s1[u] * inv));
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
-        if (row < rows && (v * lanes + lane) * VEC < dim) {
-          float xf[VEC], gf[VEC];
-          P::open(xr[u][v], xf);
-          P::open(gr[u][v], gf);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            const float h = (xf[i] - m[u]) * r[u], q = gf[i] * w[v][i];
-            s[0] += q;
-            s[1] = __fmaf_rn(q, h, s[1]);
-            dw[v][i] = __fmaf_rn(gf[i], h, dw[v][i]);
-            db[v][i] += gf[i];
-          }
-        }
-      }
-      sum(s);
-      s[0] *= inv;
-      s[1] *= inv;
-      if (row < rows) {
-#pragma unroll
-        for (int v = 0; v < NV; ++v) {
-          const int c = (v * lanes + lane) * VEC;
-          float xf[VEC], gf[VEC];
-          P::open(xr[u][v], xf);
-          P::open(gr[u][v], gf);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            const float h = (xf[i] - m[u]) * r[u];
-            gf[i] = r[u] * (__fmaf_rn(gf[i], w[v][i], -s[0]) - h * s[1]);
-          }
-          if (c < dim) P::store(dx + row * dim + c, gf);
-        }
+        const int c = (v * lanes + lane) * VEC;
+        float h[VEC], g[VEC];
+        P::open(xr[u][v], h);
+        P::open(gr[u][v], g);
+        vfma(h, h, rr.v, mr.v);
+        vmul(g, g, w[v]);
+        vfma(g, g, rr.v, c0.v);  // r q - r sum q / D - h r sum(q h) / D
+        vfma(g, h, c1.v, g);
+        if (c < dim) P::store(dx + row * dim + c, g);
       }
     }
   }
+  pdl_trigger();  // the column kernel's blocks may come as this grid's leave
   if (partial == nullptr) return;
   float *out = partial + int64_t(blockIdx.x) * 2 * dim;
   if constexpr (WIDE) {
@@ -343,6 +609,8 @@ k_norm_backward(const typename V::T *__restrict__ grad, int64_t g_stride, const 
     }
   } else {
     // the warp's row groups by shuffles, then the block's warps in warp order
+    float *cols = reinterpret_cast<float *>(raw_smem);
+    __syncthreads();
     const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -376,7 +644,7 @@ k_norm_backward_long(const typename V::T *__restrict__ grad, int64_t g_stride, c
                      int64_t x_stride, int64_t rows, int64_t dim, const float *__restrict__ mean,
                      const float *__restrict__ rstd, const void *__restrict__ weight, int ptype,
                      typename V::T *__restrict__ dx) {
-  __shared__ float red[2][32][2];
+  __shared__ float red[2][32][4];
   RowSum<2, true> sum{32, red};
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const typename V::T *xr = x + row * x_stride, *gr = grad + row * g_stride;
@@ -418,25 +686,25 @@ k_norm_columns_long(const typename V::T *__restrict__ grad, int64_t g_stride, co
 }
 
 // dw and db: the blocks' sums of each column, added in a fixed order (each of
-// the 16 threads of a column takes every 16th block, then the 16 in order).
-__global__ void __launch_bounds__(512)
+// the 32 threads of a column takes every 32nd block, then the 32 in order).
+__global__ void __launch_bounds__(1024)
 k_norm_columns(const float *__restrict__ partial, int blocks, int64_t dim, void *__restrict__ dweight,
                void *__restrict__ dbias, int ptype) {
-  __shared__ float part[16][33];
+  __shared__ float part[32][33];
   const int lane = threadIdx.x & 31, strip = threadIdx.x >> 5;
   const int64_t c = int64_t(blockIdx.x) * 32 + lane;
   pdl_wait();
   float f = 0.0f;
   if (c < 2 * dim) {
-#pragma unroll 4
-    for (int k = strip; k < blocks; k += 16) f += partial[int64_t(k) * 2 * dim + c];
+#pragma unroll 8
+    for (int k = strip; k < blocks; k += 32) f += __ldcg(partial + int64_t(k) * 2 * dim + c);
   }
   part[strip][lane] = f;
   __syncthreads();
   if (strip == 0 && c < 2 * dim) {
     f = 0.0f;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) f += part[k][lane];
+    for (int k = 0; k < 32; ++k) f += part[k][lane];
     if (c < dim) {
       if (dweight) param_put(dweight, ptype, c, f);
     } else if (dbias) {
@@ -446,6 +714,12 @@ k_norm_columns(const float *__restrict__ partial, int blocks, int64_t dim, void 
 }
 
 constexpr int kNormLongSplits = 64;
+
+// A launch of the register kernels: their blocks, buffers and shared memory.
+struct NormLaunch {
+  int blocks, stages;
+  size_t smem;
+};
 
 // How a call's rows are laid over threads.
 struct NormShape {
@@ -469,7 +743,7 @@ NormShape norm_shape(int64_t dim, size_t value_size, bool aligned) {
     return s;
   }
   s.nv = norm_wide_loads(s.vec ? per : 1);
-  s.unroll = 1;
+  s.unroll = norm_wide_rows(s.vec ? per : 1);
   s.wide = true;
   const int64_t threads = (n + s.nv - 1) / s.nv;
   const int most = norm_wide_threads(s.vec ? per : 1);
@@ -482,9 +756,30 @@ NormShape norm_shape(int64_t dim, size_t value_size, bool aligned) {
 // Most blocks of the register kernels: `sms` x 1,024 threads. More
 // blocks would add sums to the workspace and to the second kernel.
 int norm_blocks(int64_t rows, const NormShape &s, int sms) {
-  const int64_t per_block = s.wide ? 1 : int64_t(s.threads / s.lanes) * s.unroll;
+  const int64_t per_block = int64_t(s.threads / s.lanes) * s.unroll;
   const int64_t need = (rows + per_block - 1) / per_block;
   return int(std::max<int64_t>(1, std::min<int64_t>(need, int64_t(sms) * (1024 / s.threads))));
+}
+
+// The ring of a block takes at most 48 KB per array (two blocks of the backward,
+// four of the forward on an SM, with 128 KB or more of loads in flight there),
+// and the grid is what runs at once.
+template <class K>
+NormLaunch norm_launch(K *kernel, const NormShape &s, int64_t rows, int64_t dim, size_t value_size, int arrays,
+                       int device, size_t least_smem) {
+  const int sms = sm_count(device);
+  NormLaunch l{};
+  const int64_t tile_rows = int64_t(s.threads / s.lanes) * s.unroll;
+  if (s.vec) {
+    const size_t tile = size_t(tile_rows) * size_t(dim) * value_size * arrays;
+    l.stages = int(std::max<size_t>(2, std::min<size_t>(kNormStages, size_t(49152) * arrays / tile)));
+    if (tile * l.stages > 200 * 1024) l.stages = 1;  // two rows of 8,192 fp32 values of both arrays
+    l.smem = tile * l.stages;
+  }
+  l.smem = std::max(l.smem, least_smem);
+  allow_dynamic_smem(kernel, l.smem);
+  l.blocks = std::min(norm_blocks(rows, s, sms), sms * resident_blocks(kernel, device, s.threads, l.smem));
+  return l;
 }
 
 // f with the kernel's constants: values per load, loads per thread, rows at a
@@ -494,7 +789,7 @@ void with_norm_shape(const NormShape &s, F &&f) {
   using std::integral_constant;
   auto go = [&](auto vec) {
     constexpr int kVec = decltype(vec)::value;
-    if (s.wide) f(vec, integral_constant<int, norm_wide_loads(kVec)>{}, integral_constant<int, 1>{}, std::true_type{});
+    if (s.wide) f(vec, integral_constant<int, norm_wide_loads(kVec)>{}, integral_constant<int, norm_wide_rows(kVec)>{}, std::true_type{});
     else if (s.nv == 1) f(vec, integral_constant<int, 1>{}, integral_constant<int, 4>{}, std::false_type{});
     else if (s.nv == 2) f(vec, integral_constant<int, 2>{}, integral_constant<int, 2>{}, std::false_type{});
     else f(vec, integral_constant<int, 4>{}, integral_constant<int, 1>{}, std::false_type{});
@@ -534,6 +829,7 @@ extern "C" int se_layer_norm(int32_t value_dtype, int32_t param_dtype, const voi
     check_device_ptr(rstd_out, device, "rstd", true);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int sms = sm_count(device);
+    uint32_t *status = wait_status(device);
     const size_t vb = value_bytes(value_dtype);
     const NormShape s = norm_shape(dim, vb, aligned16(x) && aligned16(y) && (rows == 1 || x_stride * vb % 16 == 0));
     dispatch_value(value_dtype, [&](auto tag) {
@@ -548,11 +844,11 @@ extern "C" int se_layer_norm(int32_t value_dtype, int32_t param_dtype, const voi
         launched("k_norm_forward_long");
         return;
       }
-      const int grid = norm_blocks(int64_t(rows), s, sms * 2);
       with_norm_shape<V>(s, [&](auto vec, auto nv, auto u, auto wide) {
-        k_norm_forward<V, decltype(vec)::value, decltype(nv)::value, decltype(u)::value, decltype(wide)::value>
-            <<<grid, s.threads, 0, st>>>(xp, x_stride, int64_t(rows), int(dim), weight, bias, param_dtype, eps, yp,
-                                         mean_out, rstd_out, s.lanes);
+        auto *kernel = k_norm_forward<V, decltype(vec)::value, decltype(nv)::value, decltype(u)::value, decltype(wide)::value>;
+        const NormLaunch l = norm_launch(kernel, s, int64_t(rows), dim, vb, 1, device, 0);
+        kernel<<<l.blocks, s.threads, l.smem, st>>>(xp, x_stride, int64_t(rows), int(dim), weight, bias, param_dtype, eps,
+                                                    yp, mean_out, rstd_out, s.lanes, l.stages, status);
       });
       launched("k_norm_forward");
     });
@@ -591,6 +887,7 @@ extern "C" int se_layer_norm_backward(int32_t value_dtype, int32_t param_dtype, 
     check_device_ptr(dbias, device, "dbias", true);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int sms = sm_count(device);
+    uint32_t *status = wait_status(device);
     const bool sums = dweight != nullptr || dbias != nullptr;
     int blocks = 0;
     float *partial = nullptr;
@@ -630,16 +927,18 @@ extern "C" int se_layer_norm_backward(int32_t value_dtype, int32_t param_dtype, 
           return;
         }
         with_norm_shape<V>(s, [&](auto vec, auto nv, auto u, auto wide) {
-            const size_t smem = s.wide || !sums ? 0 : size_t(s.threads / 32) * size_t(dim) * sizeof(float);
-          k_norm_backward<V, decltype(vec)::value, decltype(nv)::value, decltype(u)::value, decltype(wide)::value>
-              <<<blocks, s.threads, smem, st>>>(gp, grad_stride, xp, x_stride, int64_t(rows), int(dim), mean, rstd,
-                                                weight, param_dtype, dxp, partial, s.lanes);
+            auto *kernel = k_norm_backward<V, decltype(vec)::value, decltype(nv)::value, decltype(u)::value, decltype(wide)::value>;
+          const size_t cols = s.wide || !sums ? 0 : size_t(s.threads / 32) * size_t(dim) * sizeof(float);
+          const NormLaunch l = norm_launch(kernel, s, int64_t(rows), dim, vb, 2, device, cols);
+          blocks = l.blocks;
+          kernel<<<blocks, s.threads, l.smem, st>>>(gp, grad_stride, xp, x_stride, int64_t(rows), int(dim), mean, rstd,
+                                                    weight, param_dtype, dxp, partial, s.lanes, l.stages, status);
         });
         launched("k_norm_backward");
       });
     }
     if (sums) {
-      pdl(k_norm_columns, unsigned((2 * dim + 31) / 32), 512, 0, st, static_cast<const float *>(partial), blocks, dim,
+      pdl(k_norm_columns, unsigned((2 * dim + 31) / 32), 1024, 0, st, static_cast<const float *>(partial), blocks, dim,
           dweight, dbias, int(param_dtype));
       count_launch();
     }
