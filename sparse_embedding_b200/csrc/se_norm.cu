@@ -37,7 +37,11 @@ constexpr int kNormNarrowThreads = 256;  // block of the kernels with several ro
 // values per column besides the row).
 constexpr __host__ __device__ int norm_wide_threads(int vec) { return vec == 1 ? 1024 : 512; }
 constexpr __host__ __device__ int norm_wide_loads(int vec) { return vec == 1 ? 8 : 16 / vec; }
-constexpr __host__ __device__ int norm_wide_rows(int vec) { return vec == 1 ? 1 : 2; }
+// Rows at a time there. Forward: 16-bit rows of 4,096 take 105 us at two and 95
+// at four (32,768 rows); backward: 156 at one and 171 at two (registers).
+constexpr __host__ __device__ int norm_wide_rows(int vec, bool backward) {
+  return backward || vec == 1 ? 1 : vec == 8 ? 4 : 2;
+}
 
 // VEC values of a row: one 16-byte load where the layout allows it, else one value.
 template <class V, int VEC>
@@ -244,38 +248,79 @@ struct RowSum {
 };
 
 // Tiles of rows on their way through shared memory, by bulk copies (one per
-// tile where the rows have no gaps, else one per row) into STAGES buffers of
+// tile where the rows have no gaps, else one per row) into a ring of buffers of
 // `rows` rows for each of N arrays. The loads of a block are so several tiles
-// deep, whatever registers its threads have left. Buffer k's tile is ready when
+// deep, whatever registers its threads have left. A buffer's tile is ready when
 // its barrier completes a phase; a wait that gives up makes the block leave.
-constexpr int kNormStages = 4;
-template <class T, int N>
+//
+// A bulk copy moves whole 16-byte units. Where rows do not start and end at
+// such (ALIGNED false), the units that hold a row's first and last bytes are
+// copied whole and the row is found inside; those of the matrix's first and
+// last row reach past it, so the tiles with these two rows are not copied:
+// the threads read them in place.
+constexpr int kNormStages = 8;
+template <class T, int N, bool ALIGNED>
 struct RowRing {
   const T *src[N];
   int64_t stride[N];
   int64_t rows_total, step;  // rows of the matrix, rows between two tiles of this block
   int rows, dim, stages;
-  T *buf;
+  uint8_t *buf;
   uint64_t *bars;
   volatile uint32_t *given_up;
   int at = 0;
   uint32_t parity = 0;
 
-  __device__ __forceinline__ T *tile(int stage, int n) const { return buf + (int64_t(stage) * N + n) * rows * dim; }
+  // bytes of a row in a buffer; rows without gaps lie there without gaps too
+  static __host__ __device__ size_t pitch(int64_t dim) {
+    return ALIGNED ? size_t(dim) * sizeof(T) : ((size_t(dim) * sizeof(T) + 15) & ~size_t(15)) + 16;
+  }
+  __device__ __forceinline__ uint8_t *buffer(int stage, int n) const {
+    return buf + size_t(stage * N + n) * rows * pitch(dim);
+  }
+  __device__ __forceinline__ bool covers(int64_t base) const {
+    return ALIGNED || (base > 0 && base + rows < rows_total);
+  }
+  // Row r of the tile in turn, which `covers` it.
+  __device__ __forceinline__ const T *row(int n, int r, int64_t base) const {
+    const uint8_t *b = buffer(at, n);
+    if constexpr (ALIGNED) return reinterpret_cast<const T *>(b) + r * dim;
+    const bool dense = stride[n] == dim;
+    const uintptr_t from = reinterpret_cast<uintptr_t>(src[n] + (dense ? base : base + r) * stride[n]);
+    return reinterpret_cast<const T *>(b + (dense ? size_t(r) * dim * sizeof(T) : r * pitch(dim)) + (from & 15));
+  }
+  __device__ __forceinline__ static uint32_t units(const T *from, int64_t values, const uint8_t *&first) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(from), e = a + size_t(values) * sizeof(T);
+    first = reinterpret_cast<const uint8_t *>(a & ~uintptr_t(15));
+    return uint32_t(((e + 15) & ~uintptr_t(15)) - (a & ~uintptr_t(15)));
+  }
   __device__ __forceinline__ void fill(int stage, int64_t base) const {  // one thread
     const int64_t left = rows_total - base;
     const int count = int(left < rows ? left : rows);
     if (count <= 0) return;
-    const uint32_t row_bytes = uint32_t(dim * sizeof(T));
-    mbar_arrive_expect_tx(&bars[stage], uint32_t(count) * row_bytes * N);
+    if (!covers(base)) {
+      mbar_arrive_expect_tx(&bars[stage], 0);
+      return;
+    }
+    uint32_t bytes = 0;
+    const uint8_t *first;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const T *from = src[n] + base * stride[n];
+      if (stride[n] == dim) bytes += units(src[n] + base * stride[n], int64_t(count) * dim, first);
+      else
+        for (int r = 0; r < count; ++r) bytes += units(src[n] + (base + r) * stride[n], dim, first);
+    }
+    mbar_arrive_expect_tx(&bars[stage], bytes);
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
       if (stride[n] == dim) {
-        bulk_copy_g2s(tile(stage, n), from, uint32_t(count) * row_bytes, &bars[stage]);
+        bytes = units(src[n] + base * stride[n], int64_t(count) * dim, first);
+        bulk_copy_g2s(buffer(stage, n), first, bytes, &bars[stage]);
       } else {
-        for (int r = 0; r < count; ++r)
-          bulk_copy_g2s(tile(stage, n) + int64_t(r) * dim, from + r * stride[n], row_bytes, &bars[stage]);
+        for (int r = 0; r < count; ++r) {
+          bytes = units(src[n] + (base + r) * stride[n], dim, first);
+          bulk_copy_g2s(buffer(stage, n) + r * pitch(dim), first, bytes, &bars[stage]);
+        }
       }
     }
   }
@@ -323,7 +368,6 @@ k_norm_forward(const typename V::T *__restrict__ x, int64_t x_stride, int64_t ro
                int stages, uint32_t *status) {
   using P = Pack<V, VEC>;
   using T = typename V::T;
-  constexpr bool kRing = VEC > 1;
   __shared__ float red[2][32][4];
   __shared__ uint64_t bars[kNormStages];
   __shared__ volatile uint32_t given_up;
@@ -344,29 +388,27 @@ k_norm_forward(const typename V::T *__restrict__ x, int64_t x_stride, int64_t ro
   RowSum<U, WIDE> sum{lanes, red};
   const float inv = 1.0f / float(dim);
   const int64_t first = int64_t(blockIdx.x) * groups * U, step = int64_t(gridDim.x) * groups * U;
-  RowRing<T, 1> ring{{x}, {x_stride}, rows, step, groups * U, dim, stages, reinterpret_cast<T *>(raw_smem), bars, &given_up};
-  if constexpr (kRing) ring.start(first);
+  RowRing<T, 1, (VEC > 1)> ring{{x}, {x_stride}, rows, step, groups * U, dim, stages, raw_smem, bars, &given_up};
+  ring.start(first);
   for (int64_t base = first; base < rows; base += step) {
     typename P::Raw raw[U][NV];
-    const bool ok = kRing ? ring.ready() : true;
+    const bool ok = ring.ready(), copied = ring.covers(base);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t row = base + group * U + u;
+      const T *staged = ring.row(0, group * U + u, base);
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
         const int c = (v * lanes + lane) * VEC;
-        const bool in = row < rows && c < dim;
-        if constexpr (kRing) raw[u][v] = in ? P::load(ring.tile(ring.at, 0) + (group * U + u) * dim + c) : P::zero();
-        else raw[u][v] = in ? P::load(x + row * x_stride + c) : P::zero();
+        raw[u][v] = P::zero();
+        if (row < rows && c < dim) raw[u][v] = copied ? P::load(staged + c) : P::load(x + row * x_stride + c);
       }
     }
-    if constexpr (kRing) {
-      if (__syncthreads_or(!ok)) {
-        ring.drain(base, status);
-        return;
-      }
-      ring.next(base);
+    if (__syncthreads_or(!ok)) {
+      ring.drain(base, status);
+      return;
     }
+    ring.next(base);
     // values beyond the row are zeros, and zeros again after the mean is taken off
     float f[U][NV][VEC], m[U], s[U];
 #pragma unroll
@@ -468,7 +510,7 @@ k_norm_forward_long(const typename V::T *__restrict__ x, int64_t x_stride, int64
 // [gridDim.x][2][dim] fp32, this block's sums of g h and of g per column
 // (null: no weight gradients wanted).
 template <class V, int VEC, int NV, int U, bool WIDE>
-__global__ void __launch_bounds__(WIDE ? norm_wide_threads(VEC) : kNormNarrowThreads)
+__global__ void __launch_bounds__(WIDE ? norm_wide_threads(VEC) : kNormNarrowThreads, !WIDE && NV <= 2 ? 2 : 1)
 k_norm_backward(const typename V::T *__restrict__ grad, int64_t g_stride, const typename V::T *__restrict__ x,
                 int64_t x_stride, int64_t rows, int dim, const float *__restrict__ mean,
                 const float *__restrict__ rstd, const void *__restrict__ weight, int ptype,
@@ -476,7 +518,6 @@ k_norm_backward(const typename V::T *__restrict__ grad, int64_t g_stride, const 
                 uint32_t *status) {
   using P = Pack<V, VEC>;
   using T = typename V::T;
-  constexpr bool kRing = VEC > 1;
   __shared__ float red[2][32][4];
   __shared__ uint64_t bars[kNormStages];
   __shared__ volatile uint32_t given_up;
@@ -498,39 +539,48 @@ k_norm_backward(const typename V::T *__restrict__ grad, int64_t g_stride, const 
   RowSum<WIDE ? 2 * U : U, WIDE> sum{lanes, red};
   const float inv = 1.0f / float(dim);
   const int64_t first = int64_t(blockIdx.x) * groups * U, step = int64_t(gridDim.x) * groups * U;
-  RowRing<T, 2> ring{{x, grad}, {x_stride, g_stride}, rows, step, groups * U, dim, stages,
-                     reinterpret_cast<T *>(raw_smem), bars, &given_up};
-  if constexpr (kRing) ring.start(first);
+  RowRing<T, 2, (VEC > 1)> ring{{x, grad}, {x_stride, g_stride}, rows,     step, groups * U, dim,
+                                stages,    raw_smem,             bars,     &given_up};
+  ring.start(first);
+  float next_m[U], next_r[U];  // a tile's statistics are asked for a tile ahead
+  auto ask = [&](int64_t at) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t row = at + group * U + u;
+      next_m[u] = row < rows ? mean[row] : 0.0f;
+      next_r[u] = row < rows ? rstd[row] : 0.0f;
+    }
+  };
+  ask(first);
   for (int64_t base = first; base < rows; base += step) {
     typename P::Raw xr[U][NV], gr[U][NV];
     float m[U], r[U];
-    const bool ok = kRing ? ring.ready() : true;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      m[u] = next_m[u];
+      r[u] = next_r[u];
+    }
+    ask(base + step);
+    const bool ok = ring.ready(), copied = ring.covers(base);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t row = base + group * U + u;
-      m[u] = row < rows ? mean[row] : 0.0f;
-      r[u] = row < rows ? rstd[row] : 0.0f;
+      const T *xs = ring.row(0, group * U + u, base), *gs = ring.row(1, group * U + u, base);
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
         const int c = (v * lanes + lane) * VEC;
-        const bool in = row < rows && c < dim;
-        if constexpr (kRing) {
-          const int at = (group * U + u) * dim + c;
-          xr[u][v] = in ? P::load(ring.tile(ring.at, 0) + at) : P::zero();
-          gr[u][v] = in ? P::load(ring.tile(ring.at, 1) + at) : P::zero();
-        } else {
-          xr[u][v] = in ? P::load(x + row * x_stride + c) : P::zero();
-          gr[u][v] = in ? P::load(grad + row * g_stride + c) : P::zero();
+        xr[u][v] = gr[u][v] = P::zero();
+        if (row < rows && c < dim) {
+          xr[u][v] = copied ? P::load(xs + c) : P::load(x + row * x_stride + c);
+          gr[u][v] = copied ? P::load(gs + c) : P::load(grad + row * g_stride + c);
         }
       }
     }
-    if constexpr (kRing) {
-      if (__syncthreads_or(!ok)) {
-        ring.drain(base, status);
-        return;
-      }
-      ring.next(base);
+    if (__syncthreads_or(!ok)) {
+      ring.drain(base, status);
+      return;
     }
+    ring.next(base);
     // rows and columns beyond the matrix have r, g and w zero: they add nothing
     float s0[U], s1[U], both[2 * U];
 #pragma unroll
@@ -729,7 +779,7 @@ struct NormShape {
   int nv, lanes, threads, unroll;
 };
 
-NormShape norm_shape(int64_t dim, size_t value_size, bool aligned) {
+NormShape norm_shape(int64_t dim, size_t value_size, bool aligned, bool backward) {
   NormShape s{};
   const int per = int(16 / value_size);
   s.vec = aligned && dim % per == 0;
@@ -743,7 +793,7 @@ NormShape norm_shape(int64_t dim, size_t value_size, bool aligned) {
     return s;
   }
   s.nv = norm_wide_loads(s.vec ? per : 1);
-  s.unroll = norm_wide_rows(s.vec ? per : 1);
+  s.unroll = norm_wide_rows(s.vec ? per : 1, backward);
   s.wide = true;
   const int64_t threads = (n + s.nv - 1) / s.nv;
   const int most = norm_wide_threads(s.vec ? per : 1);
@@ -770,12 +820,10 @@ NormLaunch norm_launch(K *kernel, const NormShape &s, int64_t rows, int64_t dim,
   const int sms = sm_count(device);
   NormLaunch l{};
   const int64_t tile_rows = int64_t(s.threads / s.lanes) * s.unroll;
-  if (s.vec) {
-    const size_t tile = size_t(tile_rows) * size_t(dim) * value_size * arrays;
-    l.stages = int(std::max<size_t>(2, std::min<size_t>(kNormStages, size_t(49152) * arrays / tile)));
-    if (tile * l.stages > 200 * 1024) l.stages = 1;  // two rows of 8,192 fp32 values of both arrays
-    l.smem = tile * l.stages;
-  }
+  const size_t row = s.vec ? size_t(dim) * value_size : ((size_t(dim) * value_size + 15) & ~size_t(15)) + 16;
+  const size_t tile = size_t(tile_rows) * row * arrays;
+  l.stages = int(std::max<size_t>(2, std::min<size_t>(kNormStages, size_t(49152) * arrays / tile)));
+  l.smem = tile * l.stages;
   l.smem = std::max(l.smem, least_smem);
   allow_dynamic_smem(kernel, l.smem);
   l.blocks = std::min(norm_blocks(rows, s, sms), sms * resident_blocks(kernel, device, s.threads, l.smem));
@@ -784,12 +832,12 @@ NormLaunch norm_launch(K *kernel, const NormShape &s, int64_t rows, int64_t dim,
 
 // f with the kernel's constants: values per load, loads per thread, rows at a
 // time, a block per row.
-template <class V, class F>
+template <class V, bool BACKWARD, class F>
 void with_norm_shape(const NormShape &s, F &&f) {
   using std::integral_constant;
   auto go = [&](auto vec) {
     constexpr int kVec = decltype(vec)::value;
-    if (s.wide) f(vec, integral_constant<int, norm_wide_loads(kVec)>{}, integral_constant<int, norm_wide_rows(kVec)>{}, std::true_type{});
+    if (s.wide) f(vec, integral_constant<int, norm_wide_loads(kVec)>{}, integral_constant<int, norm_wide_rows(kVec, BACKWARD)>{}, std::true_type{});
     else if (s.nv == 1) f(vec, integral_constant<int, 1>{}, integral_constant<int, 4>{}, std::false_type{});
     else if (s.nv == 2) f(vec, integral_constant<int, 2>{}, integral_constant<int, 2>{}, std::false_type{});
     else f(vec, integral_constant<int, 4>{}, integral_constant<int, 1>{}, std::false_type{});
@@ -831,7 +879,7 @@ extern "C" int se_layer_norm(int32_t value_dtype, int32_t param_dtype, const voi
     const int sms = sm_count(device);
     uint32_t *status = wait_status(device);
     const size_t vb = value_bytes(value_dtype);
-    const NormShape s = norm_shape(dim, vb, aligned16(x) && aligned16(y) && (rows == 1 || x_stride * vb % 16 == 0));
+    const NormShape s = norm_shape(dim, vb, aligned16(x) && aligned16(y) && (rows == 1 || x_stride * vb % 16 == 0), false);
     dispatch_value(value_dtype, [&](auto tag) {
       using V = decltype(tag);
       using T = typename V::T;
@@ -844,7 +892,7 @@ extern "C" int se_layer_norm(int32_t value_dtype, int32_t param_dtype, const voi
         launched("k_norm_forward_long");
         return;
       }
-      with_norm_shape<V>(s, [&](auto vec, auto nv, auto u, auto wide) {
+      with_norm_shape<V, false>(s, [&](auto vec, auto nv, auto u, auto wide) {
         auto *kernel = k_norm_forward<V, decltype(vec)::value, decltype(nv)::value, decltype(u)::value, decltype(wide)::value>;
         const NormLaunch l = norm_launch(kernel, s, int64_t(rows), dim, vb, 1, device, 0);
         kernel<<<l.blocks, s.threads, l.smem, st>>>(xp, x_stride, int64_t(rows), int(dim), weight, bias, param_dtype, eps,
@@ -864,7 +912,7 @@ extern "C" int se_layer_norm_backward_workspace(size_t rows, int64_t dim, int32_
     int blocks = 1;
     for (const size_t vb : {size_t(2), size_t(4)}) {
       for (const bool aligned : {false, true}) {
-        const NormShape s = norm_shape(dim, vb, aligned);
+        const NormShape s = norm_shape(dim, vb, aligned, true);
         blocks = std::max(blocks, s.longer ? int(std::min<size_t>(rows, kNormLongSplits))
                                            : norm_blocks(int64_t(rows), s, sms));
       }
@@ -899,7 +947,8 @@ extern "C" int se_layer_norm_backward(int32_t value_dtype, int32_t param_dtype, 
       check_device_ptr(dx, device, "dx");
       const size_t vb = value_bytes(value_dtype);
       const NormShape s = norm_shape(dim, vb, aligned16(x) && aligned16(grad) && aligned16(dx) &&
-                                                  (rows == 1 || (x_stride * vb % 16 == 0 && grad_stride * vb % 16 == 0)));
+                                                  (rows == 1 || (x_stride * vb % 16 == 0 && grad_stride * vb % 16 == 0)),
+                                     true);
       blocks = s.longer ? int(std::min<size_t>(rows, kNormLongSplits)) : norm_blocks(int64_t(rows), s, sms);
       if (sums) {
         check_device_ptr(workspace, device, "workspace");
@@ -926,7 +975,7 @@ extern "C" int se_layer_norm_backward(int32_t value_dtype, int32_t param_dtype, 
           }
           return;
         }
-        with_norm_shape<V>(s, [&](auto vec, auto nv, auto u, auto wide) {
+        with_norm_shape<V, true>(s, [&](auto vec, auto nv, auto u, auto wide) {
             auto *kernel = k_norm_backward<V, decltype(vec)::value, decltype(nv)::value, decltype(u)::value, decltype(wide)::value>;
           const size_t cols = s.wide || !sums ? 0 : size_t(s.threads / 32) * size_t(dim) * sizeof(float);
           const NormLaunch l = norm_launch(kernel, s, int64_t(rows), dim, vb, 2, device, cols);
