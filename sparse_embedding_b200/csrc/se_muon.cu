@@ -219,9 +219,10 @@ __device__ __forceinline__ void put_eight(__half *hi, __half *lo, const float (&
   *reinterpret_cast<uint4 *>(lo) = l;
 }
 
-// X_0 = S U / (|U| + eps) as hi + lo, s x w (transposed where m > n): tiles of
-// 64 x 64 values, 16 per thread, through shared memory where the sides are
-// exchanged, so that both are read and written by rows. X's storage reaches
+// X_0 = S U / (|U| + eps) as hi + lo, s x w (transposed where m > n): along the
+// rows in 16-byte vectors, or, where the sides are exchanged or the layout has
+// no vectors, in tiles of 64 x 64 values, 16 per thread, through shared memory,
+// so that both are read and written by rows. X's storage reaches
 // to a multiple of 64 columns, so its rows are written in whole vectors.
 template <class V, bool MOM>
 __global__ void __launch_bounds__(256)
@@ -240,6 +241,30 @@ k_muon_scale(UpdateArgs a, const double *__restrict__ parts, int nparts, float e
   }
   __syncthreads();
   const Factor k = factor;
+  if (a.vec && !transposed) {  // along the rows: as many threads per row as it has eights, up to the block
+    int shift = 0;
+    while (shift < 8 && (int64_t(8) << shift) < a.n) ++shift;
+    const int lanes = 1 << shift, sub = threadIdx.x & (lanes - 1);
+    const int64_t each = blockDim.x >> shift;
+    for (int64_t i = blockIdx.x * each + (threadIdx.x >> shift); i < a.m; i += gridDim.x * each) {
+#pragma unroll 2
+      for (int64_t j = sub * 8; j < a.n; j += lanes * 8) {
+        float u[8];
+        load_eight<V>(static_cast<const typename V::T *>(a.grad.p) + z * a.grad.batch + i * a.grad.row + j, true, 1, 8, u);
+        if constexpr (MOM) {
+          float mom[8];
+          load_eight<F32>(static_cast<const float *>(a.momentum.p) + z * a.momentum.batch + i * a.momentum.row + j, true, 1, 8,
+                          mom);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) u[e] = update_of(a, u[e], mom[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u[e] = k.times(u[e]);
+        put_eight(hi + z * batch_stride + i * ld + j, lo + z * batch_stride + i * ld + j, u);
+      }
+    }
+    return;
+  }
   const int row = threadIdx.x >> 3, at = threadIdx.x & 7;  // 8 threads of 8 values per row, rows `row` and `row` + 32
   const int step = a.vec ? 1 : 8, first = a.vec ? at * 8 : at;
   const int64_t tiles_j = (a.n + 63) / 64, tiles = tiles_j * ((a.m + 63) / 64);
@@ -262,8 +287,7 @@ k_muon_scale(UpdateArgs a, const double *__restrict__ parts, int nparts, float e
 #pragma unroll
       for (int e = 0; e < 8; ++e) u[q][e] = k.times(u[q][e]);
     }
-    const bool through = transposed || !a.vec;
-    if (through) {
+    {
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
 #pragma unroll
@@ -274,14 +298,12 @@ k_muon_scale(UpdateArgs a, const double *__restrict__ parts, int nparts, float e
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       const int r = row + 32 * q, c = at * 8;
-      if (through) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) u[q][e] = transposed ? tile[c + e][r] : tile[r][c + e];
-      }
+      for (int e = 0; e < 8; ++e) u[q][e] = transposed ? tile[c + e][r] : tile[r][c + e];
       const int64_t rr = (transposed ? j0 : i0) + r, cc = (transposed ? i0 : j0) + c;
       if (rr < (transposed ? a.n : a.m)) put_eight(hi + z * batch_stride + rr * ld + cc, lo + z * batch_stride + rr * ld + cc, u[q]);
     }
-    if (through) __syncthreads();
+    __syncthreads();
   }
 }
 
@@ -305,6 +327,7 @@ struct Pair {  // a matrix as hi + lo
 struct FinishArgs {
   void *out;  // O itself, or the weights W <- keep W - rate O
   int type, update, transposed;
+  int vec;    // four values of a row at a time: whole 8 or 16 bytes
   int64_t row, batch;
   float keep, rate;
 };
@@ -395,26 +418,67 @@ __device__ __forceinline__ void put_four(__half *hi, __half *lo, const float4 &f
         make_uint2(*reinterpret_cast<const unsigned *>(&c), *reinterpret_cast<const unsigned *>(&d));
   }
 }
-__device__ __forceinline__ float load_typed(const void *p, int type, int64_t at) {
-  if (type == SE_FLOAT32) return static_cast<const float *>(p)[at];
-  if (type == SE_FLOAT16) return __half2float(static_cast<const __half *>(p)[at]);
-  return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[at]);
-}
-__device__ __forceinline__ void store_typed(void *p, int type, int64_t at, float v) {
-  if (type == SE_FLOAT32) static_cast<float *>(p)[at] = v;
-  else if (type == SE_FLOAT16) static_cast<__half *>(p)[at] = __float2half_rn(v);
-  else static_cast<__nv_bfloat16 *>(p)[at] = __float2bfloat16_rn(v);
-}
+// Four consecutive values of the result's type as one load or store where its
+// rows allow that (`vec`), else the first `count` one by one.
+template <class OUT>
+struct Four {
+  using T = typename OUT::T;
+  using Raw = std::conditional_t<sizeof(T) == 4, uint4, uint2>;
+  Raw raw;
+  __device__ __forceinline__ void load(const T *p, bool vec, int count) {
+    T v[4];
+    if (vec) {
+      if (count > 0) *reinterpret_cast<Raw *>(v) = *reinterpret_cast<const Raw *>(p);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < count) v[e] = p[e];
+    }
+    raw = *reinterpret_cast<const Raw *>(v);
+  }
+  __device__ __forceinline__ float4 open() const {
+    const T *v = reinterpret_cast<const T *>(&raw);
+    return make_float4(OUT::load(v[0]), OUT::load(v[1]), OUT::load(v[2]), OUT::load(v[3]));
+  }
+  static __device__ __forceinline__ void store(T *p, const float4 &f, bool vec, int count) {
+    const T v[4] = {OUT::store(f.x), OUT::store(f.y), OUT::store(f.z), OUT::store(f.w)};
+    if (vec) {
+      if (count > 0) *reinterpret_cast<Raw *>(p) = *reinterpret_cast<const Raw *>(v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < count) p[e] = v[e];
+    }
+  }
+};
+
+// Where a block of O lies in the result: this lane's first four values, the rows
+// of the result below it (every fourth), and how many of the four there are.
+template <class OUT>
+struct FinishBlock {
+  typename OUT::T *at;
+  int turns, count;
+  __device__ __forceinline__ FinishBlock(const NsArgs &g, int z, int r0, int c0) {
+    const int lane = int(threadIdx.x) & 31, up = lane >> 3, four = (lane & 7) * 4;
+    const FinishArgs &f = g.fin;
+    const int row = f.transposed ? c0 : r0, col = f.transposed ? r0 : c0;
+    const int rows = f.transposed ? g.apply.cols : g.apply.rows, cols = f.transposed ? g.apply.rows : g.apply.cols;
+    at = static_cast<typename OUT::T *>(f.out) + int64_t(z) * f.batch + int64_t(row + up) * f.row + col + four;
+    turns = (min(32, rows - row) - up + 3) >> 2;
+    count = max(0, min(4, cols - col - four));
+  }
+};
 
 // What the epilogue of a 32 x 32 block reads besides the accumulator: A (kSquare)
-// or X (kApply, kFinish) and A's diagonal over the columns. A warp asks for it
-// before it waits for the accumulator, or while it still works on the block
-// before, so that the latency is hidden.
-template <int MODE, bool SPLIT>
+// or X (kApply, kFinish), A's diagonal over the columns, the weights (kFinish of
+// an update). A warp asks for it before it waits for the accumulator, or while
+// it still works on the block before, so that the latency is hidden.
+template <int MODE, class OUT>
 struct BlockInput {
-  static constexpr bool kLo = MODE == kApply || MODE == kFinish || SPLIT;
+  static constexpr bool kLo = MODE == kApply || MODE == kFinish || !std::is_same_v<OUT, BF16>;
   uint2 hi[8], lo[8];
   float4 diag;
+  Four<OUT> weight[8];
   __device__ __forceinline__ void load(const NsArgs &g, int step, int z, int r0, int c0) {
     if constexpr (MODE != kGram) {
       const int lane = int(threadIdx.x) & 31, up = lane >> 3, four = (lane & 7) * 4;
@@ -431,6 +495,14 @@ struct BlockInput {
       }
       if constexpr (MODE == kSquare)  // padded like the columns
         diag = __ldcg(reinterpret_cast<const float4 *>(g.diag_a + int64_t(z) * g.diag_ld + c0 + four));
+      if constexpr (MODE == kFinish) {
+        if (g.fin.update) {
+          const FinishBlock<OUT> f(g, z, r0, c0);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (i < f.turns) weight[i].load(f.at + int64_t(4 * i) * g.fin.row, g.fin.vec, f.count);
+        }
+      }
     }
   }
 };
@@ -443,15 +515,19 @@ struct BlockInput {
 // called where the block's input has been used. Rows are r0 .. r0 + 31,
 // columns c0 .. c0 + 31, both multiples of 32; storage reaches past the last
 // column to a multiple of 64, so columns need no guard.
-template <int MODE, bool SPLIT, class Next>
+template <int MODE, class OUT, class Next>
 __device__ __forceinline__ void finish_block(const NsArgs &g, int step, float *tile, int z, int r0, int c0,
-                                             float dr_lane, const BlockInput<MODE, SPLIT> &input, Next &&next) {
+                                             float dr_lane, const BlockInput<MODE, OUT> &input, Next &&next) {
   constexpr bool kSym = MODE == kGram || MODE == kSquare;
-  constexpr bool kInLo = BlockInput<MODE, SPLIT>::kLo;
+  constexpr bool kInLo = BlockInput<MODE, OUT>::kLo, SPLIT = !std::is_same_v<OUT, BF16>;
   const int lane = int(threadIdx.x) & 31, up = lane >> 3, four = (lane & 7) * 4;
   const int rows = g.apply.rows;
   const Pair &out = MODE == kGram ? g.a : MODE == kSquare ? g.b : g.x[(step & 1) ^ 1];
   const int turns = (min(32, rows - r0) - up + 3) >> 2;  // this lane's rows: r0 + up, r0 + up + 4, ...
+  auto down = [&](int c) {  // four rows of column c
+    return make_float4(tile[tile_place(four, c)], tile[tile_place(four + 1, c)], tile[tile_place(four + 2, c)],
+                       tile[tile_place(four + 3, c)]);
+  };
   const bool diagonal = kSym && r0 == c0;
   if (diagonal) {
     // The diagonal's value goes to its vector: (A A)_rr = acc + D_r^2. (Both
@@ -508,6 +584,34 @@ __device__ __forceinline__ void finish_block(const NsArgs &g, int step, float *t
       if (rr == four + 3) f.w = 0.0f;
     }
   }
+  if constexpr (MODE == kFinish) {
+    const FinishArgs &fin = g.fin;
+    const FinishBlock<OUT> to(g, z, r0, c0);
+    if (fin.transposed) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) *reinterpret_cast<float4 *>(tile + tile_place(4 * i + up, four)) = v[i];
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = down(4 * i + up);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float4 &f = v[i];
+      f = make_float4(f.x * (1.0f / kScale), f.y * (1.0f / kScale), f.z * (1.0f / kScale), f.w * (1.0f / kScale));
+      if (fin.update) {
+        const float4 w = input.weight[i].open();
+        f.x = __fmaf_rn(-fin.rate, f.x, fin.keep * w.x);
+        f.y = __fmaf_rn(-fin.rate, f.y, fin.keep * w.y);
+        f.z = __fmaf_rn(-fin.rate, f.z, fin.keep * w.z);
+        f.w = __fmaf_rn(-fin.rate, f.w, fin.keep * w.w);
+      }
+    }
+    next();
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < to.turns) Four<OUT>::store(to.at + int64_t(4 * i) * fin.row, v[i], fin.vec, to.count);
+    return;
+  }
   next();
   if constexpr (MODE != kFinish) {
     const int64_t to = int64_t(z) * out.batch + int64_t(r0 + up) * out.ld + c0 + four;
@@ -519,20 +623,14 @@ __device__ __forceinline__ void finish_block(const NsArgs &g, int step, float *t
       ol += 4 * out.ld;
     }
   }
-  if ((kSym && !diagonal) || MODE == kFinish) {
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 8; ++i) *reinterpret_cast<float4 *>(tile + tile_place(4 * i + up, four)) = v[i];
-    __syncwarp();
-  }
   if constexpr (kSym) {
     if (!diagonal) {  // the mirror: rows c0 .., columns r0 ..
+      __syncwarp();
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int cc = 4 * i + up;
-        v[i] = make_float4(tile[tile_place(four, cc)], tile[tile_place(four + 1, cc)], tile[tile_place(four + 2, cc)],
-                           tile[tile_place(four + 3, cc)]);
-      }
+      for (int i = 0; i < 8; ++i) *reinterpret_cast<float4 *>(tile + tile_place(4 * i + up, four)) = v[i];
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = down(4 * i + up);
       const int64_t to = int64_t(z) * out.batch + int64_t(c0 + up) * out.ld + r0 + four;
       __half *oh = out.hi + to, *ol = out.lo + to;
 #pragma unroll
@@ -543,48 +641,34 @@ __device__ __forceinline__ void finish_block(const NsArgs &g, int step, float *t
       }
     }
   }
-  if constexpr (MODE == kFinish) {
-    // by rows of the result, whichever way it lies: lane = its column
-    const FinishArgs &f = g.fin;
-    const int across = f.transposed ? r0 : c0, along = f.transposed ? c0 : r0;
-    const bool inside = across + lane < (f.transposed ? rows : g.apply.cols);
-    const int most = min(32, (f.transposed ? g.apply.cols : rows) - along);
-    const int64_t base = int64_t(z) * f.batch + int64_t(along) * f.row + across + lane;
-#pragma unroll 1
-    for (int e0 = 0; e0 < most; e0 += 8) {
-      float w[8];
-      if (f.update) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          w[e] = inside && e0 + e < most ? load_typed(f.out, f.type, base + (e0 + e) * f.row) : 0.0f;
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float o = tile[f.transposed ? tile_place(lane, e0 + e) : tile_place(e0 + e, lane)] * (1.0f / kScale);
-        if (f.update) o = __fmaf_rn(-f.rate, o, f.keep * w[e]);
-        if (inside && e0 + e < most) store_typed(f.out, f.type, base + (e0 + e) * f.row, o);
-      }
-    }
-  }
 }
 
-// A block's sum over its parts: each part leaves its own in `partial`, the one
-// that arrives last adds all of them in their order into `tile`. False: not last.
-__device__ __forceinline__ bool join_parts(const NsArgs &g, float *tile, int64_t block, int part) {
-  const int lane = int(threadIdx.x) & 31, parts = g.gram.parts;
-  auto at = [&](int i) { return reinterpret_cast<float4 *>(tile + tile_place(4 * i + (lane >> 3), (lane & 7) * 4)); };
-  float4 *mine = reinterpret_cast<float4 *>(g.partial + (block * parts + part) * 1024) + lane;
+// Parts of a sum: each leaves its block in `partial` (leave_part), and the warp
+// whose part arrives last (last_part) adds all of them in their order into
+// `tile` (join_parts). `block` numbers the blocks of all tiles.
+__device__ __forceinline__ float4 *staged_four(float *tile, int i) {
+  const int lane = int(threadIdx.x) & 31;
+  return reinterpret_cast<float4 *>(tile + tile_place(4 * i + (lane >> 3), (lane & 7) * 4));
+}
+__device__ __forceinline__ void leave_part(const NsArgs &g, float *tile, int64_t block, int part) {
+  float4 *mine = reinterpret_cast<float4 *>(g.partial + (block * g.gram.parts + part) * 1024) + (threadIdx.x & 31);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) __stcg(mine + 32 * i, *at(i));
+  for (int i = 0; i < 8; ++i) __stcg(mine + 32 * i, *staged_four(tile, i));
+}
+__device__ __forceinline__ bool last_part(const NsArgs &g, uint32_t *arrived) {
   __threadfence();
   __syncwarp();
   uint32_t before = 0;
-  if (lane == 0) before = atomicAdd(g.arrived + block, 1u);
+  if ((threadIdx.x & 31) == 0) before = atomicAdd(arrived, 1u);
   before = __shfl_sync(0xffffffffu, before, 0);
-  if (before != uint32_t(parts - 1)) return false;
+  if (before != uint32_t(g.gram.parts - 1)) return false;
   __threadfence();
-  if (lane == 0) g.arrived[block] = 0u;  // for the next step
-  const float4 *all = reinterpret_cast<const float4 *>(g.partial + block * parts * 1024) + lane;
+  if ((threadIdx.x & 31) == 0) *arrived = 0u;  // for the next step
+  return true;
+}
+__device__ __forceinline__ void join_parts(const NsArgs &g, float *tile, int64_t block) {
+  const int parts = g.gram.parts;
+  const float4 *all = reinterpret_cast<const float4 *>(g.partial + block * parts * 1024) + (threadIdx.x & 31);
   float4 sum[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) sum[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -599,10 +683,10 @@ __device__ __forceinline__ bool join_parts(const NsArgs &g, float *tile, int64_t
       sum[i].w += f.w;
     }
   }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) *at(i) = sum[i];
   __syncwarp();
-  return true;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) *staged_four(tile, i) = sum[i];
+  __syncwarp();
 }
 
 // A ring of N buffers: the one in turn and how often the ring went round (its
@@ -637,15 +721,16 @@ struct Shared {  // of a CTA
 // Warp 0 loads operand stages by TMA, warp 1 issues the matrix instructions,
 // warps 4-11 turn finished accumulators into the result while the next one is
 // computed (two accumulators of BN columns in tensor memory; each epilogue
-// warp has 32 rows and every second block of 32 columns).
+// warp has 32 rows of one half of the columns).
 //
 // SPLIT: the three products of hi and lo parts. The tensor core cuts its fp32
 // sums off instead of rounding them, which over thousands of k-values costs
 // more than the lo parts bring (measured: 3e-5 at 4,096), so a sum runs over
 // kFlush k-blocks only and the epilogue warps add those up in registers.
-template <int MODE, int CG, int BN, bool SPLIT>
+template <int MODE, int CG, int BN, class OUT>
 __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int step, Shared &sh, uint8_t *smem,
-                                            uint32_t rank, Progress<Layout<CG, BN, SPLIT>::kStages> &at) {
+                                            uint32_t rank, Progress<Layout<CG, BN, !std::is_same_v<OUT, BF16>>::kStages> &at) {
+  constexpr bool SPLIT = !std::is_same_v<OUT, BF16>;
   using L = Layout<CG, BN, SPLIT>;
   constexpr int kTM = 128 * CG, kBlocks = BN / 64;          // kBlocks: column blocks of an epilogue warp
   constexpr bool kBMN = MODE == kApply || MODE == kFinish;  // the B operand is X itself: n-contiguous
@@ -744,7 +829,7 @@ __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int s
   } else if (warp >= 4) {
     const int quad = warp & 3, side = (warp - 4) >> 2;
     float *tile = reinterpret_cast<float *>(smem + kStages * L::kStage) + (warp - 4) * L::kStaging;
-    const uint32_t tmem = sh.tmem + (uint32_t(quad * 32) << 16) + uint32_t(side * 32);
+    const uint32_t tmem = sh.tmem + (uint32_t(quad * 32) << 16) + uint32_t(side * kBlocks * 32);
     bool go = true;
     auto take = [&] {  // the accumulator in turn is full; false: gave up
       go = __all_sync(0xffffffffu, wait_or_give_up(&sh.acc_full[at.sum.at], at.sum.parity, &sh.given_up));
@@ -769,11 +854,11 @@ __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int s
       float dr = 0.0f;
       if (MODE != kGram && r0 + lane < c.rows)
         dr = __ldcg((MODE == kSquare ? g.diag_a : g.diag_b) + int64_t(z) * g.diag_ld + r0 + lane);
-      auto column = [&](int b) { return col + (2 * b + side) * 32; };
+      auto column = [&](int b) { return col + (side * kBlocks + b) * 32; };
       auto wanted = [&](int b) {
         return b < kBlocks && r0 < c.rows && column(b) < c.cols && (kBMN || column(b) <= r0);
       };
-      BlockInput<MODE, SPLIT> input;
+      BlockInput<MODE, OUT> input;
       auto ask = [&](int b) {
         if (wanted(b)) input.load(g, step, z, r0, column(b));
       };
@@ -784,13 +869,11 @@ __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int s
           *reinterpret_cast<float4 *>(to + tile_place(lane, e)) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
       };
       auto finish = [&](int b, float *staged) {
-        if (MODE == kGram && parts > 1) {
-          constexpr int kPerTile = (kTM / 32) * (BN / 32);
-          const int64_t block = int64_t(zt) * kPerTile + (int(rank) * 4 + quad) * (BN / 32) + 2 * b + side;
-          if (!join_parts(g, staged, block, part)) return;
-        }
-        finish_block<MODE, SPLIT>(g, step, staged, z, r0, column(b), dr, input, [&] { ask(b + 1); });
+        finish_block<MODE, OUT>(g, step, staged, z, r0, column(b), dr, input, [&] { ask(b + 1); });
       };
+      // in parts: this warp's place among the warps of all tiles, and its blocks
+      const int64_t place = (int64_t(zt) * CG + rank) * kEpilogueWarps + warp - 4;
+      const bool in_parts = MODE == kGram && parts > 1;
       if constexpr (SPLIT) {
         static_assert(kBlocks <= 2, "the sums stay in registers");
         float v[kBlocks][32];
@@ -804,7 +887,7 @@ __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int s
 #pragma unroll
           for (int b = 0; b < kBlocks; ++b) {
             float f[32];
-            tmem_load32(tmem + at.sum.at * BN + uint32_t(b * 64), f);
+            tmem_load32(tmem + at.sum.at * BN + uint32_t(b * 32), f);
 #pragma unroll
             for (int e = 0; e < 32; ++e) v[b][e] += f[e];
           }
@@ -815,6 +898,11 @@ __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int s
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b) stage(tile + b * 1024, v[b]);
         __syncwarp();
+        if (in_parts) {
+          for (int b = 0; b < kBlocks && wanted(b); ++b) leave_part(g, tile + b * 1024, place * kBlocks + b, part);
+          if (!wanted(0) || !last_part(g, g.arrived + place)) continue;
+          for (int b = 0; b < kBlocks && wanted(b); ++b) join_parts(g, tile + b * 1024, place * kBlocks + b);
+        }
         ask(0);  // not earlier: the sums fill the registers
 #pragma unroll 1
         for (int b = 0; b < kBlocks && wanted(b); ++b) finish(b, tile + b * 1024);
@@ -825,12 +913,20 @@ __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int s
           if (!wanted(b)) break;
           float v[32];
           __syncwarp();
-          tmem_load32(tmem + at.sum.at * BN + uint32_t(b * 64), v);
+          tmem_load32(tmem + at.sum.at * BN + uint32_t(b * 32), v);
           stage(tile, v);
           __syncwarp();
-          finish(b, tile);
+          if (in_parts) leave_part(g, tile, place * kBlocks + b, part);
+          else finish(b, tile);
         }
         give();
+        if (in_parts && wanted(0) && last_part(g, g.arrived + place)) {
+#pragma unroll 1
+          for (int b = 0; b < kBlocks && wanted(b); ++b) {
+            join_parts(g, tile, place * kBlocks + b);
+            finish(b, tile);
+          }
+        }
       }
     }
     asm volatile("fence.proxy.async.global;" ::: "memory");  // what this thread stored, for every block's TMA
@@ -860,12 +956,35 @@ __device__ __forceinline__ bool grid_wait(uint32_t *barrier, uint32_t target, Sh
   return sh.given_up == 0u;
 }
 
+// Asks for this block's share of the weights, row by row, while the products
+// before the last are busy with the tensor cores: the last epilogue's own reads
+// (64 bytes of each of 32 rows at a time) would open a page of HBM for every
+// one (8 x 1024 x 2048 bf16: the last product took 203,000 clocks, the same
+// product without weights 83,000).
+template <class OUT>
+__device__ __forceinline__ void prefetch_weights(const NsArgs &g) {
+  const FinishArgs &f = g.fin;
+  const int64_t rows = f.transposed ? g.apply.cols : g.apply.rows, cols = f.transposed ? g.apply.rows : g.apply.cols;
+  const int lane = int(threadIdx.x) & 31;
+  for (int64_t i = int64_t(blockIdx.x) * 32 + lane; i < rows * g.batch; i += int64_t(gridDim.x) * 32) {
+    const int64_t z = i / rows, r = i - z * rows;
+    const uintptr_t row = reinterpret_cast<uintptr_t>(static_cast<typename OUT::T *>(f.out) + z * f.batch + r * f.row);
+    uintptr_t at = (row + 15) & ~uintptr_t(15);
+    const uintptr_t end = (row + size_t(cols) * sizeof(typename OUT::T)) & ~uintptr_t(15);
+    while (at < end) {
+      const uint32_t bytes = uint32_t(end - at < 4096 ? end - at : 4096);
+      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(at), "r"(bytes) : "memory");
+      at += bytes;
+    }
+  }
+}
+
 // The whole iteration in one cooperative launch: 3 products a step, a barrier
 // over the grid after each. Launches cost more than the products of small
 // matrices, and for large ones the tensor cores are the bound either way.
-template <int CG, int BN, bool SPLIT>
+template <int CG, int BN, class OUT>
 __global__ void __launch_bounds__(kThreads, 1) k_newton_schulz(const __grid_constant__ NsArgs g) {
-  using L = Layout<CG, BN, SPLIT>;
+  using L = Layout<CG, BN, !std::is_same_v<OUT, BF16>>;
   extern __shared__ uint8_t raw[];
   __shared__ Shared sh;
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
@@ -892,15 +1011,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_newton_schulz(const __grid_cons
   Progress<L::kStages> at;
   uint32_t target = 0;
   for (int step = 0; step < g.steps; ++step) {
-    run_product<kGram, CG, BN, SPLIT>(g, g.gram, step, sh, smem, rank, at);
+    run_product<kGram, CG, BN, OUT>(g, g.gram, step, sh, smem, rank, at);
     if (!grid_wait(g.barrier, target += gridDim.x, sh)) break;
-    run_product<kSquare, CG, BN, SPLIT>(g, g.square, step, sh, smem, rank, at);
+    if (step + 1 == g.steps && g.fin.update && warp == 3) prefetch_weights<OUT>(g);
+    run_product<kSquare, CG, BN, OUT>(g, g.square, step, sh, smem, rank, at);
     if (!grid_wait(g.barrier, target += gridDim.x, sh)) break;
     if (step + 1 == g.steps) {
-      run_product<kFinish, CG, BN, SPLIT>(g, g.apply, step, sh, smem, rank, at);
+      run_product<kFinish, CG, BN, OUT>(g, g.apply, step, sh, smem, rank, at);
       break;
     }
-    run_product<kApply, CG, BN, SPLIT>(g, g.apply, step, sh, smem, rank, at);
+    run_product<kApply, CG, BN, OUT>(g, g.apply, step, sh, smem, rank, at);
     if (!grid_wait(g.barrier, target += gridDim.x, sh)) break;
   }
 
@@ -1412,16 +1532,16 @@ Space muon_space(void *base, int64_t batch, int64_t s, int64_t w, bool split) {
   sp.diag_b = reinterpret_cast<float *>(take(size_t(batch) * lda * sizeof(float)));
   const int64_t values = p.parts > 1 ? tile_count(true, s, s, 128 * p.cg, p.bn) * batch * 128 * p.cg * p.bn : 0;
   sp.partial = reinterpret_cast<float *>(take(size_t(values) * p.parts * sizeof(float)));
-  sp.ncounters = 1 + values / 1024;
+  sp.ncounters = 1 + values / 1024;  // (at least one per warp of a tile)
   sp.counters = reinterpret_cast<uint32_t *>(take(size_t(sp.ncounters) * sizeof(uint32_t)));
   sp.bytes = at;
   return sp;
 }
 
-template <int CG, int BN, bool SPLIT>
+template <int CG, int BN, class OUT>
 void launch_newton_schulz(const NsArgs &g, int64_t units, int sms, cudaStream_t st) {
-  using L = Layout<CG, BN, SPLIT>;
-  auto *kernel = k_newton_schulz<CG, BN, SPLIT>;
+  using L = Layout<CG, BN, !std::is_same_v<OUT, BF16>>;
+  auto *kernel = k_newton_schulz<CG, BN, OUT>;
   allow_dynamic_smem(kernel, L::kBytes);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(std::min<int64_t>(units, sms / CG) * CG));
@@ -1466,6 +1586,9 @@ void orthogonalise(UpdateArgs u, int grad_type, int64_t batch, int steps, float 
   const int sms = sm_count(device);
   g.status = wait_status(device);
   fin.transposed = transposed;
+  const size_t ob = value_bytes(fin.type);
+  fin.vec = u.n % 4 == 0 && reinterpret_cast<uintptr_t>(fin.out) % (4 * ob) == 0 && fin.row % 4 == 0 &&
+            (batch == 1 || fin.batch % 4 == 0);
   if (s <= kSmallSide && w <= kSmallWide) {
     const int xtiles = int((w + 63) / 64), stiles = int((s + 63) / 64);
     const size_t smem = size_t(2 * xtiles + (split ? 2 : 1) * stiles) * kSmallTile + 1024;
@@ -1539,17 +1662,20 @@ void orthogonalise(UpdateArgs u, int grad_type, int64_t batch, int steps, float 
   g.arrived = sp.counters + 1;
   g.fin = fin;
   const int64_t units = std::max<int64_t>(int64_t(g.gram.tiles) * plan.parts, g.apply.tiles) * batch;
-  const int form = plan.cg * 1000 + plan.bn * 2 + (split ? 1 : 0);
-  switch (form) {
-    case 2512: launch_newton_schulz<2, 256, false>(g, units, sms, st); break;
-    case 2256: launch_newton_schulz<2, 128, false>(g, units, sms, st); break;
-    case 2257: launch_newton_schulz<2, 128, true>(g, units, sms, st); break;
-    case 1512: launch_newton_schulz<1, 256, false>(g, units, sms, st); break;
-    case 1256: launch_newton_schulz<1, 128, false>(g, units, sms, st); break;
-    case 1257: launch_newton_schulz<1, 128, true>(g, units, sms, st); break;
-    case 1128: launch_newton_schulz<1, 64, false>(g, units, sms, st); break;
-    default: launch_newton_schulz<1, 64, true>(g, units, sms, st); break;
-  }
+  const int form = plan.cg * 1000 + plan.bn;
+  dispatch_value(fin.type, [&](auto out) {
+    using OUT = decltype(out);
+    switch (form) {
+      case 2128: launch_newton_schulz<2, 128, OUT>(g, units, sms, st); return;
+      case 1128: launch_newton_schulz<1, 128, OUT>(g, units, sms, st); return;
+      case 1064: launch_newton_schulz<1, 64, OUT>(g, units, sms, st); return;
+      default: break;
+    }
+    if constexpr (std::is_same_v<OUT, BF16>) {  // wider tiles: single products only
+      if (form == 2256) launch_newton_schulz<2, 256, OUT>(g, units, sms, st);
+      else launch_newton_schulz<1, 256, OUT>(g, units, sms, st);
+    }
+  });
 }
 
 void check_matrices(size_t batch, int64_t m, int64_t n, int32_t steps, float eps) {
