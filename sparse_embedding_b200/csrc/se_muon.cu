@@ -418,39 +418,21 @@ __device__ __forceinline__ void put_four(__half *hi, __half *lo, const float4 &f
         make_uint2(*reinterpret_cast<const unsigned *>(&c), *reinterpret_cast<const unsigned *>(&d));
   }
 }
-// Four consecutive values of the result's type as one load or store where its
-// rows allow that (`vec`), else the first `count` one by one.
+// Four consecutive values of the result's type as one store where its rows allow
+// that (`vec`), else the first `count` one by one.
 template <class OUT>
-struct Four {
+__device__ __forceinline__ void store_four(typename OUT::T *p, const float4 &f, bool vec, int count) {
   using T = typename OUT::T;
   using Raw = std::conditional_t<sizeof(T) == 4, uint4, uint2>;
-  Raw raw;
-  __device__ __forceinline__ void load(const T *p, bool vec, int count) {
-    T v[4];
-    if (vec) {
-      if (count > 0) *reinterpret_cast<Raw *>(v) = *reinterpret_cast<const Raw *>(p);
-    } else {
+  const T v[4] = {OUT::store(f.x), OUT::store(f.y), OUT::store(f.z), OUT::store(f.w)};
+  if (vec) {
+    if (count > 0) *reinterpret_cast<Raw *>(p) = *reinterpret_cast<const Raw *>(v);
+  } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (e < count) v[e] = p[e];
-    }
-    raw = *reinterpret_cast<const Raw *>(v);
+    for (int e = 0; e < 4; ++e)
+      if (e < count) p[e] = v[e];
   }
-  __device__ __forceinline__ float4 open() const {
-    const T *v = reinterpret_cast<const T *>(&raw);
-    return make_float4(OUT::load(v[0]), OUT::load(v[1]), OUT::load(v[2]), OUT::load(v[3]));
-  }
-  static __device__ __forceinline__ void store(T *p, const float4 &f, bool vec, int count) {
-    const T v[4] = {OUT::store(f.x), OUT::store(f.y), OUT::store(f.z), OUT::store(f.w)};
-    if (vec) {
-      if (count > 0) *reinterpret_cast<Raw *>(p) = *reinterpret_cast<const Raw *>(v);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (e < count) p[e] = v[e];
-    }
-  }
-};
+}
 
 // Where a block of O lies in the result: this lane's first four values, the rows
 // of the result below it (every fourth), and how many of the four there are.
@@ -478,7 +460,6 @@ struct BlockInput {
   static constexpr bool kLo = MODE == kApply || MODE == kFinish || !std::is_same_v<OUT, BF16>;
   uint2 hi[8], lo[8];
   float4 diag;
-  Four<OUT> weight[8];
   __device__ __forceinline__ void load(const NsArgs &g, int step, int z, int r0, int c0) {
     if constexpr (MODE != kGram) {
       const int lane = int(threadIdx.x) & 31, up = lane >> 3, four = (lane & 7) * 4;
@@ -495,14 +476,6 @@ struct BlockInput {
       }
       if constexpr (MODE == kSquare)  // padded like the columns
         diag = __ldcg(reinterpret_cast<const float4 *>(g.diag_a + int64_t(z) * g.diag_ld + c0 + four));
-      if constexpr (MODE == kFinish) {
-        if (g.fin.update) {
-          const FinishBlock<OUT> f(g, z, r0, c0);
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (i < f.turns) weight[i].load(f.at + int64_t(4 * i) * g.fin.row, g.fin.vec, f.count);
-        }
-      }
     }
   }
 };
@@ -598,18 +571,11 @@ __device__ __forceinline__ void finish_block(const NsArgs &g, int step, float *t
     for (int i = 0; i < 8; ++i) {
       float4 &f = v[i];
       f = make_float4(f.x * (1.0f / kScale), f.y * (1.0f / kScale), f.z * (1.0f / kScale), f.w * (1.0f / kScale));
-      if (fin.update) {
-        const float4 w = input.weight[i].open();
-        f.x = __fmaf_rn(-fin.rate, f.x, fin.keep * w.x);
-        f.y = __fmaf_rn(-fin.rate, f.y, fin.keep * w.y);
-        f.z = __fmaf_rn(-fin.rate, f.z, fin.keep * w.z);
-        f.w = __fmaf_rn(-fin.rate, f.w, fin.keep * w.w);
-      }
     }
     next();
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (i < to.turns) Four<OUT>::store(to.at + int64_t(4 * i) * fin.row, v[i], fin.vec, to.count);
+      if (i < to.turns) store_four<OUT>(to.at + int64_t(4 * i) * fin.row, v[i], fin.vec, to.count);
     return;
   }
   next();
@@ -956,29 +922,6 @@ __device__ __forceinline__ bool grid_wait(uint32_t *barrier, uint32_t target, Sh
   return sh.given_up == 0u;
 }
 
-// Asks for this block's share of the weights, row by row, while the products
-// before the last are busy with the tensor cores: the last epilogue's own reads
-// (64 bytes of each of 32 rows at a time) would open a page of HBM for every
-// one (8 x 1024 x 2048 bf16: the last product took 203,000 clocks, the same
-// product without weights 83,000).
-template <class OUT>
-__device__ __forceinline__ void prefetch_weights(const NsArgs &g) {
-  const FinishArgs &f = g.fin;
-  const int64_t rows = f.transposed ? g.apply.cols : g.apply.rows, cols = f.transposed ? g.apply.rows : g.apply.cols;
-  const int lane = int(threadIdx.x) & 31;
-  for (int64_t i = int64_t(blockIdx.x) * 32 + lane; i < rows * g.batch; i += int64_t(gridDim.x) * 32) {
-    const int64_t z = i / rows, r = i - z * rows;
-    const uintptr_t row = reinterpret_cast<uintptr_t>(static_cast<typename OUT::T *>(f.out) + z * f.batch + r * f.row);
-    uintptr_t at = (row + 15) & ~uintptr_t(15);
-    const uintptr_t end = (row + size_t(cols) * sizeof(typename OUT::T)) & ~uintptr_t(15);
-    while (at < end) {
-      const uint32_t bytes = uint32_t(end - at < 4096 ? end - at : 4096);
-      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(at), "r"(bytes) : "memory");
-      at += bytes;
-    }
-  }
-}
-
 // The whole iteration in one cooperative launch: 3 products a step, a barrier
 // over the grid after each. Launches cost more than the products of small
 // matrices, and for large ones the tensor cores are the bound either way.
@@ -1013,14 +956,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_newton_schulz(const __grid_cons
   for (int step = 0; step < g.steps; ++step) {
     run_product<kGram, CG, BN, OUT>(g, g.gram, step, sh, smem, rank, at);
     if (!grid_wait(g.barrier, target += gridDim.x, sh)) break;
-    if (step + 1 == g.steps && g.fin.update && warp == 3) prefetch_weights<OUT>(g);
     run_product<kSquare, CG, BN, OUT>(g, g.square, step, sh, smem, rank, at);
     if (!grid_wait(g.barrier, target += gridDim.x, sh)) break;
-    if (step + 1 == g.steps) {
+    if (step + 1 == g.steps && !g.fin.update) {
       run_product<kFinish, CG, BN, OUT>(g, g.apply, step, sh, smem, rank, at);
       break;
     }
     run_product<kApply, CG, BN, OUT>(g, g.apply, step, sh, smem, rank, at);
+    if (step + 1 == g.steps) break;
     if (!grid_wait(g.barrier, target += gridDim.x, sh)) break;
   }
 
@@ -1048,6 +991,90 @@ __global__ void __launch_bounds__(kThreads, 1) k_newton_schulz(const __grid_cons
   __syncthreads();
   if constexpr (CG == 2) cluster_sync_all();
   if (warp == 2) tmem_free<CG>(sh.tmem, 2 * BN);
+}
+
+// W <- keep W - rate O for O = (hi + lo) / S, a kernel of its own: the last
+// product's epilogue would load and store 64-byte pieces of the weights' lines,
+// and such a store waits long for its line when another piece of it is being
+// loaded (8 x 1024 x 2048 bf16: that product took 152,000 to 203,000 clocks for
+// 83,000 without weights; this kernel takes a quarter of the difference). Along
+// the rows in vectors, or through shared memory in tiles of 64 x 64, as
+// k_muon_scale.
+template <class W>
+__global__ void __launch_bounds__(256)
+k_muon_weights(const __half *__restrict__ hi, const __half *__restrict__ lo, int64_t ld, int64_t batch_stride, int64_t m,
+               int64_t n, int vec, FinishArgs f) {
+  __shared__ float tile[64][65];
+  using T = typename W::T;
+  const int64_t z = blockIdx.z;
+  T *w = static_cast<T *>(f.out) + z * f.batch;
+  hi += z * batch_stride;
+  lo += z * batch_stride;
+  const float rate = f.rate * (1.0f / kScale);
+  pdl_wait();
+  auto open = [&](int64_t at, float (&o)[8]) {  // eight values of O, not yet divided by S
+    const uint4 h = *reinterpret_cast<const uint4 *>(hi + at), l = *reinterpret_cast<const uint4 *>(lo + at);
+    const __half2 *hh = reinterpret_cast<const __half2 *>(&h), *ll = reinterpret_cast<const __half2 *>(&l);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 x = __half22float2(hh[e]), y = __half22float2(ll[e]);
+      o[2 * e] = x.x + y.x;
+      o[2 * e + 1] = x.y + y.y;
+    }
+  };
+  if (vec && !f.transposed) {
+    int shift = 0;
+    while (shift < 8 && (int64_t(8) << shift) < n) ++shift;
+    const int lanes = 1 << shift, sub = threadIdx.x & (lanes - 1);
+    const int64_t each = blockDim.x >> shift;
+    for (int64_t i = blockIdx.x * each + (threadIdx.x >> shift); i < m; i += gridDim.x * each) {
+#pragma unroll 2
+      for (int64_t j = sub * 8; j < n; j += lanes * 8) {
+        float o[8], old[8];
+        open(i * ld + j, o);
+        T *at = w + i * f.row + j;
+        load_eight<W>(at, true, 1, 8, old);
+        constexpr int kPer = 16 / sizeof(T);
+        uint4 raw[8 / kPer];
+        T *v = reinterpret_cast<T *>(raw);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = W::store(__fmaf_rn(-rate, o[e], f.keep * old[e]));
+#pragma unroll
+        for (int e = 0; e < 8 / kPer; ++e) reinterpret_cast<uint4 *>(at)[e] = raw[e];
+      }
+    }
+    return;
+  }
+  // tiles of W; X is read along its own rows
+  const int row = threadIdx.x >> 3, eight = (threadIdx.x & 7) * 8;
+  const int64_t tiles_j = (n + 63) / 64, tiles = tiles_j * ((m + 63) / 64);
+  for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
+    const int64_t i0 = t / tiles_j * 64, j0 = (t - t / tiles_j * tiles_j) * 64;
+    const int64_t r0 = f.transposed ? j0 : i0, c0 = f.transposed ? i0 : j0, rows = f.transposed ? n : m;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int r = row + 32 * q;
+      float o[8] = {};
+      if (r0 + r < rows) open((r0 + r) * ld + c0 + eight, o);  // X's storage reaches past its columns to a multiple of 64
+#pragma unroll
+      for (int e = 0; e < 8; ++e) tile[r][eight + e] = o[e];
+    }
+    __syncthreads();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const int i = warp + 8 * q;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int j = lane + 32 * h;
+        if (i0 + i < m && j0 + j < n) {
+          T *at = w + (i0 + i) * f.row + j0 + j;
+          *at = W::store(__fmaf_rn(-rate, f.transposed ? tile[j][i] : tile[i][j], f.keep * W::load(*at)));
+        }
+      }
+    }
+    __syncthreads();
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -1538,6 +1565,21 @@ Space muon_space(void *base, int64_t batch, int64_t s, int64_t w, bool split) {
   return sp;
 }
 
+// A kernel of 256 threads that waits (pdl_wait) for the one before it.
+template <class... KArgs, class... Args>
+void launch_after(void (*kernel)(KArgs...), dim3 grid, cudaStream_t st, Args... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cuda_check(cudaLaunchKernelEx(&cfg, kernel, args...), "cudaLaunchKernelEx");
+}
+
 template <int CG, int BN, class OUT>
 void launch_newton_schulz(const NsArgs &g, int64_t units, int sms, cudaStream_t st) {
   using L = Layout<CG, BN, !std::is_same_v<OUT, BF16>>;
@@ -1621,18 +1663,9 @@ void orthogonalise(UpdateArgs u, int grad_type, int64_t batch, int steps, float 
       constexpr bool kMom = decltype(mom)::value;
       k_muon_momentum<V, kMom><<<dim3(unsigned(nparts), unsigned(batch)), 256, 0, st>>>(u, sp.norms, sp.counters, sp.ncounters);
       launched("k_muon_momentum");
-      cudaLaunchConfig_t cfg{};
-      cfg.gridDim = dim3(unsigned(std::min<int64_t>(tiles64, 8 * sms)), 1, unsigned(batch));
-      cfg.blockDim = dim3(256);
-      cfg.stream = st;
-      cudaLaunchAttribute attr[1];
-      attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-      attr[0].val.programmaticStreamSerializationAllowed = 1;
-      cfg.attrs = attr;
-      cfg.numAttrs = 1;
-      cuda_check(cudaLaunchKernelEx(&cfg, k_muon_scale<V, kMom>, u, static_cast<const double *>(sp.norms), nparts, eps,
-                                    transposed, sp.x[0].hi, sp.x[0].lo, sp.x[0].ld, sp.x[0].batch),
-                 "k_muon_scale");
+      launch_after(k_muon_scale<V, kMom>, dim3(unsigned(std::min<int64_t>(tiles64, 8 * sms)), 1, unsigned(batch)), st, u,
+                   static_cast<const double *>(sp.norms), nparts, eps, transposed, sp.x[0].hi, sp.x[0].lo, sp.x[0].ld,
+                   sp.x[0].batch);
       launched("k_muon_scale");
     };
     if (u.momentum.p) go(std::true_type{});
@@ -1676,6 +1709,15 @@ void orthogonalise(UpdateArgs u, int grad_type, int64_t batch, int steps, float 
       else launch_newton_schulz<1, 256, OUT>(g, units, sms, st);
     }
   });
+  if (!fin.update) return;
+  dispatch_value(fin.type, [&](auto out) {
+    const Pair &o = sp.x[steps & 1];
+    const int vec = u.n % 8 == 0 && aligned16(fin.out) && fin.row * ob % 16 == 0 && (batch == 1 || fin.batch * ob % 16 == 0);
+    const int64_t blocks = vec && !transposed ? (u.m * ((u.n + 7) / 8) + 255) / 256 : tiles64;
+    launch_after(k_muon_weights<decltype(out)>, dim3(unsigned(std::min<int64_t>(blocks, 8 * sms)), 1, unsigned(batch)), st,
+                 static_cast<const __half *>(o.hi), static_cast<const __half *>(o.lo), o.ld, o.batch, u.m, u.n, vec, fin);
+  });
+  launched("k_muon_weights");
 }
 
 void check_matrices(size_t batch, int64_t m, int64_t n, int32_t steps, float eps) {
