@@ -30,6 +30,7 @@ NVCC_FLAGS = [
     # multiply-add; IEEE division and square root (no fast math).
     "--fmad=false", "-prec-div=true", "-prec-sqrt=true", "-ftz=false",
     "-Xcompiler", "-fPIC", "-shared", "-cudart", "static",
+    "--threads", "0",  # the sources side by side
 ]
 
 

@@ -1565,6 +1565,25 @@ Space muon_space(void *base, int64_t batch, int64_t s, int64_t w, bool split) {
   return sp;
 }
 
+// Pairs of blocks that run at once (asked once per device and kernel).
+template <class... KArgs>
+int64_t resident_clusters(void (*kernel)(KArgs...), int device, const cudaLaunchConfig_t &cfg) {
+  static std::mutex mu;
+  static std::map<std::pair<const void *, int>, int> known;
+  const auto key = std::make_pair(reinterpret_cast<const void *>(kernel), device);
+  std::lock_guard<std::mutex> lock(mu);
+  auto it = known.find(key);
+  if (it != known.end()) return it->second;
+  cudaLaunchConfig_t ask = cfg;
+  cudaLaunchAttribute cluster = cfg.attrs[1];
+  ask.attrs = &cluster;
+  ask.numAttrs = 1;
+  int n = 0;
+  cuda_check(cudaOccupancyMaxActiveClusters(&n, kernel, &ask), "cluster occupancy");
+  if (n < 1) throw Error(SE_ERR_CUDA, "no pair of blocks fits the device");
+  return known[key] = n;
+}
+
 // A kernel of 256 threads that waits (pdl_wait) for the one before it.
 template <class... KArgs, class... Args>
 void launch_after(void (*kernel)(KArgs...), dim3 grid, cudaStream_t st, Args... args) {
@@ -1581,12 +1600,13 @@ void launch_after(void (*kernel)(KArgs...), dim3 grid, cudaStream_t st, Args... 
 }
 
 template <int CG, int BN, class OUT>
-void launch_newton_schulz(const NsArgs &g, int64_t units, int sms, cudaStream_t st) {
+void launch_newton_schulz(const NsArgs &g, int64_t units, int device, cudaStream_t st) {
+  const int sms = sm_count(device);
   using L = Layout<CG, BN, !std::is_same_v<OUT, BF16>>;
   auto *kernel = k_newton_schulz<CG, BN, OUT>;
   allow_dynamic_smem(kernel, L::kBytes);
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(std::min<int64_t>(units, sms / CG) * CG));
+  cfg.gridDim = dim3(unsigned(sms / CG * CG));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = L::kBytes;
   cfg.stream = st;
@@ -1599,6 +1619,8 @@ void launch_newton_schulz(const NsArgs &g, int64_t units, int sms, cudaStream_t 
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = CG == 2 ? 2 : 1;
+  const int64_t at_once = CG == 2 ? resident_clusters(kernel, device, cfg) : sms;
+  cfg.gridDim = dim3(unsigned(std::min(units, at_once) * CG));
   cuda_check(cudaLaunchKernelEx(&cfg, kernel, g), "k_newton_schulz");
   launched("k_newton_schulz");
 }
@@ -1699,14 +1721,14 @@ void orthogonalise(UpdateArgs u, int grad_type, int64_t batch, int steps, float 
   dispatch_value(fin.type, [&](auto out) {
     using OUT = decltype(out);
     switch (form) {
-      case 2128: launch_newton_schulz<2, 128, OUT>(g, units, sms, st); return;
-      case 1128: launch_newton_schulz<1, 128, OUT>(g, units, sms, st); return;
-      case 1064: launch_newton_schulz<1, 64, OUT>(g, units, sms, st); return;
+      case 2128: launch_newton_schulz<2, 128, OUT>(g, units, device, st); return;
+      case 1128: launch_newton_schulz<1, 128, OUT>(g, units, device, st); return;
+      case 1064: launch_newton_schulz<1, 64, OUT>(g, units, device, st); return;
       default: break;
     }
     if constexpr (std::is_same_v<OUT, BF16>) {  // wider tiles: single products only
-      if (form == 2256) launch_newton_schulz<2, 256, OUT>(g, units, sms, st);
-      else launch_newton_schulz<1, 256, OUT>(g, units, sms, st);
+      if (form == 2256) launch_newton_schulz<2, 256, OUT>(g, units, device, st);
+      else launch_newton_schulz<1, 256, OUT>(g, units, device, st);
     }
   });
   if (!fin.update) return;

@@ -230,7 +230,8 @@ def muon_step(weight, grad, momentum, lr: float = 0.02, beta: float = 0.95, weig
         weight = (1 - lr weight_decay) weight - lr scale orthogonalize(U)
 
     momentum is float32 of weight's shape; grad has weight's dtype or float32.
-    scale is sqrt(max(1, m / n)) unless given. The three share no memory."""
+    scale is sqrt(max(1, m / n)) unless given. The three lie in memory of their
+    own: ranges that overlap, slices of one tensor among them, are refused."""
     w, g, mom = (_cuda_tensor(t, what) for t, what in ((weight, "weight"), (grad, "grad"), (momentum, "momentum")))
     torch = torch_mod()
     for t, what in ((g, "grad"), (mom, "momentum")):
@@ -255,3 +256,5 @@ def muon_step(weight, grad, momentum, lr: float = 0.02, beta: float = 0.95, weig
                                    mom.data_ptr(), mbs, mrs, batch, m, n, float(lr), float(beta), float(weight_decay),
                                    float(scale), int(bool(nesterov)), int(steps), float(eps), work.data_ptr(), nbytes,
                                    w.device.index, _stream(w)))
+    # written behind autograd's back: a graph that saved either notices
+    torch.autograd.graph.increment_version([t for t in (w, mom) if not t.is_inference()])

@@ -80,6 +80,16 @@ class Muon(torch.optim.Optimizer):
             if p.dim() < 2:
                 raise ValueError("Muon steps matrices: every parameter needs at least two dimensions")
 
+    def load_state_dict(self, state_dict) -> None:
+        super().load_state_dict(state_dict)
+        # torch casts an optimizer's state to its parameters' dtype: put the float32 momentum back
+        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
+        own = [p for g in self.param_groups for p in g["params"]]
+        for i, p in zip(saved, own):
+            buffer = state_dict["state"].get(i, {}).get("momentum_buffer")
+            if buffer is not None:
+                self.state[p]["momentum_buffer"] = buffer.to(device=p.device, dtype=torch.float32, copy=True)
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None

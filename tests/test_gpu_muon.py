@@ -147,10 +147,25 @@ def test_zero_infinite_and_nan_updates(dt):
         assert se.orthogonalize(torch.zeros(empty, dtype=dt, device="cuda")).shape == empty
 
 
-def test_equal_calls_give_equal_bits():
-    u = matrix(2, 300, 520).to(F32)
+@pytest.mark.parametrize("shape, dt", [((2, 300, 520), F32), ((100, 100), F32), ((200, 4096), F32), ((192, 6000), BF16),
+                                       ((1600, 1700), BF16)])
+def test_equal_calls_give_equal_bits(shape, dt):
+    u = matrix(*shape).to(dt)  # long sides are summed in parts by several blocks
     first = se.orthogonalize(u)
-    assert all(torch.equal(se.orthogonalize(u), first) for _ in range(3))
+    assert all(torch.equal(se.orthogonalize(u), first) for _ in range(10))
+    near(first if first.dim() == 2 else first[1], exact(u if u.dim() == 2 else u[1]), TOL[dt])
+
+
+@pytest.mark.parametrize("shape, dt", [((2100, 2100), BF16), ((2560, 1536), BF16), ((1100, 1000), F16), ((2, 1100, 1300), F32),
+                                       ((1024, 3000), F32), ((3500, 3500), BF16)])
+def test_large_matrices(shape, dt):
+    u = matrix(*shape).to(dt)
+    o = se.orthogonalize(u)
+    near(o[-1] if o.dim() == 3 else o, exact(u[-1] if u.dim() == 3 else u), TOL[dt])
+    w = torch.zeros(shape, dtype=dt, device="cuda")
+    mom = torch.zeros(shape, device="cuda")
+    se.muon_step(w, u, mom, lr=1.0, beta=0.0, scale=-1.0)  # from zero weights: the update itself
+    assert float((w.double() - o.double()).norm() / o.double().norm()) < 2 * TOL[dt]
 
 
 def reference_step(w, g, mom, lr, beta, decay, nesterov, steps=5, scale=None):
@@ -233,6 +248,77 @@ def test_captured_steps_continue():
     assert torch.equal(w, ref) and torch.equal(mom, ref_mom)
 
 
+def test_calls_from_two_threads():
+    import threading
+
+    us = [matrix(150, 300, seed=k).to(BF16) for k in range(3)] + [matrix(60, 90).to(F32)]
+    want = [se.orthogonalize(u) for u in us]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(u, o):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(30):
+                if not torch.equal(se.orthogonalize(u), o):
+                    bad.append(1)
+
+    threads = [threading.Thread(target=work, args=a) for a in zip(us, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
+def test_first_call_under_capture():
+    """A fresh process whose first calls are captured."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = """
+import torch, sparse_embedding_b200 as se
+x = torch.randn(300, 200, device="cuda"); w = torch.ones(200, device="cuda"); small = torch.randn(40, 60, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    y, m, r = se.layer_norm(x, w, return_stats=True)
+    d = se.layer_norm_backward(x, x, m, r, w)
+    o, p = se.orthogonalize(x), se.orthogonalize(small)
+g.replay(); torch.cuda.synchronize()
+assert torch.equal(y, se.layer_norm(x, w)) and torch.equal(o, se.orthogonalize(x)) and torch.equal(p, se.orthogonalize(small))
+print("captured")
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).resolve().parent.parent, capture_output=True,
+                       text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+def test_optimizer_state_and_versions():
+    p = torch.nn.Parameter(matrix(40, 70, kind="flat").to(BF16))
+    opt = torch_ops.Muon([p], lr=0.1)
+    p.grad = matrix(40, 70, seed=4).to(BF16)
+    version = p._version
+    opt.step()
+    assert p._version > version
+    buffer = opt.state[p]["momentum_buffer"]
+    assert buffer.dtype == F32 and torch.equal(buffer, p.grad.float())
+    other = torch.nn.Parameter(p.detach().clone())
+    resumed = torch_ops.Muon([other], lr=0.3)
+    resumed.load_state_dict(opt.state_dict())
+    assert resumed.state[other]["momentum_buffer"].dtype == F32 and resumed.param_groups[0]["lr"] == 0.1
+    other.grad = p.grad.clone()
+    opt.step()
+    resumed.step()
+    assert torch.equal(p, other) and torch.equal(buffer, resumed.state[other]["momentum_buffer"])
+    # a graph that saved the weight before the step refuses to go back through it
+    x = torch.randn(3, 70, device="cuda", dtype=BF16, requires_grad=True)
+    y = (x @ p.t()).sum()
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
 def test_refusals():
     w = torch.zeros(6, 8, device="cuda")
     g, mom = torch.zeros_like(w), torch.zeros_like(w)
@@ -248,6 +334,8 @@ def test_refusals():
         (lambda: se.muon_step(w, g.cpu(), mom), "grad must be a CUDA tensor"),
         (lambda: se.muon_step(w, w, mom), "must not share memory"),
         (lambda: se.muon_step(w, g, g), "must not share memory"),
+        (lambda: se.muon_step(g[:3], w[:3], g[2:5]), "must not share memory"),
+        (lambda: se.orthogonalize(torch.zeros(70000, 1, 1, device="cuda")), "batch must be at most"),
         (lambda: se.muon_step(w.t(), g.t(), mom.t()), "matrices at one stride"),
         (lambda: se.muon_step(w, g, mom, beta=1.0), "beta must be in"),
         (lambda: se.muon_step(w, g, mom, lr=float("nan")), "must be finite"),

@@ -284,3 +284,57 @@ def test_refusals():
     host = torch.zeros(4, 8)
     rc = N.lib().se_layer_norm(0, 0, host.data_ptr(), 4, 8, 8, None, None, 1e-5, x.data_ptr(), None, None, 0, None)
     assert rc == N.SE_ERR_INVALID_ARGUMENT and b"x must be device memory" in N.lib().se_last_error()
+
+
+def test_more_than_2_31_values():
+    rows, dim = 530_000, 4096
+    x = torch.empty(rows, dim, dtype=torch.bfloat16, device="cuda")
+    x[: rows - 100] = 1.0
+    tail = torch.randn(100, dim, device="cuda").bfloat16()
+    x[rows - 100 :] = tail
+    w = torch.linspace(0.5, 1.5, dim, device="cuda")
+    y, mean, rstd = se.layer_norm(x, w, return_stats=True)
+    assert torch.equal(y[rows - 100 :], se.layer_norm(tail, w)) and not y[rows - 200].any()
+    del y
+    dx = se.layer_norm_backward(x, x, mean, rstd, w)[0]
+    want = se.layer_norm_backward(tail, tail, mean[rows - 100 :], rstd[rows - 100 :], w)[0]
+    assert torch.equal(dx[rows - 100 :], want)
+
+
+def test_calls_from_two_threads():
+    import threading
+
+    x, g, w, b = inputs(3000, 320, torch.bfloat16, torch.float32)
+    y0, mean, rstd = se.layer_norm(x, w, b, return_stats=True)
+    want = se.layer_norm_backward(g, x, mean, rstd, w)
+    torch.cuda.synchronize()
+    bad = []
+
+    def work():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                got = se.layer_norm_backward(g, x, mean, rstd, w)
+                if not all(torch.equal(p, q) for p, q in zip(got, want)) or not torch.equal(se.layer_norm(x, w, b), y0):
+                    bad.append(1)
+
+    threads = [threading.Thread(target=work) for _ in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim, pad, offset", [(35, 0, 0), (35, 0, 1), (129, 2, 3), (1037, 0, 5), (513, 9, 1)])
+def test_neighbours_of_unaligned_rows(dim, pad, offset, dt):
+    # rows are copied in whole 16-byte units: what lies around the matrix, NaN here, must not enter it
+    rows = 400
+    flat = torch.full((offset + rows * (dim + pad) + 64,), float("nan"), dtype=dt, device="cuda")
+    x = flat[offset : offset + rows * (dim + pad)].view(rows, dim + pad)[:, :dim]
+    x.copy_(torch.randn(rows, dim, device="cuda"))
+    w = torch.ones(dim, dtype=dt, device="cuda")
+    y, mean, rstd = se.layer_norm(x, w, return_stats=True)
+    assert torch.equal(y, se.layer_norm(x.contiguous(), w)) and torch.isfinite(y).all()
+    dx, dw, db = se.layer_norm_backward(x, x, mean, rstd, w)
+    assert all(torch.isfinite(t).all() for t in (dx, dw, db))
