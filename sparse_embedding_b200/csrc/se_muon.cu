@@ -361,11 +361,19 @@ constexpr int kFlush = 4;  // k-blocks of a SPLIT accumulation between two flush
 // Shared memory of a CTA: operand stages, then the epilogue warps' staging
 // tiles (SPLIT stages all blocks of an accumulator at once: its sums would not
 // leave registers for the epilogue).
+//
+// SPLIT with BN = 64 (kStacked) has hi and lo parts of both operands in a stage,
+// B's one below the other: A_hi times both is one instruction of N = 128, which
+// takes no longer than N = 64 (75 clocks: A is read from shared memory either
+// way), and A_lo B_hi adds to the half of A_hi B_lo. Four instructions in five
+// and two thirds of the loads are left of the three products one after another.
 template <int CG, int BN, bool SPLIT>
 struct Layout {
-  static constexpr int kA = 128 * 128;        // bytes of a CTA's A tile: 128 rows of 64 values
-  static constexpr int kB = (BN / CG) * 128;  // and of its part of the B tile
+  static constexpr bool kStacked = SPLIT && BN == 64 && CG == 1;
+  static constexpr int kA = 128 * 128 * (kStacked ? 2 : 1);        // bytes of a CTA's A tile: 128 rows of 64 values
+  static constexpr int kB = (BN / CG) * 128 * (kStacked ? 2 : 1);  // and of its part of the B tile
   static constexpr int kStage = kA + kB;
+  static constexpr int kColumns = kStacked ? 2 * BN : BN;          // of an accumulator
   static constexpr int kStaging = (SPLIT ? BN / 64 : 1) * 32 * 32;  // floats of a warp
   static constexpr int kStagingBytes = kEpilogueWarps * kStaging * 4;
   static constexpr int kRoom = 232448 - 1024 - 512 - kStagingBytes;  // 1,024: tile alignment; 512: static variables
@@ -701,11 +709,12 @@ __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int s
   constexpr int kTM = 128 * CG, kBlocks = BN / 64;          // kBlocks: column blocks of an epilogue warp
   constexpr bool kBMN = MODE == kApply || MODE == kFinish;  // the B operand is X itself: n-contiguous
   constexpr uint32_t kStages = L::kStages;
+  constexpr bool kStacked = L::kStacked;
   const int warp = int(threadIdx.x) >> 5, lane = int(threadIdx.x) & 31;
   const int unit = int(blockIdx.x) / CG, units = int(gridDim.x) / CG;
   const int parts = MODE == kGram ? c.parts : 1;
   const int total = c.tiles * parts * g.batch;
-  const int kall = c.kblocks * (SPLIT ? 3 : 1);
+  const int kall = c.kblocks * (SPLIT && !kStacked ? 3 : 1);
   // the k-blocks of part p: [kall p / parts, kall (p + 1) / parts)
   auto k_from = [&](int p) { return MODE == kGram ? int(int64_t(kall) * p / parts) : p * kall; };
   auto sum_end = [&](int k, int last) { return SPLIT ? min(last, k + kFlush) : last; };
@@ -729,8 +738,9 @@ __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int s
             go = false;
             break;
           }
-          const int seg = SPLIT ? (k >= c.kblocks) + (k >= 2 * c.kblocks) : 2;  // hi lo, lo hi, hi hi
-          const int k0 = (SPLIT ? k - seg * c.kblocks : k) * kTileK;
+          // hi lo, lo hi, hi hi
+          const int seg = SPLIT && !kStacked ? (k >= c.kblocks) + (k >= 2 * c.kblocks) : 2;
+          const int k0 = (SPLIT && !kStacked ? k - seg * c.kblocks : k) * kTileK;
           const CUtensorMap *ma = seg == 1 ? al : ah, *mb = seg == 0 ? bl : bh;
           uint8_t *a = smem + st * L::kStage, *b = a + L::kA;
           uint32_t bar = smem_u32(&sh.full[st]);
@@ -742,6 +752,12 @@ __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int s
           for (int q = 0; q < BN / CG / 64; ++q) {
             if constexpr (kBMN) tma_load<CG>(b + q * 8192, mb, col + q * 64, k0, z, bar);
             else tma_load<CG>(b + q * 8192, mb, k0, col + q * 64, z, bar);
+          }
+          if constexpr (kStacked) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) tma_load<CG>(a + 16384 + q * 8192, al, k0, row + q * 64, z, bar);
+            if constexpr (kBMN) tma_load<CG>(b + 8192, bl, col, k0, z, bar);
+            else tma_load<CG>(b + 8192, bl, k0, col, z, bar);
           }
           at.stage.advance();
           ++at.loaded;
@@ -756,7 +772,7 @@ __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int s
       // instruction, the thread needed 560 to 620 clocks a stage whatever the
       // tile (now 515 at 128 x 256, 305 at 128 x 128; the arithmetic takes 512
       // and 256).
-      constexpr uint32_t kDesc = mma_desc(kTM, BN, kBMN);
+      constexpr uint32_t kDesc = mma_desc(kTM, L::kColumns, kBMN), kLoDesc = mma_desc(kTM, BN, kBMN);
       constexpr uint32_t kStepA = 32 >> 4, kStepB = (kBMN ? 2048 : 32) >> 4;  // 16 k-values: along a row, or 16 rows
       const uint32_t first_a = smem_u32(smem), tmem = sh.tmem;
       const uint64_t desc_a = operand_desc(first_a, 16), desc_b = operand_desc(first_a + L::kA, kBMN ? 8192 : 16);
@@ -764,7 +780,7 @@ __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int s
       for (int t = unit; go && t < total; t += units) {
         const int part = parts > 1 ? t % parts : 0, last = k_from(part + 1);
         for (int k = k_from(part); go && k < last; at.sum.advance()) {
-          const uint32_t acc = tmem + at.sum.at * BN;
+          const uint32_t acc = tmem + at.sum.at * L::kColumns;
           if (!wait_or_give_up(&sh.acc_empty[at.sum.at], at.sum.parity ^ 1u, &sh.given_up)) {
             go = false;
             break;
@@ -784,6 +800,11 @@ __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int s
             add = true;
 #pragma unroll
             for (int q = 1; q < kTileK / 16; ++q) mma_f16<CG>(acc, da + q * kStepA, db + q * kStepB, kDesc, true);
+            if constexpr (kStacked) {
+#pragma unroll
+              for (int q = 0; q < kTileK / 16; ++q)
+                mma_f16<CG>(acc + BN, da + (16384 >> 4) + q * kStepA, db + q * kStepB, kLoDesc, true);
+            }
             mma_commit<CG>(&sh.empty[st]);
             at.stage.advance();
           }
@@ -853,9 +874,14 @@ __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int s
 #pragma unroll
           for (int b = 0; b < kBlocks; ++b) {
             float f[32];
-            tmem_load32(tmem + at.sum.at * BN + uint32_t(b * 32), f);
+            tmem_load32(tmem + at.sum.at * L::kColumns + uint32_t(b * 32), f);
 #pragma unroll
             for (int e = 0; e < 32; ++e) v[b][e] += f[e];
+            if constexpr (kStacked) {
+              tmem_load32(tmem + at.sum.at * L::kColumns + uint32_t(BN + b * 32), f);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) v[b][e] += f[e];
+            }
           }
           give();
         }
@@ -879,7 +905,7 @@ __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int s
           if (!wanted(b)) break;
           float v[32];
           __syncwarp();
-          tmem_load32(tmem + at.sum.at * BN + uint32_t(b * 32), v);
+          tmem_load32(tmem + at.sum.at * L::kColumns + uint32_t(b * 32), v);
           stage(tile, v);
           __syncwarp();
           if (in_parts) leave_part(g, tile, place * kBlocks + b, part);
@@ -945,7 +971,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_newton_schulz(const __grid_cons
     mbar_init(&sh.drained, 1);
     sh.given_up = 0u;
   }
-  if (warp == 2) tmem_alloc<CG>(&sh.tmem, 2 * BN);
+  if (warp == 2) tmem_alloc<CG>(&sh.tmem, 2 * L::kColumns);
   tmem_fence_before();
   __syncthreads();
   if constexpr (CG == 2) cluster_sync_all();
@@ -990,7 +1016,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_newton_schulz(const __grid_cons
   tmem_fence_before();
   __syncthreads();
   if constexpr (CG == 2) cluster_sync_all();
-  if (warp == 2) tmem_free<CG>(sh.tmem, 2 * BN);
+  if (warp == 2) tmem_free<CG>(sh.tmem, 2 * L::kColumns);
 }
 
 // W <- keep W - rate O for O = (hi + lo) / S, a kernel of its own: the last
@@ -1495,23 +1521,23 @@ Plan plan_for(int64_t batch, int64_t s, int64_t w, bool split) {
   struct Form {
     int cg, bn, stage, end, stage_split, end_split;
   };
-  constexpr Form forms[] = {{1, 64, 330, 8000, 330, 12000}, {1, 128, 420, 11000, 450, 16000}, {2, 128, 400, 11000, 430, 16000},
+  constexpr Form forms[] = {{1, 64, 330, 8000, 650, 12000}, {1, 128, 420, 11000, 1350, 16000}, {2, 128, 400, 11000, 1290, 16000},
                             {1, 256, 600, 20000, 0, 0},     {2, 256, 560, 20000, 0, 0}};
-  auto blocks = [&](int64_t values) { return (values + kTileK - 1) / kTileK * (split ? 3 : 1); };
+  constexpr int kJoin = 8000;  // clocks to add up parts
   Plan best{};
   int64_t least = 0;
   for (const Form &f : forms) {
-    if (split && f.stage_split == 0) continue;
-    const int64_t units = kUnits / f.cg;
+    const int64_t stage = split ? f.stage_split : f.stage, end = split ? f.end_split : f.end, units = kUnits / f.cg;
+    if (stage == 0) continue;
     auto rounds = [&](int64_t tiles) { return (tiles + units - 1) / units; };
     const int64_t sym = tile_count(true, s, s, 128 * f.cg, f.bn) * batch;
     const int64_t app = tile_count(false, s, w, 128 * f.cg, f.bn) * batch;
-    // joining parts costs about as much as 24 stages
-    const int64_t kall = blocks(w);
-    const int64_t parts = kall < 48 ? 1 : std::max<int64_t>(1, std::min<int64_t>(units / sym, kall / 16));
-    const int64_t stages = rounds(sym * parts) * ((kall + parts - 1) / parts) + (parts > 1 ? 24 : 0) +
-                           rounds(sym) * blocks(s) + rounds(app) * blocks(s);
-    const int64_t clocks = stages * (split ? f.stage_split : f.stage) + 3 * (split ? f.end_split : f.end);
+    const int64_t kw = (w + kTileK - 1) / kTileK, ks = (s + kTileK - 1) / kTileK;
+    // a part saves stages, of at least 5,000 clocks each
+    const int64_t parts =
+        kw * stage < 2 * kJoin ? 1 : std::max<int64_t>(1, std::min<int64_t>(units / sym, kw * stage / 5000));
+    const int64_t clocks = (rounds(sym * parts) * ((kw + parts - 1) / parts) + rounds(sym) * ks + rounds(app) * ks) * stage +
+                           (parts > 1 ? kJoin : 0) + 3 * end;
     if (least == 0 || clocks < least) {
       least = clocks;
       best = Plan{f.cg, f.bn, int(parts)};
