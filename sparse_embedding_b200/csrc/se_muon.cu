@@ -1085,18 +1085,24 @@ k_muon_weights(const __half *__restrict__ hi, const __half *__restrict__ lo, int
 #pragma unroll
       for (int e = 0; e < 8; ++e) tile[r][eight + e] = o[e];
     }
-    __syncthreads();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    float old[8][2];  // all loads before the first store
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
-      const int i = warp + 8 * q;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int j = lane + 32 * h;
-        if (i0 + i < m && j0 + j < n) {
-          T *at = w + (i0 + i) * f.row + j0 + j;
-          *at = W::store(__fmaf_rn(-rate, f.transposed ? tile[j][i] : tile[i][j], f.keep * W::load(*at)));
-        }
+        const int64_t i = i0 + warp + 8 * q, j = j0 + lane + 32 * h;
+        old[q][h] = i < m && j < n ? W::load(w[i * f.row + j]) : 0.0f;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int i = warp + 8 * q, j = lane + 32 * h;
+        if (i0 + i < m && j0 + j < n)
+          w[(i0 + i) * f.row + j0 + j] = W::store(__fmaf_rn(-rate, f.transposed ? tile[j][i] : tile[i][j], f.keep * old[q][h]));
       }
     }
     __syncthreads();
