@@ -21,8 +21,9 @@
 //    would be the largest error left. With A = D + O:  A A = O O + D O + O D + D D.
 //  * bf16 outputs: products of the hi parts alone. fp32 and f16 outputs:
 //    hi hi + hi lo + lo hi, three times the matrix work, for errors of fp32's order.
-// Against 64 bits, for the matrices of the tests: 0.1 % at most from the single
-// products (below bf16's own 0.17 % rounding), about 2e-6 from the triple ones.
+// Against 64 bits, for gradient-like matrices: 0.03 to 0.1 % from the single
+// products (bf16's own rounding is 0.17 %), 0.5e-6 to 1.3e-6 from the triple ones
+// (fp32 operations in place of them: 0.7e-6 to 3e-6).
 //
 // A and A A are symmetric: only tiles that touch the lower triangle are
 // computed, and an element below the diagonal is written to both places by the
@@ -287,14 +288,12 @@ k_muon_scale(UpdateArgs a, const double *__restrict__ parts, int nparts, float e
 #pragma unroll
       for (int e = 0; e < 8; ++e) u[q][e] = k.times(u[q][e]);
     }
-    {
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
+    for (int q = 0; q < 2; ++q) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) tile[row + 32 * q][first + e * step] = u[q][e];
-      }
-      __syncthreads();
+      for (int e = 0; e < 8; ++e) tile[row + 32 * q][first + e * step] = u[q][e];
     }
+    __syncthreads();
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       const int r = row + 32 * q, c = at * 8;
@@ -365,8 +364,10 @@ constexpr int kFlush = 4;  // k-blocks of a SPLIT accumulation between two flush
 // SPLIT with BN = 64 (kStacked) has hi and lo parts of both operands in a stage,
 // B's one below the other: A_hi times both is one instruction of N = 128, which
 // takes no longer than N = 64 (75 clocks: A is read from shared memory either
-// way), and A_lo B_hi adds to the half of A_hi B_lo. Four instructions in five
-// and two thirds of the loads are left of the three products one after another.
+// way), and A_lo B_hi adds to the half of A_hi B_lo: two thirds of the
+// instructions and of the loads of the three products one after another
+// (1000 x 517 fp32: 188 -> 159 us). At N = 128 an instruction of twice the width
+// takes twice as long, and there they stay apart.
 template <int CG, int BN, bool SPLIT>
 struct Layout {
   static constexpr bool kStacked = SPLIT && BN == 64 && CG == 1;
@@ -460,9 +461,9 @@ struct FinishBlock {
 };
 
 // What the epilogue of a 32 x 32 block reads besides the accumulator: A (kSquare)
-// or X (kApply, kFinish), A's diagonal over the columns, the weights (kFinish of
-// an update). A warp asks for it before it waits for the accumulator, or while
-// it still works on the block before, so that the latency is hidden.
+// or X (kApply, kFinish), and A's diagonal over the columns. A warp asks for it
+// before it waits for the accumulator, or while it still works on the block
+// before, so that the latency is hidden.
 template <int MODE, class OUT>
 struct BlockInput {
   static constexpr bool kLo = MODE == kApply || MODE == kFinish || !std::is_same_v<OUT, BF16>;
@@ -949,8 +950,13 @@ __device__ __forceinline__ bool grid_wait(uint32_t *barrier, uint32_t target, Sh
 }
 
 // The whole iteration in one cooperative launch: 3 products a step, a barrier
-// over the grid after each. Launches cost more than the products of small
-// matrices, and for large ones the tensor cores are the bound either way.
+// over the grid after each (about 2,500 clocks). One launch per product took 81
+// us of host time and 10 us each at 1000 x 517; now a call takes 20 us of it.
+// What bounds it: large sides the tensor cores at the power limit (4096 x 4096
+// bf16 1,150 us, 1.2 PFLOP/s of the 1.37e12 counted operations; of each product
+// 70 of 85 thousand clocks are instructions, the rest its last epilogue and the
+// barrier); 1,000 the chain of a product's stages, epilogue and barrier, 12 to
+// 20 thousand clocks, mostly latency (1000 x 517 fp32 160 us).
 template <int CG, int BN, class OUT>
 __global__ void __launch_bounds__(kThreads, 1) k_newton_schulz(const __grid_constant__ NsArgs g) {
   using L = Layout<CG, BN, !std::is_same_v<OUT, BF16>>;
@@ -1140,7 +1146,8 @@ __device__ __forceinline__ void open_eight(const uint4 &v, float (&f)[8]) {
 // memory, in the layout of the matrix instructions (X serves as a K-major
 // operand of X X^T and, the same bytes, as the MN-major one of B X). Between two products there is only a
 // barrier of the CTA, where the kernel for large matrices passes through L2
-// and a barrier of the grid (128 x 64 bf16: 64 us there with its launches).
+// and a barrier of the grid (128 x 64 bf16: 64 us there with its launches, 23 us
+// here; 128 x 256 42 us, 64 matrices of 64 x 64 19 us).
 // Bound by the instructions of one SM and the latency of 3 products a step;
 // with X and A in shared memory as f16 pairs, unpacked and packed again in
 // every epilogue, it took 33 us at 128 x 64 and 70 at 128 x 256.
