@@ -131,10 +131,11 @@ def test_scale_of_the_update(dt):
 
 
 @pytest.mark.parametrize("dt", [F32, F16, BF16])
-def test_zero_infinite_and_nan_updates(dt):
-    z = torch.zeros(3, 70, 40, dtype=dt, device="cuda")
+@pytest.mark.parametrize("m, n", [(70, 40), (300, 190), (130, 2200)])
+def test_zero_infinite_and_nan_updates(m, n, dt):
+    z = torch.zeros(3, m, n, dtype=dt, device="cuda")
     assert not se.orthogonalize(z).any()
-    z[1] = matrix(70, 40).to(dt)
+    z[1] = matrix(m, n).to(dt)
     z[2] = z[1]
     z[2, 3, 4] = float("nan")
     o = se.orthogonalize(z)
