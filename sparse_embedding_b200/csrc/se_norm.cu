@@ -32,50 +32,83 @@ namespace se_gpu {
 namespace {
 
 constexpr int kNormNarrowThreads = 256;  // block of the kernels with several rows per block
-// A block per row: its most threads and the loads of each. Rows of up to 8,192
+// A block per row: its most threads and the values of each. Rows of up to 8,192
 // values fit the registers in every layout (the backward holds three fp32
 // values per column besides the row).
-constexpr __host__ __device__ int norm_wide_threads(int vec) { return vec == 1 ? 1024 : 512; }
-constexpr __host__ __device__ int norm_wide_loads(int vec) { return vec == 1 ? 8 : 16 / vec; }
+constexpr __host__ __device__ int norm_wide_threads(bool gather) { return gather ? 1024 : 512; }
 // Rows at a time there. Forward: 16-bit rows of 4,096 take 105 us at two and 95
 // at four (32,768 rows); backward: 156 at one and 171 at two (registers).
-constexpr __host__ __device__ int norm_wide_rows(int vec, bool backward) {
-  return backward || vec == 1 ? 1 : vec == 8 ? 4 : 2;
+constexpr __host__ __device__ int norm_wide_rows(int vec, bool gather, bool backward) {
+  return backward || gather ? 1 : vec == 8 ? 4 : 2;
 }
 
-// VEC values of a row: one 16-byte load where the layout allows it, else one value.
-template <class V, int VEC>
+// Whether such rows take a whole warp each: norm_shape raises the values of a
+// thread only where 32 threads are too few.
+constexpr __host__ __device__ bool norm_full_warp(int vec, int nv, bool wide, bool gather) {
+  return !wide && (gather ? vec > 4 : nv > 1);
+}
+
+// VEC values of a row for one thread: 16 consecutive bytes, or, where the layout
+// has no such vectors (GATHER), every `step`-th value from the thread's first,
+// `count` of them, so that a warp's accesses are consecutive.
+template <class V, int VEC, bool GATHER>
 struct Pack {
   using T = typename V::T;
-  using Raw = std::conditional_t<VEC == 1, T, uint4>;
-  static_assert(VEC == 1 || VEC * sizeof(T) == 16, "a vector is 16 bytes");
-  static __device__ __forceinline__ Raw load(const T *p) {
-    if constexpr (VEC == 1) return *p;
-    else return *reinterpret_cast<const uint4 *>(p);
-  }
-  static __device__ __forceinline__ Raw zero() {
-    if constexpr (VEC == 1) return V::store(0.0f);
-    else return make_uint4(0u, 0u, 0u, 0u);
-  }
-  static __device__ __forceinline__ void open(const Raw &r, float (&f)[VEC]) {
-    if constexpr (VEC == 1) {
-      f[0] = V::load(r);
-    } else {
-      const T *v = reinterpret_cast<const T *>(&r);
+  struct Values {
+    T v[VEC];
+  };
+  using Raw = std::conditional_t<GATHER, Values, uint4>;
+  static_assert(GATHER || VEC * sizeof(T) == 16, "a vector is 16 bytes");
+  // Values that every thread has whatever the row's length, by norm_shape's
+  // choice of VEC: no test of their columns. One of 4 (dim >= 1), half of 8 to
+  // 32 over a warp (dim > 16 VEC), the same of 8 over a block (dim > 1,024).
+  static constexpr int kSure = !GATHER ? 0 : VEC == 4 ? 1 : VEC / 2;
+  static __device__ __forceinline__ Raw zeros() {
+    if constexpr (GATHER) {
+      Values r;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) f[i] = V::load(v[i]);
+      for (int i = 0; i < VEC; ++i) r.v[i] = V::store(0.0f);
+      return r;
+    } else {
+      return make_uint4(0u, 0u, 0u, 0u);
     }
   }
-  static __device__ __forceinline__ void store(T *p, const float (&f)[VEC]) {
-    if constexpr (VEC == 1) {
-      *p = V::store(f[0]);
+  // of a row that is there; zeros behind its `count` values
+  static __device__ __forceinline__ Raw load(const T *p, int step, int count) {
+    if constexpr (GATHER) {
+      Values r;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) r.v[i] = i < kSure || i < count ? p[i * step] : V::store(0.0f);
+      return r;
     } else {
+      return count > 0 ? *reinterpret_cast<const uint4 *>(p) : make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
+  static __device__ __forceinline__ void open(const Raw &r, float (&f)[VEC]) {
+    const T *v = reinterpret_cast<const T *>(&r);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) f[i] = V::load(v[i]);
+  }
+  static __device__ __forceinline__ void store(T *p, const float (&f)[VEC], int step, int count) {
+    if constexpr (GATHER) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        if (i < kSure || i < count) p[i * step] = V::store(f[i]);
+    } else if (count > 0) {
       uint4 r;
       T *v = reinterpret_cast<T *>(&r);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) v[i] = V::store(f[i]);
       *reinterpret_cast<uint4 *>(p) = r;
     }
+  }
+  // Column of value i of a thread's vector v, and how many values that has.
+  static __device__ __forceinline__ int column(int v, int lane, int lanes, int i) {
+    return GATHER ? lane + i * lanes : (v * lanes + lane) * VEC + i;
+  }
+  static __device__ __forceinline__ int count(int v, int lane, int lanes, int dim) {
+    if constexpr (GATHER) return max(0, min(VEC, (dim - lane + lanes - 1) / lanes));
+    else return (v * lanes + lane) * VEC < dim ? VEC : 0;
   }
 };
 
@@ -256,9 +289,15 @@ struct RowSum {
 // A bulk copy moves whole 16-byte units. Where rows do not start and end at
 // such (ALIGNED false), the units that hold a row's first and last bytes are
 // copied whole and the row is found inside; those of the matrix's first and
-// last row reach past it, so the tiles with these two rows are not copied:
-// the threads read them in place.
+// last rows reach past it, so the tiles with these rows (or, where a row is
+// shorter than a unit, within a unit of them) are not copied: the threads read
+// them in place.
 constexpr int kNormStages = 8;
+// Up to this many bytes, rows with gaps are not copied either but read in place
+// (`direct`): a copy for each is then too many copies. 2^25 values, forward:
+// rows of 8 fp32 values with a gap of one 386 us copied, 157 in place; of 256,
+// 64 and 61; of 517, 110 and 117.
+constexpr size_t kNormDirectBytes = 1024;
 template <class T, int N, bool ALIGNED>
 struct RowRing {
   const T *src[N];
@@ -268,6 +307,7 @@ struct RowRing {
   uint8_t *buf;
   uint64_t *bars;
   volatile uint32_t *given_up;
+  bool direct;
   int at = 0;
   uint32_t parity = 0;
 
@@ -279,15 +319,18 @@ struct RowRing {
     return buf + size_t(stage * N + n) * rows * pitch(dim);
   }
   __device__ __forceinline__ bool covers(int64_t base) const {
-    return ALIGNED || (base > 0 && base + rows < rows_total);
+    const int edge = size_t(dim) * sizeof(T) >= 16 ? 1 : 8;  // rows of at least 16 bytes together
+    return ALIGNED || (!direct && base >= edge && base + rows + edge <= rows_total);
   }
   // Row r of the tile in turn, which `covers` it.
   __device__ __forceinline__ const T *row(int n, int r, int64_t base) const {
     const uint8_t *b = buffer(at, n);
     if constexpr (ALIGNED) return reinterpret_cast<const T *>(b) + r * dim;
+    // the address modulo 16, for which 32 bits are enough
     const bool dense = stride[n] == dim;
-    const uintptr_t from = reinterpret_cast<uintptr_t>(src[n] + (dense ? base : base + r) * stride[n]);
-    return reinterpret_cast<const T *>(b + (dense ? size_t(r) * dim * sizeof(T) : r * pitch(dim)) + (from & 15));
+    const uint32_t at_row = uint32_t(base) + (dense ? 0u : uint32_t(r));
+    const uint32_t from = uint32_t(reinterpret_cast<uintptr_t>(src[n])) + at_row * uint32_t(stride[n] * sizeof(T));
+    return reinterpret_cast<const T *>(b + uint32_t(r) * uint32_t(dense ? dim * sizeof(T) : pitch(dim)) + (from & 15));
   }
   __device__ __forceinline__ static uint32_t units(const T *from, int64_t values, const uint8_t *&first) {
     const uintptr_t a = reinterpret_cast<uintptr_t>(from), e = a + size_t(values) * sizeof(T);
@@ -360,18 +403,19 @@ struct RowRing {
 // Rows held in registers: `lanes` threads per row (a power of two up to 32, or
 // with WIDE the block), NV vectors of VEC values per thread, U rows at a time
 // (their loads are in flight together).
-template <class V, int VEC, int NV, int U, bool WIDE>
-__global__ void __launch_bounds__(WIDE ? norm_wide_threads(VEC) : kNormNarrowThreads, !WIDE && NV == 1 ? 3 : 1)
+template <class V, int VEC, int NV, int U, bool WIDE, bool GATHER>
+__global__ void __launch_bounds__(WIDE ? norm_wide_threads(GATHER) : kNormNarrowThreads, !WIDE && (GATHER ? VEC <= 8 : NV == 1) ? 3 : 1)
 k_norm_forward(const typename V::T *__restrict__ x, int64_t x_stride, int64_t rows, int dim,
                const void *__restrict__ weight, const void *__restrict__ bias, int ptype, float eps,
-               typename V::T *__restrict__ y, float *__restrict__ mean_out, float *__restrict__ rstd_out, int lanes,
+               typename V::T *__restrict__ y, float *__restrict__ mean_out, float *__restrict__ rstd_out, int lanes_of_row,
                int stages, uint32_t *status) {
-  using P = Pack<V, VEC>;
+  using P = Pack<V, VEC, GATHER>;
   using T = typename V::T;
   __shared__ float red[2][32][4];
   __shared__ uint64_t bars[kNormStages];
   __shared__ volatile uint32_t given_up;
   extern __shared__ __align__(128) uint8_t raw_smem[];
+  const int lanes = norm_full_warp(VEC, NV, WIDE, GATHER) ? 32 : lanes_of_row;
   const int lane = WIDE ? int(threadIdx.x) : int(threadIdx.x) & (lanes - 1);
   const int group = WIDE ? 0 : int(threadIdx.x) / lanes;
   const int groups = WIDE ? 1 : int(blockDim.x) / lanes;
@@ -380,7 +424,7 @@ k_norm_forward(const typename V::T *__restrict__ x, int64_t x_stride, int64_t ro
   for (int v = 0; v < NV; ++v) {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      const int c = (v * lanes + lane) * VEC + i;
+      const int c = P::column(v, lane, lanes, i);
       w[v][i] = c < dim ? param_at(weight, ptype, c, 1.0f) : 0.0f;
       b[v][i] = c < dim ? param_at(bias, ptype, c, 0.0f) : 0.0f;
     }
@@ -388,7 +432,7 @@ k_norm_forward(const typename V::T *__restrict__ x, int64_t x_stride, int64_t ro
   RowSum<U, WIDE> sum{lanes, red};
   const float inv = 1.0f / float(dim);
   const int64_t first = int64_t(blockIdx.x) * groups * U, step = int64_t(gridDim.x) * groups * U;
-  RowRing<T, 1, (VEC > 1)> ring{{x}, {x_stride}, rows, step, groups * U, dim, stages, raw_smem, bars, &given_up};
+  RowRing<T, 1, !GATHER> ring{{x}, {x_stride}, rows, step, groups * U, dim, stages, raw_smem, bars, &given_up, !WIDE && x_stride != dim && dim * sizeof(T) <= kNormDirectBytes};
   ring.start(first);
   for (int64_t base = first; base < rows; base += step) {
     typename P::Raw raw[U][NV];
@@ -399,9 +443,10 @@ k_norm_forward(const typename V::T *__restrict__ x, int64_t x_stride, int64_t ro
       const T *staged = ring.row(0, group * U + u, base);
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
-        const int c = (v * lanes + lane) * VEC;
-        raw[u][v] = P::zero();
-        if (row < rows && c < dim) raw[u][v] = copied ? P::load(staged + c) : P::load(x + row * x_stride + c);
+        const int c = P::column(v, lane, lanes, 0), n = P::count(v, lane, lanes, dim);
+        if (GATHER ? !copied && row >= rows : row >= rows) raw[u][v] = P::zeros();
+        else if (copied) raw[u][v] = P::load(staged + c, lanes, n);
+        else raw[u][v] = P::load(x + row * x_stride + c, lanes, n);
       }
     }
     if (__syncthreads_or(!ok)) {
@@ -430,7 +475,12 @@ k_norm_forward(const typename V::T *__restrict__ x, int64_t x_stride, int64_t ro
       float t[VEC];
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
-        if ((v * lanes + lane) * VEC < dim) vadd(f[u][v], f[u][v], minus.v);
+        const int n = P::count(v, lane, lanes, dim);
+        if (GATHER || n > 0) vadd(f[u][v], f[u][v], minus.v);
+        if (GATHER) {
+#pragma unroll
+          for (int i = P::kSure; i < VEC; ++i) f[u][v][i] = i < n ? f[u][v][i] : 0.0f;
+        }
         if (v == 0) vmul(t, f[u][v], f[u][v]);
         else vfma(t, f[u][v], f[u][v], t);
       }
@@ -466,10 +516,9 @@ k_norm_forward(const typename V::T *__restrict__ x, int64_t x_stride, int64_t ro
       const All<VEC> r(s[u]);
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
-        const int c = (v * lanes + lane) * VEC;
         vmul(f[u][v], f[u][v], r.v);
         vfma(f[u][v], f[u][v], w[v], b[v]);
-        if (c < dim) P::store(y + row * dim + c, f[u][v]);
+        P::store(y + row * dim + P::column(v, lane, lanes, 0), f[u][v], lanes, P::count(v, lane, lanes, dim));
       }
     }
   }
@@ -509,19 +558,20 @@ k_norm_forward_long(const typename V::T *__restrict__ x, int64_t x_stride, int64
 // Backward of rows held in registers (layout as k_norm_forward). partial:
 // [gridDim.x][2][dim] fp32, this block's sums of g h and of g per column
 // (null: no weight gradients wanted).
-template <class V, int VEC, int NV, int U, bool WIDE>
-__global__ void __launch_bounds__(WIDE ? norm_wide_threads(VEC) : kNormNarrowThreads, !WIDE && NV <= 2 ? 2 : 1)
+template <class V, int VEC, int NV, int U, bool WIDE, bool GATHER>
+__global__ void __launch_bounds__(WIDE ? norm_wide_threads(GATHER) : kNormNarrowThreads, !WIDE && (GATHER ? VEC <= 16 : NV <= 2) ? 2 : 1)
 k_norm_backward(const typename V::T *__restrict__ grad, int64_t g_stride, const typename V::T *__restrict__ x,
                 int64_t x_stride, int64_t rows, int dim, const float *__restrict__ mean,
                 const float *__restrict__ rstd, const void *__restrict__ weight, int ptype,
-                typename V::T *__restrict__ dx, float *__restrict__ partial, int lanes, int stages,
+                typename V::T *__restrict__ dx, float *__restrict__ partial, int lanes_of_row, int stages,
                 uint32_t *status) {
-  using P = Pack<V, VEC>;
+  using P = Pack<V, VEC, GATHER>;
   using T = typename V::T;
   __shared__ float red[2][32][4];
   __shared__ uint64_t bars[kNormStages];
   __shared__ volatile uint32_t given_up;
   extern __shared__ __align__(128) uint8_t raw_smem[];  // the ring; at the end, narrow: [warps][dim] fp32
+  const int lanes = norm_full_warp(VEC, NV, WIDE, GATHER) ? 32 : lanes_of_row;
   const int lane = WIDE ? int(threadIdx.x) : int(threadIdx.x) & (lanes - 1);
   const int group = WIDE ? 0 : int(threadIdx.x) / lanes;
   const int groups = WIDE ? 1 : int(blockDim.x) / lanes;
@@ -530,7 +580,7 @@ k_norm_backward(const typename V::T *__restrict__ grad, int64_t g_stride, const 
   for (int v = 0; v < NV; ++v) {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      const int c = (v * lanes + lane) * VEC + i;
+      const int c = P::column(v, lane, lanes, i);
       w[v][i] = c < dim ? param_at(weight, ptype, c, 1.0f) : 0.0f;
       dw[v][i] = 0.0f;
       db[v][i] = 0.0f;
@@ -539,8 +589,8 @@ k_norm_backward(const typename V::T *__restrict__ grad, int64_t g_stride, const 
   RowSum<WIDE ? 2 * U : U, WIDE> sum{lanes, red};
   const float inv = 1.0f / float(dim);
   const int64_t first = int64_t(blockIdx.x) * groups * U, step = int64_t(gridDim.x) * groups * U;
-  RowRing<T, 2, (VEC > 1)> ring{{x, grad}, {x_stride, g_stride}, rows,     step, groups * U, dim,
-                                stages,    raw_smem,             bars,     &given_up};
+  RowRing<T, 2, !GATHER> ring{{x, grad}, {x_stride, g_stride}, rows,     step, groups * U, dim,
+                                stages, raw_smem, bars, &given_up, !WIDE && (x_stride != dim || g_stride != dim) && dim * sizeof(T) <= kNormDirectBytes};
   ring.start(first);
   float next_m[U], next_r[U];  // a tile's statistics are asked for a tile ahead
   auto ask = [&](int64_t at) {
@@ -568,11 +618,15 @@ k_norm_backward(const typename V::T *__restrict__ grad, int64_t g_stride, const 
       const T *xs = ring.row(0, group * U + u, base), *gs = ring.row(1, group * U + u, base);
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
-        const int c = (v * lanes + lane) * VEC;
-        xr[u][v] = gr[u][v] = P::zero();
-        if (row < rows && c < dim) {
-          xr[u][v] = copied ? P::load(xs + c) : P::load(x + row * x_stride + c);
-          gr[u][v] = copied ? P::load(gs + c) : P::load(grad + row * g_stride + c);
+        const int c = P::column(v, lane, lanes, 0), n = P::count(v, lane, lanes, dim);
+        if (GATHER ? !copied && row >= rows : row >= rows) {
+          xr[u][v] = gr[u][v] = P::zeros();
+        } else if (copied) {
+          xr[u][v] = P::load(xs + c, lanes, n);
+          gr[u][v] = P::load(gs + c, lanes, n);
+        } else {
+          xr[u][v] = P::load(x + row * x_stride + c, lanes, n);
+          gr[u][v] = P::load(grad + row * g_stride + c, lanes, n);
         }
       }
     }
@@ -630,7 +684,6 @@ k_norm_backward(const typename V::T *__restrict__ grad, int64_t g_stride, const 
       const All<VEC> rr(r[u]), mr(-m[u] * r[u]), c0(-r[u] * (s0[u] * inv)), c1(-r[u] * (s1[u] * inv));
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
-        const int c = (v * lanes + lane) * VEC;
         float h[VEC], g[VEC];
         P::open(xr[u][v], h);
         P::open(gr[u][v], g);
@@ -638,7 +691,7 @@ k_norm_backward(const typename V::T *__restrict__ grad, int64_t g_stride, const 
         vmul(g, g, w[v]);
         vfma(g, g, rr.v, c0.v);  // r q - r sum q / D - h r sum(q h) / D
         vfma(g, h, c1.v, g);
-        if (c < dim) P::store(dx + row * dim + c, g);
+        P::store(dx + row * dim + P::column(v, lane, lanes, 0), g, lanes, P::count(v, lane, lanes, dim));
       }
     }
   }
@@ -650,7 +703,7 @@ k_norm_backward(const typename V::T *__restrict__ grad, int64_t g_stride, const 
     for (int v = 0; v < NV; ++v) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        const int c = (v * lanes + lane) * VEC + i;
+        const int c = P::column(v, lane, lanes, i);
         if (c < dim) {
           out[c] = dw[v][i];
           out[dim + c] = db[v][i];
@@ -673,7 +726,7 @@ k_norm_backward(const typename V::T *__restrict__ grad, int64_t g_stride, const 
           for (int o = 16; o > 0; o >>= 1) {
             if (o >= lanes) f += __shfl_xor_sync(0xffffffffu, f, o);
           }
-          const int c = (v * lanes + lane) * VEC + i;
+          const int c = P::column(v, lane, lanes, i);
           if ((threadIdx.x & 31) < unsigned(lanes) && c < dim) cols[warp * dim + c] = f;
         }
       }
@@ -785,18 +838,24 @@ NormShape norm_shape(int64_t dim, size_t value_size, bool aligned, bool backward
   s.vec = aligned && dim % per == 0;
   const int64_t n = s.vec ? dim / per : dim;  // loads per row
   s.threads = kNormNarrowThreads;
-  if (n <= 128) {
-    s.nv = n <= 32 ? 1 : n <= 64 ? 2 : 4;
-    s.unroll = 4 / s.nv;
+  if (s.vec ? n <= 128 : n <= 1024) {
+    if (s.vec) {
+      s.nv = n <= 32 ? 1 : n <= 64 ? 2 : 4;
+      s.unroll = 4 / s.nv;
+    } else {
+      s.nv = n <= 128 ? 4 : n <= 256 ? 8 : n <= 512 ? 16 : 32;
+      s.unroll = s.nv == 4 ? 4 : s.nv == 8 ? 2 : 1;
+    }
+    const int64_t lanes = s.vec ? n : (n + s.nv - 1) / s.nv;
     s.lanes = 1;
-    while (s.lanes < n && s.lanes < 32) s.lanes *= 2;
+    while (s.lanes < lanes && s.lanes < 32) s.lanes *= 2;
     return s;
   }
-  s.nv = norm_wide_loads(s.vec ? per : 1);
-  s.unroll = norm_wide_rows(s.vec ? per : 1, backward);
+  s.nv = s.vec ? 16 / per : 8;
+  s.unroll = norm_wide_rows(per, !s.vec, backward);
   s.wide = true;
   const int64_t threads = (n + s.nv - 1) / s.nv;
-  const int most = norm_wide_threads(s.vec ? per : 1);
+  const int most = norm_wide_threads(!s.vec);
   s.longer = threads > most;
   s.threads = int(std::min<int64_t>(most, (threads + 31) / 32 * 32));
   s.lanes = s.threads;
@@ -834,16 +893,24 @@ NormLaunch norm_launch(K *kernel, const NormShape &s, int64_t rows, int64_t dim,
 // time, a block per row.
 template <class V, bool BACKWARD, class F>
 void with_norm_shape(const NormShape &s, F &&f) {
+  constexpr int kVec = int(16 / sizeof(typename V::T));
+  const std::false_type no{};
+  const std::true_type yes{};
   using std::integral_constant;
-  auto go = [&](auto vec) {
-    constexpr int kVec = decltype(vec)::value;
-    if (s.wide) f(vec, integral_constant<int, norm_wide_loads(kVec)>{}, integral_constant<int, norm_wide_rows(kVec, BACKWARD)>{}, std::true_type{});
-    else if (s.nv == 1) f(vec, integral_constant<int, 1>{}, integral_constant<int, 4>{}, std::false_type{});
-    else if (s.nv == 2) f(vec, integral_constant<int, 2>{}, integral_constant<int, 2>{}, std::false_type{});
-    else f(vec, integral_constant<int, 4>{}, integral_constant<int, 1>{}, std::false_type{});
-  };
-  if (s.vec) go(integral_constant<int, int(16 / sizeof(typename V::T))>{});
-  else go(integral_constant<int, 1>{});
+  if (s.vec) {
+    const integral_constant<int, kVec> vec{};
+    if (s.wide) f(vec, integral_constant<int, 16 / kVec>{}, integral_constant<int, norm_wide_rows(kVec, false, BACKWARD)>{}, yes, no);
+    else if (s.nv == 1) f(vec, integral_constant<int, 1>{}, integral_constant<int, 4>{}, no, no);
+    else if (s.nv == 2) f(vec, integral_constant<int, 2>{}, integral_constant<int, 2>{}, no, no);
+    else f(vec, integral_constant<int, 4>{}, integral_constant<int, 1>{}, no, no);
+  } else {
+    const integral_constant<int, 1> one{};
+    if (s.wide) f(integral_constant<int, 8>{}, one, one, yes, yes);
+    else if (s.nv == 4) f(integral_constant<int, 4>{}, one, integral_constant<int, 4>{}, no, yes);
+    else if (s.nv == 8) f(integral_constant<int, 8>{}, one, integral_constant<int, 2>{}, no, yes);
+    else if (s.nv == 16) f(integral_constant<int, 16>{}, one, one, no, yes);
+    else f(integral_constant<int, 32>{}, one, one, no, yes);
+  }
 }
 
 void check_norm(int32_t value_dtype, int32_t param_dtype, size_t rows, int64_t dim) {
@@ -892,8 +959,9 @@ extern "C" int se_layer_norm(int32_t value_dtype, int32_t param_dtype, const voi
         launched("k_norm_forward_long");
         return;
       }
-      with_norm_shape<V, false>(s, [&](auto vec, auto nv, auto u, auto wide) {
-        auto *kernel = k_norm_forward<V, decltype(vec)::value, decltype(nv)::value, decltype(u)::value, decltype(wide)::value>;
+      with_norm_shape<V, false>(s, [&](auto vec, auto nv, auto u, auto wide, auto gather) {
+        auto *kernel = k_norm_forward<V, decltype(vec)::value, decltype(nv)::value, decltype(u)::value, decltype(wide)::value,
+                                      decltype(gather)::value>;
         const NormLaunch l = norm_launch(kernel, s, int64_t(rows), dim, vb, 1, device, 0);
         kernel<<<l.blocks, s.threads, l.smem, st>>>(xp, x_stride, int64_t(rows), int(dim), weight, bias, param_dtype, eps,
                                                     yp, mean_out, rstd_out, s.lanes, l.stages, status);
@@ -975,8 +1043,9 @@ extern "C" int se_layer_norm_backward(int32_t value_dtype, int32_t param_dtype, 
           }
           return;
         }
-        with_norm_shape<V, true>(s, [&](auto vec, auto nv, auto u, auto wide) {
-            auto *kernel = k_norm_backward<V, decltype(vec)::value, decltype(nv)::value, decltype(u)::value, decltype(wide)::value>;
+        with_norm_shape<V, true>(s, [&](auto vec, auto nv, auto u, auto wide, auto gather) {
+            auto *kernel = k_norm_backward<V, decltype(vec)::value, decltype(nv)::value, decltype(u)::value, decltype(wide)::value,
+                                         decltype(gather)::value>;
           const size_t cols = s.wide || !sums ? 0 : size_t(s.threads / 32) * size_t(dim) * sizeof(float);
           const NormLaunch l = norm_launch(kernel, s, int64_t(rows), dim, vb, 2, device, cols);
           blocks = l.blocks;
