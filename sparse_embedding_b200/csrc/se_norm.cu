@@ -42,12 +42,6 @@ constexpr __host__ __device__ int norm_wide_rows(int vec, bool gather, bool back
   return backward || gather ? 1 : vec == 8 ? 4 : 2;
 }
 
-// Whether such rows take a whole warp each: norm_shape raises the values of a
-// thread only where 32 threads are too few.
-constexpr __host__ __device__ bool norm_full_warp(int vec, int nv, bool wide, bool gather) {
-  return !wide && (gather ? vec > 4 : nv > 1);
-}
-
 // VEC values of a row for one thread: 16 consecutive bytes, or, where the layout
 // has no such vectors (GATHER), every `step`-th value from the thread's first,
 // `count` of them, so that a warp's accesses are consecutive.
@@ -60,8 +54,10 @@ struct Pack {
   using Raw = std::conditional_t<GATHER, Values, uint4>;
   static_assert(GATHER || VEC * sizeof(T) == 16, "a vector is 16 bytes");
   // Values that every thread has whatever the row's length, by norm_shape's
-  // choice of VEC: no test of their columns. One of 4 (dim >= 1), half of 8 to
-  // 32 over a warp (dim > 16 VEC), the same of 8 over a block (dim > 1,024).
+  // choice of VEC and lanes: no test of their columns. Lanes are the least power
+  // of two with VEC values each, so the row fills more than half of them (VEC
+  // 8 to 32: dim > VEC / 2 lanes); VEC 4 takes rows from one value on. Over a
+  // block lanes < dim / 8 + 32 and dim > 1,024, so 4 of 8 as well.
   static constexpr int kSure = !GATHER ? 0 : VEC == 4 ? 1 : VEC / 2;
   static __device__ __forceinline__ Raw zeros() {
     if constexpr (GATHER) {
@@ -293,11 +289,6 @@ struct RowSum {
 // shorter than a unit, within a unit of them) are not copied: the threads read
 // them in place.
 constexpr int kNormStages = 8;
-// Up to this many bytes, rows with gaps are not copied either but read in place
-// (`direct`): a copy for each is then too many copies. 2^25 values, forward:
-// rows of 8 fp32 values with a gap of one 386 us copied, 157 in place; of 256,
-// 64 and 61; of 517, 110 and 117.
-constexpr size_t kNormDirectBytes = 1024;
 template <class T, int N, bool ALIGNED>
 struct RowRing {
   const T *src[N];
@@ -307,7 +298,6 @@ struct RowRing {
   uint8_t *buf;
   uint64_t *bars;
   volatile uint32_t *given_up;
-  bool direct;
   int at = 0;
   uint32_t parity = 0;
 
@@ -320,7 +310,7 @@ struct RowRing {
   }
   __device__ __forceinline__ bool covers(int64_t base) const {
     const int edge = size_t(dim) * sizeof(T) >= 16 ? 1 : 8;  // rows of at least 16 bytes together
-    return ALIGNED || (!direct && base >= edge && base + rows + edge <= rows_total);
+    return ALIGNED || (base >= edge && base + rows + edge <= rows_total);
   }
   // Row r of the tile in turn, which `covers` it.
   __device__ __forceinline__ const T *row(int n, int r, int64_t base) const {
@@ -403,8 +393,9 @@ struct RowRing {
 // Rows held in registers: `lanes` threads per row (a power of two up to 32, or
 // with WIDE the block), NV vectors of VEC values per thread, U rows at a time
 // (their loads are in flight together).
-template <class V, int VEC, int NV, int U, bool WIDE, bool GATHER>
-__global__ void __launch_bounds__(WIDE ? norm_wide_threads(GATHER) : kNormNarrowThreads, !WIDE && (GATHER ? VEC <= 8 : NV == 1) ? 3 : 1)
+template <class V, int VEC, int NV, int U, bool WIDE, bool GATHER, bool RING, int LANES>
+__global__ void __launch_bounds__(WIDE ? norm_wide_threads(GATHER) : kNormNarrowThreads,
+                                  !WIDE && (GATHER ? VEC <= 8 : NV == 1) ? 3 : 1)
 k_norm_forward(const typename V::T *__restrict__ x, int64_t x_stride, int64_t rows, int dim,
                const void *__restrict__ weight, const void *__restrict__ bias, int ptype, float eps,
                typename V::T *__restrict__ y, float *__restrict__ mean_out, float *__restrict__ rstd_out, int lanes_of_row,
@@ -415,7 +406,7 @@ k_norm_forward(const typename V::T *__restrict__ x, int64_t x_stride, int64_t ro
   __shared__ uint64_t bars[kNormStages];
   __shared__ volatile uint32_t given_up;
   extern __shared__ __align__(128) uint8_t raw_smem[];
-  const int lanes = norm_full_warp(VEC, NV, WIDE, GATHER) ? 32 : lanes_of_row;
+  const int lanes = LANES > 0 ? LANES : lanes_of_row;
   const int lane = WIDE ? int(threadIdx.x) : int(threadIdx.x) & (lanes - 1);
   const int group = WIDE ? 0 : int(threadIdx.x) / lanes;
   const int groups = WIDE ? 1 : int(blockDim.x) / lanes;
@@ -432,15 +423,15 @@ k_norm_forward(const typename V::T *__restrict__ x, int64_t x_stride, int64_t ro
   RowSum<U, WIDE> sum{lanes, red};
   const float inv = 1.0f / float(dim);
   const int64_t first = int64_t(blockIdx.x) * groups * U, step = int64_t(gridDim.x) * groups * U;
-  RowRing<T, 1, !GATHER> ring{{x}, {x_stride}, rows, step, groups * U, dim, stages, raw_smem, bars, &given_up, !WIDE && x_stride != dim && dim * sizeof(T) <= kNormDirectBytes};
-  ring.start(first);
+  RowRing<T, 1, !GATHER> ring{{x}, {x_stride}, rows, step, groups * U, dim, stages, raw_smem, bars, &given_up};
+  if (RING) ring.start(first);
   for (int64_t base = first; base < rows; base += step) {
     typename P::Raw raw[U][NV];
-    const bool ok = ring.ready(), copied = ring.covers(base);
+    const bool ok = !RING || ring.ready(), copied = RING && ring.covers(base);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t row = base + group * U + u;
-      const T *staged = ring.row(0, group * U + u, base);
+      const T *staged = RING ? ring.row(0, group * U + u, base) : nullptr;
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
         const int c = P::column(v, lane, lanes, 0), n = P::count(v, lane, lanes, dim);
@@ -449,11 +440,13 @@ k_norm_forward(const typename V::T *__restrict__ x, int64_t x_stride, int64_t ro
         else raw[u][v] = P::load(x + row * x_stride + c, lanes, n);
       }
     }
-    if (__syncthreads_or(!ok)) {
-      ring.drain(base, status);
-      return;
+    if constexpr (RING) {
+      if (__syncthreads_or(!ok)) {
+        ring.drain(base, status);
+        return;
+      }
+      ring.next(base);
     }
-    ring.next(base);
     // values beyond the row are zeros, and zeros again after the mean is taken off
     float f[U][NV][VEC], m[U], s[U];
 #pragma unroll
@@ -558,8 +551,9 @@ k_norm_forward_long(const typename V::T *__restrict__ x, int64_t x_stride, int64
 // Backward of rows held in registers (layout as k_norm_forward). partial:
 // [gridDim.x][2][dim] fp32, this block's sums of g h and of g per column
 // (null: no weight gradients wanted).
-template <class V, int VEC, int NV, int U, bool WIDE, bool GATHER>
-__global__ void __launch_bounds__(WIDE ? norm_wide_threads(GATHER) : kNormNarrowThreads, !WIDE && (GATHER ? VEC <= 16 : NV <= 2) ? 2 : 1)
+template <class V, int VEC, int NV, int U, bool WIDE, bool GATHER, bool RING, int LANES>
+__global__ void __launch_bounds__(WIDE ? norm_wide_threads(GATHER) : kNormNarrowThreads,
+                                  !WIDE && (GATHER ? VEC <= 16 : NV <= 2) ? 2 : 1)
 k_norm_backward(const typename V::T *__restrict__ grad, int64_t g_stride, const typename V::T *__restrict__ x,
                 int64_t x_stride, int64_t rows, int dim, const float *__restrict__ mean,
                 const float *__restrict__ rstd, const void *__restrict__ weight, int ptype,
@@ -571,7 +565,7 @@ k_norm_backward(const typename V::T *__restrict__ grad, int64_t g_stride, const 
   __shared__ uint64_t bars[kNormStages];
   __shared__ volatile uint32_t given_up;
   extern __shared__ __align__(128) uint8_t raw_smem[];  // the ring; at the end, narrow: [warps][dim] fp32
-  const int lanes = norm_full_warp(VEC, NV, WIDE, GATHER) ? 32 : lanes_of_row;
+  const int lanes = LANES > 0 ? LANES : lanes_of_row;
   const int lane = WIDE ? int(threadIdx.x) : int(threadIdx.x) & (lanes - 1);
   const int group = WIDE ? 0 : int(threadIdx.x) / lanes;
   const int groups = WIDE ? 1 : int(blockDim.x) / lanes;
@@ -589,9 +583,9 @@ k_norm_backward(const typename V::T *__restrict__ grad, int64_t g_stride, const 
   RowSum<WIDE ? 2 * U : U, WIDE> sum{lanes, red};
   const float inv = 1.0f / float(dim);
   const int64_t first = int64_t(blockIdx.x) * groups * U, step = int64_t(gridDim.x) * groups * U;
-  RowRing<T, 2, !GATHER> ring{{x, grad}, {x_stride, g_stride}, rows,     step, groups * U, dim,
-                                stages, raw_smem, bars, &given_up, !WIDE && (x_stride != dim || g_stride != dim) && dim * sizeof(T) <= kNormDirectBytes};
-  ring.start(first);
+  RowRing<T, 2, !GATHER> ring{{x, grad}, {x_stride, g_stride}, rows, step, groups * U, dim,
+                              stages,    raw_smem,             bars, &given_up};
+  if (RING) ring.start(first);
   float next_m[U], next_r[U];  // a tile's statistics are asked for a tile ahead
   auto ask = [&](int64_t at) {
 #pragma unroll
@@ -611,11 +605,12 @@ k_norm_backward(const typename V::T *__restrict__ grad, int64_t g_stride, const 
       r[u] = next_r[u];
     }
     ask(base + step);
-    const bool ok = ring.ready(), copied = ring.covers(base);
+    const bool ok = !RING || ring.ready(), copied = RING && ring.covers(base);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t row = base + group * U + u;
-      const T *xs = ring.row(0, group * U + u, base), *gs = ring.row(1, group * U + u, base);
+      const T *xs = RING ? ring.row(0, group * U + u, base) : nullptr;
+      const T *gs = RING ? ring.row(1, group * U + u, base) : nullptr;
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
         const int c = P::column(v, lane, lanes, 0), n = P::count(v, lane, lanes, dim);
@@ -630,11 +625,13 @@ k_norm_backward(const typename V::T *__restrict__ grad, int64_t g_stride, const 
         }
       }
     }
-    if (__syncthreads_or(!ok)) {
-      ring.drain(base, status);
-      return;
+    if constexpr (RING) {
+      if (__syncthreads_or(!ok)) {
+        ring.drain(base, status);
+        return;
+      }
+      ring.next(base);
     }
-    ring.next(base);
     // rows and columns beyond the matrix have r, g and w zero: they add nothing
     float s0[U], s1[U], both[2 * U];
 #pragma unroll
@@ -828,11 +825,21 @@ struct NormLaunch {
 struct NormShape {
   bool vec;    // 16-byte vectors
   bool wide;   // a block per row
+  bool ring;   // through shared memory
   bool longer; // rows beyond a block's registers
   int nv, lanes, threads, unroll;
 };
 
-NormShape norm_shape(int64_t dim, size_t value_size, bool aligned, bool backward) {
+// Rows of up to 256 values without 16-byte layout, and vectors of up to 64 loads
+// with gaps, are read in place: a copy for each such row is too many copies, and
+// without gaps copying gains nothing there. 2^25 values, forward, copied and in
+// place: fp32 rows of 64 with a gap of 8 78 and 49 us, of 8 with a gap of 8 407
+// and 74, bf16 rows of 33 106 and 88; in place loses at longer rows (517 fp32
+// values with a gap of 8, 110 and 118).
+//
+// Single values: 8 a thread where the row fits a part of a warp (33 bf16 values
+// 88 us with 4 a thread, 66 with 8, 81 with 16), more only for longer rows.
+NormShape norm_shape(int64_t dim, size_t value_size, bool aligned, bool gaps, bool backward) {
   NormShape s{};
   const int per = int(16 / value_size);
   s.vec = aligned && dim % per == 0;
@@ -842,9 +849,11 @@ NormShape norm_shape(int64_t dim, size_t value_size, bool aligned, bool backward
     if (s.vec) {
       s.nv = n <= 32 ? 1 : n <= 64 ? 2 : 4;
       s.unroll = 4 / s.nv;
+      s.ring = !gaps || s.nv > 2;
     } else {
-      s.nv = n <= 128 ? 4 : n <= 256 ? 8 : n <= 512 ? 16 : 32;
-      s.unroll = s.nv == 4 ? 4 : s.nv == 8 ? 2 : 1;
+      s.nv = n <= 32 ? 4 : n <= 256 ? 8 : n <= 512 ? 16 : 32;
+      s.unroll = s.nv <= 8 ? 2 : 1;
+      s.ring = s.nv > 8;
     }
     const int64_t lanes = s.vec ? n : (n + s.nv - 1) / s.nv;
     s.lanes = 1;
@@ -853,7 +862,7 @@ NormShape norm_shape(int64_t dim, size_t value_size, bool aligned, bool backward
   }
   s.nv = s.vec ? 16 / per : 8;
   s.unroll = norm_wide_rows(per, !s.vec, backward);
-  s.wide = true;
+  s.wide = s.ring = true;
   const int64_t threads = (n + s.nv - 1) / s.nv;
   const int most = norm_wide_threads(!s.vec);
   s.longer = threads > most;
@@ -881,35 +890,48 @@ NormLaunch norm_launch(K *kernel, const NormShape &s, int64_t rows, int64_t dim,
   const int64_t tile_rows = int64_t(s.threads / s.lanes) * s.unroll;
   const size_t row = s.vec ? size_t(dim) * value_size : ((size_t(dim) * value_size + 15) & ~size_t(15)) + 16;
   const size_t tile = size_t(tile_rows) * row * arrays;
-  l.stages = int(std::max<size_t>(2, std::min<size_t>(kNormStages, size_t(49152) * arrays / tile)));
-  l.smem = tile * l.stages;
-  l.smem = std::max(l.smem, least_smem);
+  l.stages = s.ring ? int(std::max<size_t>(2, std::min<size_t>(kNormStages, size_t(49152) * arrays / tile))) : 0;
+  l.smem = std::max(tile * l.stages, least_smem);
   allow_dynamic_smem(kernel, l.smem);
   l.blocks = std::min(norm_blocks(rows, s, sms), sms * resident_blocks(kernel, device, s.threads, l.smem));
   return l;
 }
 
 // f with the kernel's constants: values per load, loads per thread, rows at a
-// time, a block per row.
+// time, a block per row, values one by one, rows through shared memory,
+// threads of a row (0: a variable; as a constant it makes the columns of single
+// values immediate offsets: rows of 65 fp32 values 69 -> 54 us forward, 116 -> 85
+// backward).
 template <class V, bool BACKWARD, class F>
 void with_norm_shape(const NormShape &s, F &&f) {
   constexpr int kVec = int(16 / sizeof(typename V::T));
   const std::false_type no{};
   const std::true_type yes{};
   using std::integral_constant;
+  const integral_constant<int, kVec> vec{};
+  const integral_constant<int, 1> one{};
+  const integral_constant<int, 2> two{};
+  const integral_constant<int, 4> four{};
+  const integral_constant<int, 0> any{};
+  const integral_constant<int, 32> all{};
   if (s.vec) {
-    const integral_constant<int, kVec> vec{};
-    if (s.wide) f(vec, integral_constant<int, 16 / kVec>{}, integral_constant<int, norm_wide_rows(kVec, false, BACKWARD)>{}, yes, no);
-    else if (s.nv == 1) f(vec, integral_constant<int, 1>{}, integral_constant<int, 4>{}, no, no);
-    else if (s.nv == 2) f(vec, integral_constant<int, 2>{}, integral_constant<int, 2>{}, no, no);
-    else f(vec, integral_constant<int, 4>{}, integral_constant<int, 1>{}, no, no);
+    const integral_constant<int, norm_wide_rows(kVec, false, BACKWARD)> wide_rows{};
+    if (s.wide) f(vec, integral_constant<int, 16 / kVec>{}, wide_rows, yes, no, yes, any);
+    else if (s.nv == 4) f(vec, four, one, no, no, yes, all);
+    else if (s.nv == 2 && s.ring) f(vec, two, two, no, no, yes, all);
+    else if (s.nv == 2) f(vec, two, two, no, no, no, all);
+    else if (s.ring) f(vec, one, four, no, no, yes, any);
+    else f(vec, one, four, no, no, no, any);
   } else {
-    const integral_constant<int, 1> one{};
-    if (s.wide) f(integral_constant<int, 8>{}, one, one, yes, yes);
-    else if (s.nv == 4) f(integral_constant<int, 4>{}, one, integral_constant<int, 4>{}, no, yes);
-    else if (s.nv == 8) f(integral_constant<int, 8>{}, one, integral_constant<int, 2>{}, no, yes);
-    else if (s.nv == 16) f(integral_constant<int, 16>{}, one, one, no, yes);
-    else f(integral_constant<int, 32>{}, one, one, no, yes);
+    const integral_constant<int, 8> eight{};
+    const integral_constant<int, 16> sixteen{};
+    if (s.wide) f(eight, one, one, yes, yes, yes, any);
+    else if (s.nv == 4) f(four, one, two, no, yes, no, any);
+    else if (s.nv == 8 && s.lanes == 8) f(eight, one, two, no, yes, no, eight);
+    else if (s.nv == 8 && s.lanes == 16) f(eight, one, two, no, yes, no, sixteen);
+    else if (s.nv == 8) f(eight, one, two, no, yes, no, all);
+    else if (s.nv == 16) f(sixteen, one, one, no, yes, yes, all);
+    else f(integral_constant<int, 32>{}, one, one, no, yes, yes, all);
   }
 }
 
@@ -946,7 +968,8 @@ extern "C" int se_layer_norm(int32_t value_dtype, int32_t param_dtype, const voi
     const int sms = sm_count(device);
     uint32_t *status = wait_status(device);
     const size_t vb = value_bytes(value_dtype);
-    const NormShape s = norm_shape(dim, vb, aligned16(x) && aligned16(y) && (rows == 1 || x_stride * vb % 16 == 0), false);
+    const NormShape s = norm_shape(dim, vb, aligned16(x) && aligned16(y) && (rows == 1 || x_stride * vb % 16 == 0),
+                                   rows > 1 && x_stride != dim, false);
     dispatch_value(value_dtype, [&](auto tag) {
       using V = decltype(tag);
       using T = typename V::T;
@@ -959,9 +982,10 @@ extern "C" int se_layer_norm(int32_t value_dtype, int32_t param_dtype, const voi
         launched("k_norm_forward_long");
         return;
       }
-      with_norm_shape<V, false>(s, [&](auto vec, auto nv, auto u, auto wide, auto gather) {
-        auto *kernel = k_norm_forward<V, decltype(vec)::value, decltype(nv)::value, decltype(u)::value, decltype(wide)::value,
-                                      decltype(gather)::value>;
+      with_norm_shape<V, false>(s, [&](auto vec, auto nv, auto u, auto wide, auto gather, auto ring, auto lanes) {
+        auto *kernel = k_norm_forward<V, decltype(vec)::value, decltype(nv)::value, decltype(u)::value,
+                                      decltype(wide)::value, decltype(gather)::value, decltype(ring)::value,
+                                      decltype(lanes)::value>;
         const NormLaunch l = norm_launch(kernel, s, int64_t(rows), dim, vb, 1, device, 0);
         kernel<<<l.blocks, s.threads, l.smem, st>>>(xp, x_stride, int64_t(rows), int(dim), weight, bias, param_dtype, eps,
                                                     yp, mean_out, rstd_out, s.lanes, l.stages, status);
@@ -980,7 +1004,7 @@ extern "C" int se_layer_norm_backward_workspace(size_t rows, int64_t dim, int32_
     int blocks = 1;
     for (const size_t vb : {size_t(2), size_t(4)}) {
       for (const bool aligned : {false, true}) {
-        const NormShape s = norm_shape(dim, vb, aligned, true);
+        const NormShape s = norm_shape(dim, vb, aligned, false, true);
         blocks = std::max(blocks, s.longer ? int(std::min<size_t>(rows, kNormLongSplits))
                                            : norm_blocks(int64_t(rows), s, sms));
       }
@@ -1016,7 +1040,7 @@ extern "C" int se_layer_norm_backward(int32_t value_dtype, int32_t param_dtype, 
       const size_t vb = value_bytes(value_dtype);
       const NormShape s = norm_shape(dim, vb, aligned16(x) && aligned16(grad) && aligned16(dx) &&
                                                   (rows == 1 || (x_stride * vb % 16 == 0 && grad_stride * vb % 16 == 0)),
-                                     true);
+                                     rows > 1 && (x_stride != dim || grad_stride != dim), true);
       blocks = s.longer ? int(std::min<size_t>(rows, kNormLongSplits)) : norm_blocks(int64_t(rows), s, sms);
       if (sums) {
         check_device_ptr(workspace, device, "workspace");
@@ -1043,9 +1067,10 @@ extern "C" int se_layer_norm_backward(int32_t value_dtype, int32_t param_dtype, 
           }
           return;
         }
-        with_norm_shape<V, true>(s, [&](auto vec, auto nv, auto u, auto wide, auto gather) {
-            auto *kernel = k_norm_backward<V, decltype(vec)::value, decltype(nv)::value, decltype(u)::value, decltype(wide)::value,
-                                         decltype(gather)::value>;
+        with_norm_shape<V, true>(s, [&](auto vec, auto nv, auto u, auto wide, auto gather, auto ring, auto lanes) {
+          auto *kernel = k_norm_backward<V, decltype(vec)::value, decltype(nv)::value, decltype(u)::value,
+                                         decltype(wide)::value, decltype(gather)::value, decltype(ring)::value,
+                                         decltype(lanes)::value>;
           const size_t cols = s.wide || !sums ? 0 : size_t(s.threads / 32) * size_t(dim) * sizeof(float);
           const NormLaunch l = norm_launch(kernel, s, int64_t(rows), dim, vb, 2, device, cols);
           blocks = l.blocks;

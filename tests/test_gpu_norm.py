@@ -338,3 +338,31 @@ def test_neighbours_of_unaligned_rows(dim, pad, offset, dt):
     assert torch.equal(y, se.layer_norm(x.contiguous(), w)) and torch.isfinite(y).all()
     dx, dw, db = se.layer_norm_backward(x, x, mean, rstd, w)
     assert all(torch.isfinite(t).all() for t in (dx, dw, db))
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("pad", [0, 1, 8])
+@pytest.mark.parametrize("dim", [4, 5, 8, 9, 16, 17, 24, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257, 511, 512, 513,
+                                 1023, 1024, 1025, 1279])
+def test_both_sides_of_each_layout(dim, pad, dt):
+    # 301 rows: whole tiles and a last one that ends inside
+    check(*inputs(301, dim, dt, torch.float32, pad, 0))
+
+
+@pytest.mark.parametrize("dim", [1, 5, 12, 20, 33, 40, 65, 104, 129, 300, 600, 1030])
+@pytest.mark.parametrize("pad", [0, 1, 8])
+def test_rows_of_a_warp_do_not_mix(dim, pad):
+    x, g, w, b = inputs(40, dim, torch.float32, torch.float32, pad)
+    x[7, dim - 1] = float("nan")
+    x[18, 0] = float("inf")
+    g[30, dim // 2] = float("nan")
+    y, mean, rstd = se.layer_norm(x, w, b, return_stats=True)
+    dx, dw, db = se.layer_norm_backward(g, x, mean, rstd, w)
+    bad = torch.zeros(40, dtype=torch.bool, device="cuda")
+    bad[[7, 18]] = True
+    assert torch.isnan(y[bad]).all() and torch.isfinite(y[~bad]).all() and torch.isfinite(mean[~bad]).all()
+    bad[30] = True
+    assert torch.isnan(dx[bad]).all() and torch.isfinite(dx[~bad]).all()
+    want = torch.zeros(dim, dtype=torch.bool, device="cuda")
+    want[dim // 2] = True
+    assert torch.equal(torch.isnan(db), want) and torch.isnan(dw).all()
