@@ -32,14 +32,16 @@ namespace se_gpu {
 namespace {
 
 constexpr int kNormNarrowThreads = 256;  // block of the kernels with several rows per block
-// A block per row: its most threads and the values of each. Rows of up to 8,192
-// values fit the registers in every layout (the backward holds three fp32
+// A block per row: its most threads, of 16 values each, so that rows of up to
+// 8,192 values fit the registers in every layout (the backward holds three fp32
 // values per column besides the row).
-constexpr __host__ __device__ int norm_wide_threads(bool gather) { return gather ? 1024 : 512; }
+constexpr int kNormWideThreads = 512;
 // Rows at a time there. Forward: 16-bit rows of 4,096 take 105 us at two and 95
-// at four (32,768 rows); backward: 156 at one and 171 at two (registers).
+// at four (32,768 rows); backward: 156 at one and 171 at two (registers). Single
+// values, 33,538 bf16 rows of 2,001: forward 89 us at one and 78 at two (115 with
+// 8 values a thread), backward 131 at one and 183 at two.
 constexpr __host__ __device__ int norm_wide_rows(int vec, bool gather, bool backward) {
-  return backward || gather ? 1 : vec == 8 ? 4 : 2;
+  return gather ? (backward ? 1 : 2) : backward ? 1 : vec == 8 ? 4 : 2;
 }
 
 // VEC values of a row for one thread: 16 consecutive bytes, or, where the layout
@@ -57,7 +59,7 @@ struct Pack {
   // choice of VEC and lanes: no test of their columns. Lanes are the least power
   // of two with VEC values each, so the row fills more than half of them (VEC
   // 8 to 32: dim > VEC / 2 lanes); VEC 4 takes rows from one value on. Over a
-  // block lanes < dim / 8 + 32 and dim > 1,024, so 4 of 8 as well.
+  // block lanes < dim / 16 + 32 and dim > 1,024, so 8 of 16 as well.
   static constexpr int kSure = !GATHER ? 0 : VEC == 4 ? 1 : VEC / 2;
   static __device__ __forceinline__ Raw zeros() {
     if constexpr (GATHER) {
@@ -394,7 +396,7 @@ struct RowRing {
 // with WIDE the block), NV vectors of VEC values per thread, U rows at a time
 // (their loads are in flight together).
 template <class V, int VEC, int NV, int U, bool WIDE, bool GATHER, bool RING, int LANES>
-__global__ void __launch_bounds__(WIDE ? norm_wide_threads(GATHER) : kNormNarrowThreads,
+__global__ void __launch_bounds__(WIDE ? kNormWideThreads : kNormNarrowThreads,
                                   !WIDE && (GATHER ? VEC <= 8 : NV == 1) ? 3 : 1)
 k_norm_forward(const typename V::T *__restrict__ x, int64_t x_stride, int64_t rows, int dim,
                const void *__restrict__ weight, const void *__restrict__ bias, int ptype, float eps,
@@ -552,7 +554,7 @@ k_norm_forward_long(const typename V::T *__restrict__ x, int64_t x_stride, int64
 // [gridDim.x][2][dim] fp32, this block's sums of g h and of g per column
 // (null: no weight gradients wanted).
 template <class V, int VEC, int NV, int U, bool WIDE, bool GATHER, bool RING, int LANES>
-__global__ void __launch_bounds__(WIDE ? norm_wide_threads(GATHER) : kNormNarrowThreads,
+__global__ void __launch_bounds__(WIDE ? kNormWideThreads : kNormNarrowThreads,
                                   !WIDE && (GATHER ? VEC <= 16 : NV <= 2) ? 2 : 1)
 k_norm_backward(const typename V::T *__restrict__ grad, int64_t g_stride, const typename V::T *__restrict__ x,
                 int64_t x_stride, int64_t rows, int dim, const float *__restrict__ mean,
@@ -860,13 +862,12 @@ NormShape norm_shape(int64_t dim, size_t value_size, bool aligned, bool gaps, bo
     while (s.lanes < lanes && s.lanes < 32) s.lanes *= 2;
     return s;
   }
-  s.nv = s.vec ? 16 / per : 8;
+  s.nv = s.vec ? 16 / per : 16;
   s.unroll = norm_wide_rows(per, !s.vec, backward);
   s.wide = s.ring = true;
   const int64_t threads = (n + s.nv - 1) / s.nv;
-  const int most = norm_wide_threads(!s.vec);
-  s.longer = threads > most;
-  s.threads = int(std::min<int64_t>(most, (threads + 31) / 32 * 32));
+  s.longer = threads > kNormWideThreads;
+  s.threads = int(std::min<int64_t>(kNormWideThreads, (threads + 31) / 32 * 32));
   s.lanes = s.threads;
   return s;
 }
@@ -925,7 +926,7 @@ void with_norm_shape(const NormShape &s, F &&f) {
   } else {
     const integral_constant<int, 8> eight{};
     const integral_constant<int, 16> sixteen{};
-    if (s.wide) f(eight, one, one, yes, yes, yes, any);
+    if (s.wide) f(sixteen, one, integral_constant<int, norm_wide_rows(kVec, true, BACKWARD)>{}, yes, yes, yes, any);
     else if (s.nv == 4) f(four, one, two, no, yes, no, any);
     else if (s.nv == 8 && s.lanes == 8) f(eight, one, two, no, yes, no, eight);
     else if (s.nv == 8 && s.lanes == 16) f(eight, one, two, no, yes, no, sixteen);
