@@ -116,6 +116,17 @@ def _affine(x, dim: int, weight, bias):
     return weight, bias, _code(weight.dtype)
 
 
+def _like(x):
+    # empty_like is torch's quickest allocation (1.3 us of host time; new_empty 2.3), but it keeps the order of the axes
+    return torch_mod().empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
+
+
+def _bytes(x, nbytes: int):
+    """A workspace on x's device (torch's allocations are aligned to 512 bytes)."""
+    torch = torch_mod()
+    return torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -137,10 +148,12 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, return_stats: bool 
     eps = float(eps)
     if not math.isfinite(eps) or eps < 0.0:
         raise ValueError("eps must be finite and non-negative")
-    y = x.new_empty(x.shape)
+    y = _like(x)
     mean = rstd = None
     if return_stats:
-        mean, rstd = (x.new_empty(x.shape[:-1], dtype=torch_mod().float32) for _ in range(2))
+        torch = torch_mod()
+        mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        rstd = torch.empty_like(mean)
     N.check(_entry("se_layer_norm")(_code(x.dtype), pcode, x.data_ptr(), rows, dim, stride, _ptr(weight), _ptr(bias), eps,
                                     y.data_ptr(), _ptr(mean), _ptr(rstd), x.device.index, _stream(x)))
     return (y, mean, rstd) if return_stats else y
@@ -164,14 +177,14 @@ def layer_norm_backward(grad, x, mean, rstd, weight=None, with_bias: bool = True
         if not is_torch_tensor(t) or t.dtype != torch_mod().float32 or t.numel() != rows or not t.is_contiguous():
             raise ValueError(f"{what} must be a contiguous float32 tensor with a value per row")
         _same_device(x, t, what)
-    dx = x.new_empty(x.shape)
+    dx = _like(x)
     dw = db = work = None
     nbytes = 0
     if weight is not None:
-        dw = weight.new_empty(weight.shape)
-        db = weight.new_empty(weight.shape) if with_bias else None
+        dw = _like(weight)
+        db = _like(weight) if with_bias else None
         nbytes = _workspace_bytes("se_layer_norm_backward_workspace", rows, dim, x.device.index)
-        work = x.new_empty(nbytes, dtype=torch_mod().uint8)
+        work = _bytes(x, nbytes)
     N.check(_entry("se_layer_norm_backward")(_code(x.dtype), pcode, grad.data_ptr(), gstride, x.data_ptr(), stride, rows,
                                              dim, mean.data_ptr(), rstd.data_ptr(), _ptr(weight), dx.data_ptr(),
                                              _ptr(dw), _ptr(db), _ptr(work), nbytes, x.device.index, _stream(x)))
@@ -197,7 +210,7 @@ def _matrices(x, what: str):
 
 def _muon_work(x, batch: int, m: int, n: int):
     nbytes = _workspace_bytes("se_muon_workspace", _code(x.dtype), batch, m, n)
-    return x.new_empty(nbytes, dtype=torch_mod().uint8), nbytes  # torch's allocations are aligned to 512 bytes
+    return _bytes(x, nbytes), nbytes
 
 
 def orthogonalize(update, steps: int = 5, eps: float = 1e-7):
@@ -208,7 +221,7 @@ def orthogonalize(update, steps: int = 5, eps: float = 1e-7):
     Returns a new tensor of update's shape and dtype."""
     u = _cuda_tensor(update, "update")
     batch, m, n, bs, rs = _matrices(u, "update")
-    out = u.new_empty(u.shape)
+    out = _like(u)
     work, nbytes = _muon_work(u, batch, m, n)
     N.check(_entry("se_orthogonalize")(_code(u.dtype), u.data_ptr(), batch, m, n, bs, rs, int(steps), float(eps),
                                        out.data_ptr(), work.data_ptr(), nbytes, u.device.index, _stream(u)))
