@@ -396,7 +396,7 @@ struct RowRing {
 // with WIDE the block), NV vectors of VEC values per thread, U rows at a time
 // (their loads are in flight together). Vectors are bound by HBM and, in short
 // 16-bit rows, by instructions between load and store (212,992 x 128 fp32 40 us,
-// 5.4 TB/s; 262,144 x 256 bf16 52 us, 5.1; 32,768 x 4,096 bf16 92 us, 5.9);
+// 5.4 TB/s; 262,144 x 256 bf16 49 us, 5.5; 32,768 x 4,096 bf16 92 us, 5.9);
 // single values by their loads, stores and tests (65,536 x 517 fp32 45 us, 6.0;
 // 2^25 bf16 values in rows of 33 58 us, 2.3).
 template <class V, int VEC, int NV, int U, bool WIDE, bool GATHER, bool RING, int LANES>
@@ -913,7 +913,9 @@ NormLaunch norm_launch(K *kernel, const NormShape &s, int64_t rows, int64_t dim,
 // time, a block per row, values one by one, rows through shared memory,
 // threads of a row (0: a variable; as a constant it makes the columns of single
 // values immediate offsets: rows of 65 fp32 values 69 -> 54 us forward, 116 -> 85
-// backward).
+// backward; and saves vectors the tests in the row sums: 262,144 x 256 bf16
+// forward 52 -> 49, 65,536 x 64 fp32 backward 15.1 -> 13.4; in place, 256 bf16
+// values with a gap of 8, backward 52 -> 44, forward 30 -> 33, so not there).
 template <class V, bool BACKWARD, class F>
 void with_norm_shape(const NormShape &s, F &&f) {
   constexpr int kVec = int(16 / sizeof(typename V::T));
@@ -926,17 +928,20 @@ void with_norm_shape(const NormShape &s, F &&f) {
   const integral_constant<int, 4> four{};
   const integral_constant<int, 0> any{};
   const integral_constant<int, 32> all{};
+  const integral_constant<int, 16> sixteen{};
   if (s.vec) {
     const integral_constant<int, norm_wide_rows(kVec, false, BACKWARD)> wide_rows{};
     if (s.wide) f(vec, integral_constant<int, 16 / kVec>{}, wide_rows, yes, no, yes, any);
     else if (s.nv == 4) f(vec, four, one, no, no, yes, all);
     else if (s.nv == 2 && s.ring) f(vec, two, two, no, no, yes, all);
     else if (s.nv == 2) f(vec, two, two, no, no, no, all);
+    else if (s.ring && s.lanes == 32) f(vec, one, four, no, no, yes, all);
+    else if (s.ring && s.lanes == 16) f(vec, one, four, no, no, yes, sixteen);
     else if (s.ring) f(vec, one, four, no, no, yes, any);
+    else if (BACKWARD && s.lanes == 32) f(vec, one, four, no, no, no, all);
     else f(vec, one, four, no, no, no, any);
   } else {
     const integral_constant<int, 8> eight{};
-    const integral_constant<int, 16> sixteen{};
     if (s.wide) f(sixteen, one, integral_constant<int, norm_wide_rows(kVec, true, BACKWARD)>{}, yes, yes, yes, any);
     else if (s.nv == 4) f(four, one, two, no, yes, no, any);
     else if (s.nv == 8 && s.lanes == 8) f(eight, one, two, no, yes, no, eight);
