@@ -287,9 +287,8 @@ struct RowSum {
 // A bulk copy moves whole 16-byte units. Where rows do not start and end at
 // such (ALIGNED false), the units that hold a row's first and last bytes are
 // copied whole and the row is found inside; those of the matrix's first and
-// last rows reach past it, so the tiles with these rows (or, where a row is
-// shorter than a unit, within a unit of them) are not copied: the threads read
-// them in place.
+// last row reach past it (no row here is shorter than a unit), so the tiles
+// with these two rows are not copied: the threads read them in place.
 constexpr int kNormStages = 8;
 template <class T, int N, bool ALIGNED>
 struct RowRing {
@@ -311,8 +310,7 @@ struct RowRing {
     return buf + size_t(stage * N + n) * rows * pitch(dim);
   }
   __device__ __forceinline__ bool covers(int64_t base) const {
-    const int edge = size_t(dim) * sizeof(T) >= 16 ? 1 : 8;  // rows of at least 16 bytes together
-    return ALIGNED || (base >= edge && base + rows + edge <= rows_total);
+    return ALIGNED || (base > 0 && base + rows < rows_total);
   }
   // Row r of the tile in turn, which `covers` it.
   __device__ __forceinline__ const T *row(int n, int r, int64_t base) const {
