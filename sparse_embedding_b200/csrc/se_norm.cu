@@ -366,7 +366,11 @@ struct RowRing {
     __syncthreads();
   }
   __device__ __forceinline__ bool ready() const { return wait_or_give_up(&bars[at], parity, given_up); }
-  // The tile has been read by all threads (a barrier lies between): refill its buffer.
+  // The tile has been read by all threads: refill its buffer. Each thread has
+  // passed fence_proxy_async_smem after its reads and then the block's barrier. The
+  // barrier alone does not hold a copy back: a read that waits in the memory
+  // pipe, behind stores that HBM holds up, comes after the copy (a warp's part of
+  // one row in about 400,000 was a later row's, 32,768 x 4,096 bf16 backward).
   __device__ __forceinline__ void next(int64_t base) {
     if (threadIdx.x == 0) fill(at, base + stages * step);
     if (++at == stages) {
@@ -445,6 +449,7 @@ k_norm_forward(const typename V::T *__restrict__ x, int64_t x_stride, int64_t ro
       }
     }
     if constexpr (RING) {
+      fence_proxy_async_smem();
       if (__syncthreads_or(!ok)) {
         ring.drain(base, status);
         return;
@@ -635,6 +640,7 @@ k_norm_backward(const typename V::T *__restrict__ grad, int64_t g_stride, const 
       }
     }
     if constexpr (RING) {
+      fence_proxy_async_smem();
       if (__syncthreads_or(!ok)) {
         ring.drain(base, status);
         return;

@@ -41,3 +41,49 @@ def test_backward_of_rows_far_from_zero(dim, dt, offset):
     DX = q * (wg - wg.mean(1, keepdim=True) - h * (wg * h).mean(1, keepdim=True))
     size = wg.abs().amax(1, keepdim=True) + h.abs().amax(1, keepdim=True) * (wg * h).abs().mean(1, keepdim=True)
     within(dx, DX, 100 * U * q * size + half(dt) * (DX.abs() + torch.finfo(dt).tiny), "dx")
+
+
+# Rows enough that every block fills each buffer of its ring several times: vectors with one, two and four loads a
+# thread, single values with 16 and 32, a block per row in both; without gaps, with a gap, from an odd address.
+RING = [(200_000, 128, torch.float32, 0, 0), (262_144, 256, torch.bfloat16, 0, 0), (100_000, 256, torch.float32, 0, 0),
+        (100_000, 512, torch.bfloat16, 0, 0), (100_000, 512, torch.float32, 4, 0), (60_000, 1000, torch.float16, 8, 0),
+        (60_000, 301, torch.float32, 0, 1), (120_000, 301, torch.bfloat16, 2, 3), (60_000, 517, torch.float32, 0, 0),
+        (60_000, 1001, torch.bfloat16, 0, 1), (60_000, 1037, torch.float32, 3, 1), (90_000, 1037, torch.bfloat16, 0, 0),
+        (60_000, 1032, torch.float32, 0, 0), (65_536, 2048, torch.bfloat16, 0, 0), (33_000, 4096, torch.bfloat16, 0, 0),
+        (33_000, 4096, torch.float32, 0, 0), (33_000, 4104, torch.float16, 8, 0), (20_000, 8192, torch.bfloat16, 0, 0)]
+
+
+def laid_out(values, pad, offset, dt):
+    rows, dim = values.shape
+    flat = torch.zeros(rows * (dim + pad) + offset, dtype=dt, device="cuda")
+    t = flat[offset:].view(rows, dim + pad)[:, :dim]
+    t.copy_(values)
+    return t
+
+
+@pytest.mark.parametrize("rows, dim, dt, pad, offset", RING)
+def test_many_tiles_a_block(rows, dim, dt, pad, offset):
+    """x and grad are whole numbers from -3 to 3 and mean = 0, rstd = 1 are given, so that h = x and every sum over
+    rows stays below 2^24: dweight and dbias are exact, whatever the order of the sums. So are a row's sums; with
+    weight 1 dx is g - sum g / D - x sum(g x) / D: two quotients, each rounded twice (1 / D and the product), and two fused
+    adds: 4 u (|g| + |mean g| + |x mean(g x)|) before the result's own rounding. y: means of whole numbers, tolerance as
+    derived for the other tests (|x| <= 3). Calls repeat bit by bit."""
+    gen = torch.Generator(device="cuda").manual_seed(rows + dim)
+    ints = lambda: torch.randint(-3, 4, (rows, dim), generator=gen, device="cuda", dtype=torch.int8)  # noqa: E731
+    x, g = laid_out(ints(), pad, offset, dt), laid_out(ints(), pad, offset, dt)
+    w, zero, one = torch.ones(dim, device="cuda"), torch.zeros(rows, device="cuda"), torch.ones(rows, device="cuda")
+    first = se.layer_norm_backward(g, x, zero, one, w)
+    X, G = x.double(), g.double()
+    assert torch.equal(first[1].double(), (G * X).sum(0)) and torch.equal(first[2].double(), G.sum(0))
+    c0, c1 = G.mean(1, keepdim=True), X * (G * X).mean(1, keepdim=True)
+    DX = G - c0 - c1
+    within(first[0], DX, 4 * U * (G.abs() + c0.abs() + c1.abs()) + half(dt) * DX.abs(), "dx")
+    y = se.layer_norm(x, w)
+    m = X.mean(1, keepdim=True)
+    r = 1 / ((X - m).square().mean(1, keepdim=True) + 1e-5).sqrt()
+    Y = (X - m) * r
+    within(y, Y, U * 100 * 3 * r + half(dt) * Y.abs(), "y")
+    del X, G, DX, Y, c1
+    for _ in range(10):
+        assert all(torch.equal(p, q) for p, q in zip(se.layer_norm_backward(g, x, zero, one, w), first))
+        assert torch.equal(se.layer_norm(x, w), y)
