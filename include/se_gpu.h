@@ -321,12 +321,17 @@ int se_layer_norm_backward_workspace(size_t rows, int64_t dim, int32_t device, s
 int se_orthogonalize(int32_t dtype, const void *update, size_t batch, int64_t m, int64_t n, int64_t batch_stride,
                      int64_t row_stride, int32_t steps, float eps, void *out, void *workspace,
                      size_t workspace_bytes, int32_t device, void *stream);
+/* Clocks of a multiprocessor after which a wait inside the dense operators'
+ * kernels gives up, for calls made from now on (0: the default, 8e9, which is
+ * also the most). A healthy wait takes microseconds. */
+int se_set_wait_limit(uint64_t clocks);
 /* One Muon step of `batch` weight matrices (m x n, weight_dtype), in place:
  *   momentum = beta momentum + grad                        (fp32)
  *   U = grad + beta momentum if nesterov, else momentum
  *   weight = (1 - lr weight_decay) weight - lr scale orthogonalize(U)
  * grad_dtype is weight_dtype or SE_FLOAT32. Weight, gradient and momentum
- * overlap nowhere. */
+ * overlap nowhere. Where a wait inside the kernels gives up the weights stay as
+ * they were (the momentum has taken the gradient). */
 int se_muon_step(int32_t weight_dtype, int32_t grad_dtype, void *weight, int64_t weight_batch_stride,
                  int64_t weight_row_stride, const void *grad, int64_t grad_batch_stride, int64_t grad_row_stride,
                  float *momentum, int64_t momentum_batch_stride, int64_t momentum_row_stride, size_t batch,

@@ -2,6 +2,7 @@
 // update): argument checks and dispatch on the value type.
 #pragma once
 
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 #include <stdexcept>
@@ -71,6 +72,14 @@ inline int resident_blocks(void (*kernel)(KArgs...), int device, int threads, si
   int n = 0;
   cuda_check(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem), "occupancy");
   return known[key] = n < 1 ? 1 : n;
+}
+
+// Clocks after which a wait inside the dense operators' kernels gives up
+// (se_set_wait_limit).
+constexpr long long kWaitClocks = 8000000000ll;
+inline std::atomic<long long> &wait_limit() {
+  static std::atomic<long long> clocks{kWaitClocks};
+  return clocks;
 }
 
 // A word in host memory that a kernel sets when one of its waits for a copy gave

@@ -351,7 +351,9 @@ struct NsArgs {
   float *partial;          // gram.parts > 1: partial sums of its blocks, [block][part][32][32]
   uint32_t *arrived;       // and how many parts of a block are there
   uint32_t *barrier;       // blocks that finished a product
+  uint32_t *failed;        // set when a wait gave up: X is not the result
   FinishArgs fin;
+  long long limit;
   uint32_t *status;
 };
 
@@ -737,7 +739,7 @@ __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int s
         col += int(rank) * (BN / CG);
         for (int k = k_from(part), last = k_from(part + 1); k < last; ++k) {
           const uint32_t st = at.stage.at;
-          if (!wait_or_give_up(&sh.empty[st], at.stage.parity ^ 1u, &sh.given_up)) {
+          if (!wait_or_give_up<true>(&sh.empty[st], at.stage.parity ^ 1u, &sh.given_up, g.limit)) {
             go = false;
             break;
           }
@@ -784,7 +786,7 @@ __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int s
         const int part = parts > 1 ? t % parts : 0, last = k_from(part + 1);
         for (int k = k_from(part); go && k < last; at.sum.advance()) {
           const uint32_t acc = tmem + at.sum.at * L::kColumns;
-          if (!wait_or_give_up(&sh.acc_empty[at.sum.at], at.sum.parity ^ 1u, &sh.given_up)) {
+          if (!wait_or_give_up<true>(&sh.acc_empty[at.sum.at], at.sum.parity ^ 1u, &sh.given_up, g.limit)) {
             go = false;
             break;
           }
@@ -793,7 +795,7 @@ __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int s
           bool add = false;
           for (; k < end; ++k) {
             const uint32_t st = at.stage.at;
-            if (!wait_or_give_up(&sh.full[st], at.stage.parity, &sh.given_up)) {
+            if (!wait_or_give_up<true>(&sh.full[st], at.stage.parity, &sh.given_up, g.limit)) {
               go = false;
               break;
             }
@@ -822,7 +824,7 @@ __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int s
     const uint32_t tmem = sh.tmem + (uint32_t(quad * 32) << 16) + uint32_t(side * kBlocks * 32);
     bool go = true;
     auto take = [&] {  // the accumulator in turn is full; false: gave up
-      go = __all_sync(0xffffffffu, wait_or_give_up(&sh.acc_full[at.sum.at], at.sum.parity, &sh.given_up));
+      go = __all_sync(0xffffffffu, wait_or_give_up<true>(&sh.acc_full[at.sum.at], at.sum.parity, &sh.given_up, g.limit));
       tmem_fence_after();
       return go;
     };
@@ -930,7 +932,7 @@ __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int s
 
 // All blocks have finished the product (their stores are visible to every
 // block's loads); false: a wait gave up somewhere.
-__device__ __forceinline__ bool grid_wait(uint32_t *barrier, uint32_t target, Shared &sh) {
+__device__ __forceinline__ bool grid_wait(uint32_t *barrier, uint32_t target, Shared &sh, long long limit) {
   __syncthreads();
   if (gridDim.x > 1) {
     if (threadIdx.x == 0) {
@@ -940,7 +942,7 @@ __device__ __forceinline__ bool grid_wait(uint32_t *barrier, uint32_t target, Sh
         uint32_t seen;
         asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(barrier) : "memory");
         if (seen >= target) break;
-        if (sh.given_up || n >= kWaitTries || clock64() - start > kWaitClocks) {
+        if (sh.given_up || n >= kWaitTries || clock64() - start > limit) {
           sh.given_up = 1u;
           break;
         }
@@ -989,16 +991,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_newton_schulz(const __grid_cons
   uint32_t target = 0;
   for (int step = 0; step < g.steps; ++step) {
     run_product<kGram, CG, BN, OUT>(g, g.gram, step, sh, smem, rank, at);
-    if (!grid_wait(g.barrier, target += gridDim.x, sh)) break;
+    if (!grid_wait(g.barrier, target += gridDim.x, sh, g.limit)) break;
     run_product<kSquare, CG, BN, OUT>(g, g.square, step, sh, smem, rank, at);
-    if (!grid_wait(g.barrier, target += gridDim.x, sh)) break;
+    if (!grid_wait(g.barrier, target += gridDim.x, sh, g.limit)) break;
     if (step + 1 == g.steps && !g.fin.update) {
       run_product<kFinish, CG, BN, OUT>(g, g.apply, step, sh, smem, rank, at);
       break;
     }
     run_product<kApply, CG, BN, OUT>(g, g.apply, step, sh, smem, rank, at);
     if (step + 1 == g.steps) break;
-    if (!grid_wait(g.barrier, target += gridDim.x, sh)) break;
+    if (!grid_wait(g.barrier, target += gridDim.x, sh, g.limit)) break;
   }
 
   // No arrival or copy is outstanding when the CTA ends: the stages' last uses
@@ -1007,16 +1009,25 @@ __global__ void __launch_bounds__(kThreads, 1) k_newton_schulz(const __grid_cons
   __syncthreads();
   const bool failed = sh.given_up != 0u;
   const uint32_t issued = __reduce_max_sync(0xffffffffu, at.loaded);
+  const long long end = clock64() + kDrainClocks;
   if (warp == 0 && (!failed || rank == 0)) {
     for (uint32_t i = issued > L::kStages ? issued - L::kStages : 0; i < issued; ++i)
-      wait_for(failed ? &sh.full[i % L::kStages] : &sh.empty[i % L::kStages], (i / L::kStages) & 1u, nullptr);
+      wait_until(failed ? &sh.full[i % L::kStages] : &sh.empty[i % L::kStages], (i / L::kStages) & 1u, end);
   }
   if (failed) {
-    if (threadIdx.x == 32 && rank == 0) {
-      mma_commit<CG>(&sh.drained);
-      wait_for(&sh.drained, 0u, nullptr);
+    // A pair's barrier counts the loads of both CTAs and completes no more where
+    // they loaded different numbers of stages: they wait a hundred times a load's latency.
+    while (CG == 2 && end - clock64() > kDrainClocks - 200000) {
+    }
+    if (warp == 1 && rank == 0) {
+      if (elect_one()) {  // the thread that issued the instructions
+        mma_commit<CG>(&sh.drained);
+        wait_until(&sh.drained, 0u, end);
+      }
+      __syncwarp();
     }
     if (threadIdx.x == 0) {
+      *reinterpret_cast<volatile uint32_t *>(g.failed) = 1u;
       *reinterpret_cast<volatile uint32_t *>(g.status) = 1u;
       __threadfence_system();
     }
@@ -1033,11 +1044,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_newton_schulz(const __grid_cons
 // loaded (8 x 1024 x 2048 bf16: that product took 152,000 to 203,000 clocks for
 // 83,000 without weights; this kernel takes a quarter of the difference). Along
 // the rows in vectors, or through shared memory in tiles of 64 x 64, as
-// k_muon_scale. Bound by HBM (8 x 1024 x 2048 bf16 29 us, 4.7 TB/s).
+// k_muon_scale. Bound by HBM (8 x 1024 x 2048 bf16 29 us, 4.7 TB/s). Where the
+// products gave up, the weights stay as they were.
 template <class W>
 __global__ void __launch_bounds__(256)
 k_muon_weights(const __half *__restrict__ hi, const __half *__restrict__ lo, int64_t ld, int64_t batch_stride, int64_t m,
-               int64_t n, int vec, FinishArgs f) {
+               int64_t n, int vec, FinishArgs f, const uint32_t *__restrict__ failed) {
   __shared__ float tile[64][65];
   using T = typename W::T;
   const int64_t z = blockIdx.z;
@@ -1046,6 +1058,7 @@ k_muon_weights(const __half *__restrict__ hi, const __half *__restrict__ lo, int
   lo += z * batch_stride;
   const float rate = f.rate * (1.0f / kScale);
   pdl_wait();
+  if (__ldcg(failed) != 0u) return;
   auto open = [&](int64_t at, float (&o)[8]) {  // eight values of O, not yet divided by S
     const uint4 h = *reinterpret_cast<const uint4 *>(hi + at), l = *reinterpret_cast<const uint4 *>(lo + at);
     const __half2 *hh = reinterpret_cast<const __half2 *>(&h), *ll = reinterpret_cast<const __half2 *>(&l);
@@ -1160,7 +1173,7 @@ __device__ __forceinline__ void open_eight(const uint4 &v, float (&f)[8]) {
 template <class V, class W, bool MOM, int SIDES>
 __global__ void __launch_bounds__(128 * SIDES)
 k_newton_schulz_small(UpdateArgs a, int s, int w, int transposed, int steps, float eps, FinishArgs fin,
-                      uint32_t tmem_columns, uint32_t *status) {
+                      uint32_t tmem_columns, long long limit, uint32_t *status) {
   constexpr bool SPLIT = !std::is_same_v<W, BF16>;  // as split_products says
   constexpr int kThreads = 128 * SIDES, kWarps = 4 * SIDES;
   constexpr int kX = SIDES == 2 ? 4 : 1, kA = 4 / SIDES;  // blocks of X and of A that a thread owns
@@ -1302,7 +1315,7 @@ k_newton_schulz_small(UpdateArgs a, int s, int w, int transposed, int steps, flo
       mma_commit<1>(&done);
     }
     __syncwarp();
-    const bool ok = wait_or_give_up(&done, parity, &given_up);
+    const bool ok = wait_or_give_up<false>(&done, parity, &given_up, limit);
     parity ^= 1u;
     const bool all = __syncthreads_and(ok) != 0;
     tmem_fence_after();
@@ -1440,7 +1453,7 @@ k_newton_schulz_small(UpdateArgs a, int s, int w, int transposed, int steps, flo
   __syncthreads();
   if (!ok) {
     if (tid == 0) {
-      wait_for(&done, parity ^ 1u, nullptr);
+      wait_until(&done, parity ^ 1u, clock64() + kDrainClocks);
       *reinterpret_cast<volatile uint32_t *>(status) = 1u;
       __threadfence_system();
     }
@@ -1568,7 +1581,7 @@ struct Space {
   double *norms;
   Pair x[2], a, b;
   float *diag_a, *diag_b, *partial;
-  uint32_t *counters;  // the barrier, then one per block of X X^T
+  uint32_t *counters;  // the barrier, the failure word, then one per block of X X^T
   int64_t ncounters;
   size_t bytes;
 };
@@ -1600,7 +1613,7 @@ Space muon_space(void *base, int64_t batch, int64_t s, int64_t w, bool split) {
   sp.diag_b = reinterpret_cast<float *>(take(size_t(batch) * lda * sizeof(float)));
   const int64_t values = p.parts > 1 ? tile_count(true, s, s, 128 * p.cg, p.bn) * batch * 128 * p.cg * p.bn : 0;
   sp.partial = reinterpret_cast<float *>(take(size_t(values) * p.parts * sizeof(float)));
-  sp.ncounters = 1 + values / 1024;  // (at least one per warp of a tile)
+  sp.ncounters = 2 + values / 1024;  // (at least one per warp of a tile)
   sp.counters = reinterpret_cast<uint32_t *>(take(size_t(sp.ncounters) * sizeof(uint32_t)));
   sp.bytes = at;
   return sp;
@@ -1690,6 +1703,7 @@ void orthogonalise(UpdateArgs u, int grad_type, int64_t batch, int steps, float 
   g.apply = cut(false, w, s, 1);
   const int sms = sm_count(device);
   g.status = wait_status(device);
+  g.limit = wait_limit();
   fin.transposed = transposed;
   const size_t ob = value_bytes(fin.type);
   fin.vec = u.n % 4 == 0 && reinterpret_cast<uintptr_t>(fin.out) % (4 * ob) == 0 && fin.row % 4 == 0 &&
@@ -1703,7 +1717,7 @@ void orthogonalise(UpdateArgs u, int grad_type, int64_t batch, int steps, float 
         auto *kernel = k_newton_schulz_small<decltype(grad), decltype(out), decltype(mom)::value, decltype(sides)::value>;
         allow_dynamic_smem(kernel, smem);
         kernel<<<unsigned(batch), 128 * decltype(sides)::value, smem, st>>>(u, int(s), int(w), int(transposed), steps, eps,
-                                                                            fin, columns, g.status);
+                                                                            fin, columns, g.limit, g.status);
       };
       if (w > 128) start(std::integral_constant<int, 2>{});
       else start(std::integral_constant<int, 4>{});
@@ -1755,7 +1769,8 @@ void orthogonalise(UpdateArgs u, int grad_type, int64_t batch, int steps, float 
   g.diag_ld = sp.a.ld;
   g.partial = sp.partial;
   g.barrier = sp.counters;
-  g.arrived = sp.counters + 1;
+  g.failed = sp.counters + 1;
+  g.arrived = sp.counters + 2;
   g.fin = fin;
   const int64_t units = std::max<int64_t>(int64_t(g.gram.tiles) * plan.parts, g.apply.tiles) * batch;
   const int form = plan.cg * 1000 + plan.bn;
@@ -1778,7 +1793,8 @@ void orthogonalise(UpdateArgs u, int grad_type, int64_t batch, int steps, float 
     const int vec = u.n % 8 == 0 && aligned16(fin.out) && fin.row * ob % 16 == 0 && (batch == 1 || fin.batch * ob % 16 == 0);
     const int64_t blocks = vec && !transposed ? (u.m * ((u.n + 7) / 8) + 255) / 256 : tiles64;
     launch_after(k_muon_weights<decltype(out)>, dim3(unsigned(std::min<int64_t>(blocks, 8 * sms)), 1, unsigned(batch)), st,
-                 static_cast<const __half *>(o.hi), static_cast<const __half *>(o.lo), o.ld, o.batch, u.m, u.n, vec, fin);
+                 static_cast<const __half *>(o.hi), static_cast<const __half *>(o.lo), o.ld, o.batch, u.m, u.n, vec, fin,
+                 static_cast<const uint32_t *>(g.failed));
   });
   launched("k_muon_weights");
 }

@@ -278,6 +278,20 @@ struct RowSum {
   }
 };
 
+// Waits for `count` copies from stage `at` on, and reports that a wait gave up.
+static __device__ __noinline__ void let_land(uint64_t *bars, int at, uint32_t parity, int stages, int count, uint32_t *status) {
+  const long long end = clock64() + kDrainClocks;
+  for (int i = 0; i < count; ++i) {
+    wait_until(&bars[at], parity, end);
+    if (++at == stages) {
+      at = 0;
+      parity ^= 1u;
+    }
+  }
+  *reinterpret_cast<volatile uint32_t *>(status) = 1u;
+  __threadfence_system();
+}
+
 // Tiles of rows on their way through shared memory, by bulk copies (one per
 // tile where the rows have no gaps, else one per row) into a ring of buffers of
 // `rows` rows for each of N arrays. The loads of a block are so several tiles
@@ -299,6 +313,7 @@ struct RowRing {
   uint8_t *buf;
   uint64_t *bars;
   volatile uint32_t *given_up;
+  long long limit;
   int at = 0;
   uint32_t parity = 0;
 
@@ -365,7 +380,7 @@ struct RowRing {
     }
     __syncthreads();
   }
-  __device__ __forceinline__ bool ready() const { return wait_or_give_up(&bars[at], parity, given_up); }
+  __device__ __forceinline__ bool ready() const { return wait_or_give_up<N == 1>(&bars[at], parity, given_up, limit); }
   // The tile has been read by all threads: refill its buffer. Each thread has
   // passed fence_proxy_async_smem after its reads and then the block's barrier. The
   // barrier alone does not hold a copy back: a read that waits in the memory
@@ -379,17 +394,10 @@ struct RowRing {
     }
   }
   // After a wait that gave up: the copies still in flight.
-  __device__ __forceinline__ void drain(int64_t base, uint32_t *status) {
+  __device__ __forceinline__ void drain(int64_t base, uint32_t *status) const {
     if (threadIdx.x == 0) {
-      for (int i = 0; i < stages; ++i) {
-        if (base + i * step < rows_total) wait_for(&bars[at], parity, nullptr);
-        if (++at == stages) {
-          at = 0;
-          parity ^= 1u;
-        }
-      }
-      *reinterpret_cast<volatile uint32_t *>(status) = 1u;
-      __threadfence_system();
+      const int64_t tiles = (rows_total - base + step - 1) / step;
+      let_land(bars, at, parity, stages, int(tiles < stages ? tiles : stages), status);
     }
   }
 };
@@ -407,7 +415,7 @@ __global__ void __launch_bounds__(WIDE ? kNormWideThreads : kNormNarrowThreads,
 k_norm_forward(const typename V::T *__restrict__ x, int64_t x_stride, int64_t rows, int dim,
                const void *__restrict__ weight, const void *__restrict__ bias, int ptype, float eps,
                typename V::T *__restrict__ y, float *__restrict__ mean_out, float *__restrict__ rstd_out, int lanes_of_row,
-               int stages, uint32_t *status) {
+               int stages, uint32_t *status, long long limit) {
   using P = Pack<V, VEC, GATHER>;
   using T = typename V::T;
   __shared__ float red[2][32][4];
@@ -431,7 +439,7 @@ k_norm_forward(const typename V::T *__restrict__ x, int64_t x_stride, int64_t ro
   RowSum<U, WIDE> sum{lanes, red};
   const float inv = 1.0f / float(dim);
   const int64_t first = int64_t(blockIdx.x) * groups * U, step = int64_t(gridDim.x) * groups * U;
-  RowRing<T, 1, !GATHER> ring{{x}, {x_stride}, rows, step, groups * U, dim, stages, raw_smem, bars, &given_up};
+  RowRing<T, 1, !GATHER> ring{{x}, {x_stride}, rows, step, groups * U, dim, stages, raw_smem, bars, &given_up, limit};
   if (RING) ring.start(first);
   for (int64_t base = first; base < rows; base += step) {
     typename P::Raw raw[U][NV];
@@ -572,7 +580,7 @@ k_norm_backward(const typename V::T *__restrict__ grad, int64_t g_stride, const 
                 int64_t x_stride, int64_t rows, int dim, const float *__restrict__ mean,
                 const float *__restrict__ rstd, const void *__restrict__ weight, int ptype,
                 typename V::T *__restrict__ dx, float *__restrict__ partial, int lanes_of_row, int stages,
-                uint32_t *status) {
+                long long limit, uint32_t *status) {
   using P = Pack<V, VEC, GATHER>;
   using T = typename V::T;
   __shared__ float red[2][32][4];
@@ -598,7 +606,7 @@ k_norm_backward(const typename V::T *__restrict__ grad, int64_t g_stride, const 
   const float inv = 1.0f / float(dim);
   const int64_t first = int64_t(blockIdx.x) * groups * U, step = int64_t(gridDim.x) * groups * U;
   RowRing<T, 2, !GATHER> ring{{x, grad}, {x_stride, g_stride}, rows, step, groups * U, dim,
-                              stages,    raw_smem,             bars, &given_up};
+                              stages,    raw_smem,             bars, &given_up, limit};
   if (RING) ring.start(first);
   float next_m[U], next_r[U];  // a tile's statistics are asked for a tile ahead
   auto ask = [&](int64_t at) {
@@ -975,6 +983,13 @@ void check_norm(int32_t value_dtype, int32_t param_dtype, size_t rows, int64_t d
 
 using namespace se_gpu;
 
+extern "C" int se_set_wait_limit(uint64_t clocks) {
+  return guarded([&] {
+    if (clocks > uint64_t(kWaitClocks)) throw std::invalid_argument("clocks must be at most 8e9");
+    wait_limit() = clocks == 0 ? kWaitClocks : (long long)(clocks);
+  });
+}
+
 extern "C" int se_layer_norm(int32_t value_dtype, int32_t param_dtype, const void *x, size_t rows, int64_t dim,
                              int64_t x_stride, const void *weight, const void *bias, float eps, void *y,
                              float *mean_out, float *rstd_out, int32_t device, void *stream) {
@@ -1014,7 +1029,7 @@ extern "C" int se_layer_norm(int32_t value_dtype, int32_t param_dtype, const voi
                                       decltype(lanes)::value>;
         const NormLaunch l = norm_launch(kernel, s, int64_t(rows), dim, vb, 1, device, 0);
         kernel<<<l.blocks, s.threads, l.smem, st>>>(xp, x_stride, int64_t(rows), int(dim), weight, bias, param_dtype, eps,
-                                                    yp, mean_out, rstd_out, s.lanes, l.stages, status);
+                                                    yp, mean_out, rstd_out, s.lanes, l.stages, status, wait_limit().load());
       });
       launched("k_norm_forward");
     });
@@ -1101,7 +1116,7 @@ extern "C" int se_layer_norm_backward(int32_t value_dtype, int32_t param_dtype, 
           const NormLaunch l = norm_launch(kernel, s, int64_t(rows), dim, vb, 2, device, cols);
           blocks = l.blocks;
           kernel<<<blocks, s.threads, l.smem, st>>>(gp, grad_stride, xp, x_stride, int64_t(rows), int(dim), mean, rstd,
-                                                    weight, param_dtype, dxp, partial, s.lanes, l.stages, status);
+                                                    weight, param_dtype, dxp, partial, s.lanes, l.stages, wait_limit().load(), status);
         });
         launched("k_norm_backward");
       });

@@ -11,21 +11,55 @@
 
 namespace se_gpu {
 
-// A wait gives up after this many clocks (seconds), or this many tries (each
-// may suspend the thread for a while). In a healthy launch a wait takes
+// A wait gives up after `limit` clocks (kWaitClocks unless se_set_wait_limit
+// changed it: seconds), or this many tries. In a healthy launch a wait takes
 // microseconds. (Clocks, since a read of the nanosecond timer is slow enough
-// to show in every wait.)
-constexpr long long kWaitClocks = 8000000000ll;
+// to show in every wait.) The limit is looked at after a first look that failed:
+// before it, its load would be in every wait (4096 x 1024 fp32 370 -> 383 us).
 constexpr uint32_t kWaitTries = 1u << 30;
+// Limits below this are kept by looking: a try suspends the thread for a time of its own choice.
+constexpr long long kBriefClocks = 10000000ll;
+// What a launch that gave up allows its copies and matrix instructions in flight, in all.
+constexpr long long kDrainClocks = 2000000000ll;
 
-__device__ __forceinline__ bool wait_for(uint64_t *bar, uint32_t parity, const volatile uint32_t *given_up) {
-  if (mbar_try_wait(bar, parity)) return true;
+__device__ __forceinline__ bool mbar_test_wait(uint64_t *bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+               " selp.u32 %0, 1, 0, p;\n}"
+               : "=r"(done)
+               : "r"(smem_u32(bar)), "r"(parity)
+               : "memory");
+  return done != 0u;
+}
+// Waits for a barrier's phase; false when the limit ran out or another role
+// of the CTA gave up (*given_up). The caller then leaves its loop. CALL: all but
+// the first look as a call of a function, which leaves the caller's loop short
+// (1000 x 517 fp32 159.7 us in place, 156.5 by call; but the matrices on chip 25.1
+// and 26.6 at 128 x 64, and normalisation backward 173 and 175 at 32,768 x 4,096).
+__device__ __forceinline__ bool wait_on(uint64_t *bar, uint32_t parity, volatile uint32_t *given_up, long long limit) {
+  const bool brief = limit < kBriefClocks;
   const long long start = clock64();
   for (uint32_t n = 0; n < kWaitTries; ++n) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((given_up != nullptr && *given_up) || clock64() - start > kWaitClocks) return false;
+    if (brief ? mbar_test_wait(bar, parity) : mbar_try_wait(bar, parity)) return true;
+    if (*given_up || clock64() - start > limit) break;
   }
+  *given_up = 1u;
   return false;
+}
+static __device__ __noinline__ bool wait_by_call(uint64_t *bar, uint32_t parity, volatile uint32_t *given_up, long long limit) {
+  return wait_on(bar, parity, given_up, limit);
+}
+template <bool CALL>
+__device__ __forceinline__ bool wait_or_give_up(uint64_t *bar, uint32_t parity, volatile uint32_t *given_up,
+                                                long long limit) {
+  if (mbar_test_wait(bar, parity)) return true;
+  if constexpr (CALL) return wait_by_call(bar, parity, given_up, limit);
+  else return wait_on(bar, parity, given_up, limit);
+}
+// A wait for what is in flight when a launch has given up: until clock `end`.
+__device__ __forceinline__ void wait_until(uint64_t *bar, uint32_t parity, long long end) {
+  while (!mbar_try_wait(bar, parity) && clock64() < end) {
+  }
 }
 // One lane of the converged warp, the same one every time.
 __device__ __forceinline__ bool elect_one() {
@@ -51,14 +85,6 @@ __device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {
 // tcgen05 fences; a wider release would wait for the thread's stores.)
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
-}
-
-// Waits for a barrier's phase; false when the tries ran out or another role
-// of the CTA gave up (*given_up). The caller then leaves its loop.
-__device__ __forceinline__ bool wait_or_give_up(uint64_t *bar, uint32_t parity, volatile uint32_t *given_up) {
-  if (wait_for(bar, parity, given_up)) return true;
-  *given_up = 1u;
-  return false;
 }
 
 __device__ __forceinline__ void prefetch_map(const CUtensorMap *map) {

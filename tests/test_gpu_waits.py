@@ -72,8 +72,8 @@ def test_normalisations_that_gave_up(dim, dt):
             call()
         except RuntimeError as e:
             assert "gave up waiting" in str(e)
-        else:  # odd rows take longer to work on than to copy: no wait need run out
-            assert dim not in (128, 4096) and all(torch.equal(p, q) for p, q in zip(got, right))
+        else:  # rows that take longer to work on than to copy: no wait need run out
+            assert dim != 128 and all(torch.equal(p, q) for p, q in zip(got, right))
     assert torch.equal(se.layer_norm(x, w), y)
     assert all(torch.equal(p, q) for p, q in zip(se.layer_norm_backward(g, x, mean, rstd, w), want))
 
