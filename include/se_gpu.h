@@ -281,7 +281,9 @@ int se_unique(int32_t key_dtype, const void *keys, size_t num_keys, void *unique
  * the dense part of a model outside it). Device pointers only, on `device`
  * (others are refused); asynchronous on `stream`; nothing is allocated and the
  * host waits for nothing, so the calls can be captured into CUDA graphs. A
- * workspace belongs to the caller: one per call in flight.
+ * workspace belongs to the caller: one per call in flight. Waits inside the
+ * kernels have a limit: a call whose kernels gave up has no valid results, and
+ * the next call on its stream reports that (SE_ERR_RUNTIME) instead of running.
  */
 
 /* Layer normalisation of `rows` rows of dim values (value_dtype; row i starts
@@ -316,8 +318,7 @@ int se_layer_norm_backward_workspace(size_t rows, int64_t dim, int32_t device, s
  * apart; out is batch x m x n without gaps, of the same dtype, and overlaps
  * no input. Products of f16 pairs with fp32 sums: a bf16 result is within its
  * own rounding of the exact one, fp32 and f16 results use three products for
- * one. `workspace`: se_muon_workspace bytes, 256-byte aligned. A wait inside
- * the kernels that gives up is reported by the next call (SE_ERR_RUNTIME). */
+ * one. `workspace`: se_muon_workspace bytes, 256-byte aligned. */
 int se_orthogonalize(int32_t dtype, const void *update, size_t batch, int64_t m, int64_t n, int64_t batch_stride,
                      int64_t row_stride, int32_t steps, float eps, void *out, void *workspace,
                      size_t workspace_bytes, int32_t device, void *stream);
@@ -325,6 +326,11 @@ int se_orthogonalize(int32_t dtype, const void *update, size_t batch, int64_t m,
  * kernels gives up, for calls made from now on (0: the default, 8e9, which is
  * also the most). A healthy wait takes microseconds. */
 int se_set_wait_limit(uint64_t clocks);
+/* SE_ERR_RUNTIME where a wait inside a dense operator's kernel on `device` has
+ * given up, on any stream, and the report was not taken yet (each is taken
+ * once: here, or by the next call on its stream). Does not wait for the GPU; a
+ * replayed graph reports to the stream that it was captured on. */
+int se_check_waits(int32_t device);
 /* One Muon step of `batch` weight matrices (m x n, weight_dtype), in place:
  *   momentum = beta momentum + grad                        (fp32)
  *   U = grad + beta momentum if nesterov, else momentum

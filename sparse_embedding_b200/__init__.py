@@ -29,7 +29,7 @@ from .partitioner import (
     register_partitioner,
 )
 from .unique import async_unique, unique
-from .dense import layer_norm, layer_norm_backward, muon_step, orthogonalize
+from .dense import check_waits, layer_norm, layer_norm_backward, muon_step, orthogonalize
 from .store import (
     Adagrad,
     Adam,
@@ -60,7 +60,7 @@ __all__ = [
     "ModuloPartition", "ModuloPartitioner", "Optimizer", "PartitionSpec", "PartitionStrategy",
     "Partitioner", "SPARSE_EMBEDDING_FAST_RANGE_ASSIGNMENT_NAME", "SPARSE_EMBEDDING_HASH_ASSIGNMENT_NAME",
     "SPARSE_EMBEDDING_MODULO_ASSIGNMENT_NAME", "SUPPORTED_KEY_DTYPES", "Sgd", "StorageTuningOptions",
-    "Uniform", "Zeros", "create_partitioner", "create_strategy", "filter_partition",
+    "Uniform", "Zeros", "check_waits", "create_partitioner", "create_strategy", "filter_partition",
     "generate_reference_vectors", "is_partitioner_registered", "layer_norm", "layer_norm_backward",
     "muon_step", "orthogonalize", "partition", "register_partitioner",
 ]

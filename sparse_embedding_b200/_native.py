@@ -124,6 +124,7 @@ _SIGNATURES = {
     "se_muon_step": [_i32, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _sz, _i64, _i64, C.c_double,
                      C.c_double, C.c_double, C.c_double, _i32, _i32, C.c_float, _vp, _sz, _i32, _vp],
     "se_set_wait_limit": [_u64],
+    "se_check_waits": [_i32],
     "se_muon_workspace": [_i32, _sz, _i64, _i64, C.POINTER(_sz)],
     "se_exchange_create": [_vp, _i32, _u32, _u32, _u64, _i64, _u32, C.POINTER(_vp)],
     "se_exchange_handle": [_vp, _vp, _sz],

@@ -2,6 +2,7 @@
 // update): argument checks and dispatch on the value type.
 #pragma once
 
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 #include <cstdint>
@@ -82,32 +83,65 @@ inline std::atomic<long long> &wait_limit() {
   return clocks;
 }
 
-// A word in host memory that a kernel sets when one of its waits for a copy gave
-// up. The next call on the device reads it, without waiting for the GPU, and
-// reports it. (The word is allocated by the device's first call, which may be
-// under stream capture.)
-inline uint32_t *wait_status(int device) {
-  static std::mutex mu;
-  static std::map<int, uint32_t *> known;
-  std::lock_guard<std::mutex> lock(mu);
-  uint32_t *&word = known[device];
-  if (word == nullptr) {
-    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-    cuda_check(cudaThreadExchangeStreamCaptureMode(&mode), "cudaThreadExchangeStreamCaptureMode");
-    void *p = nullptr;
-    const cudaError_t e = cudaHostAlloc(&p, sizeof(uint32_t), cudaHostAllocMapped | cudaHostAllocPortable);
-    cudaThreadExchangeStreamCaptureMode(&mode);
-    cuda_check(e, "cudaHostAlloc");
-    *static_cast<volatile uint32_t *>(p) = 0u;
-    word = static_cast<uint32_t *>(p);
+// Words in host memory that a kernel sets when one of its waits gave up: one per
+// device and stream, so that the report reaches who works on that stream, and
+// not another thread or stream. They live as long as the process, as graphs do
+// that hold their addresses. A report is taken by an exchange: one that comes
+// while it is taken is seen then or the next time.
+class WaitWords {
+ public:
+  static WaitWords &get() {
+    static WaitWords words;
+    return words;
   }
-  volatile uint32_t *seen = word;
-  if (*seen != 0u) {
-    *seen = 0u;
-    throw Error(SE_ERR_RUNTIME, "an earlier layer normalisation or Muon update on cuda:" + std::to_string(device) +
-                                    " gave up waiting for its copies; its results are not valid");
+  // The word of a call on `stream`; throws where an earlier call's report is in it.
+  // (Memory for words may be asked for under stream capture.)
+  uint32_t *of(int device, cudaStream_t stream) {
+    static thread_local char here;
+    if (stream == cudaStreamLegacy) stream = nullptr;
+    const Key key{{device, stream}, stream == cudaStreamPerThread ? &here : nullptr};
+    std::lock_guard<std::mutex> lock(mu_);
+    auto it = known_.find(key);
+    if (it == known_.end()) it = known_.emplace(key, fresh()).first;
+    if (taken(it->second))
+      throw Error(SE_ERR_RUNTIME, "an earlier layer normalisation or Muon update on this stream of cuda:" +
+                                      std::to_string(device) + kGaveUp);
+    return it->second;
   }
-  return word;
-}
+  // All reports of a device.
+  void check(int device) {
+    std::lock_guard<std::mutex> lock(mu_);
+    bool any = false;
+    for (auto &k : known_)
+      if (k.first.first.first == device) any |= taken(k.second);
+    if (any) throw Error(SE_ERR_RUNTIME, "a layer normalisation or Muon update on cuda:" + std::to_string(device) + kGaveUp);
+  }
+
+ private:
+  using Key = std::pair<std::pair<int, cudaStream_t>, const void *>;
+  static constexpr const char *kGaveUp = " gave up waiting for its copies; its results are not valid";
+  static constexpr int kPage = 1024;
+  static bool taken(uint32_t *word) {
+    return *static_cast<volatile uint32_t *>(word) != 0u && __atomic_exchange_n(word, 0u, __ATOMIC_ACQ_REL) != 0u;
+  }
+  uint32_t *fresh() {
+    if (left_ == 0) {
+      cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+      cuda_check(cudaThreadExchangeStreamCaptureMode(&mode), "cudaThreadExchangeStreamCaptureMode");
+      void *p = nullptr;
+      const cudaError_t e = cudaHostAlloc(&p, kPage * sizeof(uint32_t), cudaHostAllocMapped | cudaHostAllocPortable);
+      cudaThreadExchangeStreamCaptureMode(&mode);
+      cuda_check(e, "cudaHostAlloc");
+      page_ = static_cast<uint32_t *>(p);
+      std::fill(page_, page_ + kPage, 0u);
+      left_ = kPage;
+    }
+    return page_ + --left_;
+  }
+  std::mutex mu_;
+  std::map<Key, uint32_t *> known_;
+  uint32_t *page_ = nullptr;
+  int left_ = 0;
+};
 
 }  // namespace se_gpu

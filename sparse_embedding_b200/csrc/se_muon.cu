@@ -1702,7 +1702,7 @@ void orthogonalise(UpdateArgs u, int grad_type, int64_t batch, int steps, float 
   g.square = cut(true, s, s, 1);
   g.apply = cut(false, w, s, 1);
   const int sms = sm_count(device);
-  g.status = wait_status(device);
+  g.status = WaitWords::get().of(device, st);
   g.limit = wait_limit();
   fin.transposed = transposed;
   const size_t ob = value_bytes(fin.type);

@@ -990,6 +990,10 @@ extern "C" int se_set_wait_limit(uint64_t clocks) {
   });
 }
 
+extern "C" int se_check_waits(int32_t device) {
+  return guarded([&] { WaitWords::get().check(device); });
+}
+
 extern "C" int se_layer_norm(int32_t value_dtype, int32_t param_dtype, const void *x, size_t rows, int64_t dim,
                              int64_t x_stride, const void *weight, const void *bias, float eps, void *y,
                              float *mean_out, float *rstd_out, int32_t device, void *stream) {
@@ -1007,7 +1011,7 @@ extern "C" int se_layer_norm(int32_t value_dtype, int32_t param_dtype, const voi
     check_device_ptr(rstd_out, device, "rstd", true);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int sms = sm_count(device);
-    uint32_t *status = wait_status(device);
+    uint32_t *status = WaitWords::get().of(device, st);
     const size_t vb = value_bytes(value_dtype);
     const NormShape s = norm_shape(dim, vb, aligned16(x) && aligned16(y) && (rows == 1 || x_stride * vb % 16 == 0),
                                    rows > 1 && x_stride != dim, false);
@@ -1068,7 +1072,7 @@ extern "C" int se_layer_norm_backward(int32_t value_dtype, int32_t param_dtype, 
     check_device_ptr(dbias, device, "dbias", true);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int sms = sm_count(device);
-    uint32_t *status = wait_status(device);
+    uint32_t *status = WaitWords::get().of(device, st);
     const bool sums = dweight != nullptr || dbias != nullptr;
     int blocks = 0;
     float *partial = nullptr;

@@ -8,7 +8,9 @@ Inputs are CUDA tensors (or DLPack objects in CUDA memory) whose last axis is
 contiguous; rows may lie further apart than their length, as slices of wider
 tensors do. The work runs on the current torch stream of the tensors' device,
 allocates from torch's allocator only and never waits for the GPU, so calls can
-be captured into CUDA graphs. `torch_ops` has the autograd forms.
+be captured into CUDA graphs. `torch_ops` has the autograd forms. A kernel
+whose waits gave up is reported by the next call on its stream (RuntimeError),
+or by `check_waits`.
 """
 
 from __future__ import annotations
@@ -189,6 +191,23 @@ def layer_norm_backward(grad, x, mean, rstd, weight=None, with_bias: bool = True
                                              dim, mean.data_ptr(), rstd.data_ptr(), _ptr(weight), dx.data_ptr(),
                                              _ptr(dw), _ptr(db), _ptr(work), nbytes, x.device.index, _stream(x)))
     return dx, dw, db
+
+
+def check_waits(device=None) -> None:
+    """Raises RuntimeError where a wait inside a dense operator's kernel on the
+    device (an index, a torch.device; the current one by default) has given up
+    and no call has reported it: the results of that call are not valid. The
+    host does not wait for the GPU, so synchronise first where it matters, as
+    after the last replay of a graph."""
+    torch = torch_mod()
+    if device is None or isinstance(device, int):
+        index = device
+    else:
+        where = torch.device(device)
+        if where.type != "cuda":
+            raise ValueError("device must be a CUDA device")
+        index = where.index
+    N.check(_entry("se_check_waits")(torch.cuda.current_device() if index is None else index))
 
 
 def _matrices(x, what: str):

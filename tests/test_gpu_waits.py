@@ -81,3 +81,40 @@ def test_normalisations_that_gave_up(dim, dt):
 def test_limits_are_checked():
     assert N.lib().se_set_wait_limit(8_000_000_001) == N.SE_ERR_INVALID_ARGUMENT
     assert b"at most 8e9" in N.lib().se_last_error()
+
+
+def test_reports_stay_with_their_stream():
+    u = rand(40, 96)
+    x, w = rand(2000, 128), torch.ones(128, device="cuda")
+    want, y = se.orthogonalize(u), se.layer_norm(x, w)
+    bad, other = torch.cuda.Stream(), torch.cuda.Stream()
+    with brief_waits(), torch.cuda.stream(bad):
+        se.orthogonalize(u)
+    with torch.cuda.stream(other):  # nobody else is refused
+        assert torch.equal(se.orthogonalize(u), want) and torch.equal(se.layer_norm(x, w), y)
+    assert torch.equal(se.orthogonalize(u), want)
+    with torch.cuda.stream(bad):
+        with pytest.raises(RuntimeError, match="gave up waiting"):
+            se.layer_norm(x, w)
+        assert torch.equal(se.layer_norm(x, w), y)
+
+
+def test_replayed_graphs_report():
+    w, g, mom = rand(300, 200), rand(300, 200, seed=1), torch.zeros(300, 200, device="cuda")
+    before = w.clone()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with brief_waits(), torch.cuda.graph(graph, stream=side):  # a graph keeps the limit of its capture
+        se.muon_step(w, g, mom)
+    se.check_waits()
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(w, before)
+        for device in (None, torch.device("cuda", 0)):
+            if device is None:
+                with pytest.raises(RuntimeError, match="gave up waiting"):
+                    se.check_waits()
+            else:
+                se.check_waits(device)  # taken once
+    se.check_waits(0)
+    se.check_waits("cuda:0")

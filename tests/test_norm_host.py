@@ -67,3 +67,10 @@ def test_no_rows_need_no_device():
     assert N.lib().se_layer_norm_backward_workspace(1, 8, 0, None) == N.SE_ERR_INVALID_ARGUMENT
     size = C.c_size_t()
     assert N.lib().se_layer_norm_backward_workspace(1, 0, 0, C.byref(size)) == N.SE_ERR_INVALID_ARGUMENT
+
+
+def test_waits_of_a_device():
+    N.check(N.lib().se_check_waits(0))  # nothing ran: nothing to report
+    se.check_waits(0)
+    with pytest.raises(ValueError, match="must be a CUDA device"):
+        se.check_waits("cpu")
