@@ -30,6 +30,7 @@
 // thread that holds it.
 
 #include <algorithm>
+#include <iterator>
 #include <type_traits>
 
 #include "se_dense.hpp"
@@ -362,24 +363,26 @@ constexpr int kThreads = 128 + 32 * kEpilogueWarps;
 constexpr int kFlush = 4;  // k-blocks of a SPLIT accumulation between two flushes
 
 // Shared memory of a CTA: operand stages, then the epilogue warps' staging
-// tiles (SPLIT stages all blocks of an accumulator at once: its sums would not
-// leave registers for the epilogue).
+// tiles.
 //
-// SPLIT with BN = 64 (kStacked) has hi and lo parts of both operands in a stage,
-// B's one below the other: A_hi times both is one instruction of N = 128, which
-// takes no longer than N = 64 (75 clocks: A is read from shared memory either
-// way), and A_lo B_hi adds to the half of A_hi B_lo: two thirds of the
-// instructions and of the loads of the three products one after another
-// (1000 x 517 fp32: 188 -> 159 us). At N = 128 an instruction of twice the width
-// takes twice as long, and there they stay apart.
+// SPLIT has hi and lo parts of both operands in a stage, B's one below the
+// other: A_hi times both is one instruction of N = 128, which takes no longer
+// than N = 64 (75 clocks: A is read from shared memory either way), and A_lo B_hi
+// adds to the half of A_hi B_lo: two thirds of the instructions and of the loads
+// of the three products one after another (1000 x 517 fp32: 188 -> 159 us). At
+// N = 128 an instruction of twice the width takes twice as long, so its tiles
+// are 128 x 64 always. (Wider ones with three products one after another, us,
+// 128 x 64 and the best of 128 x 128 and pairs: 1024 x 1024 fp32 181 and 286,
+// 2560 x 2560 1,210 and 1,393, 4096 x 4096 5,056 and 4,985, 6144 x 6144 18,070
+// and 17,408: too little and too rarely for kernels of their own.)
 template <int CG, int BN, bool SPLIT>
 struct Layout {
-  static constexpr bool kStacked = SPLIT && BN == 64 && CG == 1;
-  static constexpr int kA = 128 * 128 * (kStacked ? 2 : 1);        // bytes of a CTA's A tile: 128 rows of 64 values
-  static constexpr int kB = (BN / CG) * 128 * (kStacked ? 2 : 1);  // and of its part of the B tile
+  static_assert(!SPLIT || (CG == 1 && BN == 64), "the tile of three products");
+  static constexpr int kA = 128 * 128 * (SPLIT ? 2 : 1);        // bytes of a CTA's A tile: 128 rows of 64 values
+  static constexpr int kB = (BN / CG) * 128 * (SPLIT ? 2 : 1);  // and of its part of the B tile
   static constexpr int kStage = kA + kB;
-  static constexpr int kColumns = kStacked ? 2 * BN : BN;          // of an accumulator
-  static constexpr int kStaging = (SPLIT ? BN / 64 : 1) * 32 * 32;  // floats of a warp
+  static constexpr int kColumns = SPLIT ? 2 * BN : BN;          // of an accumulator
+  static constexpr int kStaging = 32 * 32;                      // floats of a warp
   static constexpr int kStagingBytes = kEpilogueWarps * kStaging * 4;
   static constexpr int kRoom = 232448 - 1024 - 512 - kStagingBytes;  // 1,024: tile alignment; 512: static variables
   static constexpr int kStages = kRoom / kStage < 8 ? kRoom / kStage : 8;
@@ -714,14 +717,12 @@ __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int s
   constexpr int kTM = 128 * CG, kBlocks = BN / 64;          // kBlocks: column blocks of an epilogue warp
   constexpr bool kBMN = MODE == kApply || MODE == kFinish;  // the B operand is X itself: n-contiguous
   constexpr uint32_t kStages = L::kStages;
-  constexpr bool kStacked = L::kStacked;
   const int warp = int(threadIdx.x) >> 5, lane = int(threadIdx.x) & 31;
   const int unit = int(blockIdx.x) / CG, units = int(gridDim.x) / CG;
   const int parts = MODE == kGram ? c.parts : 1;
   const int total = c.tiles * parts * g.batch;
-  const int kall = c.kblocks * (SPLIT && !kStacked ? 3 : 1);
-  // the k-blocks of part p: [kall p / parts, kall (p + 1) / parts)
-  auto k_from = [&](int p) { return MODE == kGram ? int(int64_t(kall) * p / parts) : p * kall; };
+  // the k-blocks of part p
+  auto k_from = [&](int p) { return MODE == kGram ? int(int64_t(c.kblocks) * p / parts) : p * c.kblocks; };
   auto sum_end = [&](int k, int last) { return SPLIT ? min(last, k + kFlush) : last; };
 
   if (warp == 0) {
@@ -743,22 +744,19 @@ __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int s
             go = false;
             break;
           }
-          // hi lo, lo hi, hi hi
-          const int seg = SPLIT && !kStacked ? (k >= c.kblocks) + (k >= 2 * c.kblocks) : 2;
-          const int k0 = (SPLIT && !kStacked ? k - seg * c.kblocks : k) * kTileK;
-          const CUtensorMap *ma = seg == 1 ? al : ah, *mb = seg == 0 ? bl : bh;
+          const int k0 = k * kTileK;
           uint8_t *a = smem + st * L::kStage, *b = a + L::kA;
           uint32_t bar = smem_u32(&sh.full[st]);
           if constexpr (CG == 2) bar = mapa(bar, 0);
           if (rank == 0) mbar_arrive_expect_tx(&sh.full[st], CG * L::kStage);
 #pragma unroll
-          for (int q = 0; q < 2; ++q) tma_load<CG>(a + q * 8192, ma, k0, row + q * 64, z, bar);
+          for (int q = 0; q < 2; ++q) tma_load<CG>(a + q * 8192, ah, k0, row + q * 64, z, bar);
 #pragma unroll
           for (int q = 0; q < BN / CG / 64; ++q) {
-            if constexpr (kBMN) tma_load<CG>(b + q * 8192, mb, col + q * 64, k0, z, bar);
-            else tma_load<CG>(b + q * 8192, mb, k0, col + q * 64, z, bar);
+            if constexpr (kBMN) tma_load<CG>(b + q * 8192, bh, col + q * 64, k0, z, bar);
+            else tma_load<CG>(b + q * 8192, bh, k0, col + q * 64, z, bar);
           }
-          if constexpr (kStacked) {
+          if constexpr (SPLIT) {
 #pragma unroll
             for (int q = 0; q < 2; ++q) tma_load<CG>(a + 16384 + q * 8192, al, k0, row + q * 64, z, bar);
             if constexpr (kBMN) tma_load<CG>(b + 8192, bl, col, k0, z, bar);
@@ -805,7 +803,7 @@ __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int s
             add = true;
 #pragma unroll
             for (int q = 1; q < kTileK / 16; ++q) mma_f16<CG>(acc, da + q * kStepA, db + q * kStepB, kDesc, true);
-            if constexpr (kStacked) {
+            if constexpr (SPLIT) {
 #pragma unroll
               for (int q = 0; q < kTileK / 16; ++q)
                 mma_f16<CG>(acc + BN, da + (16384 >> 4) + q * kStepA, db + q * kStepB, kLoDesc, true);
@@ -860,49 +858,37 @@ __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int s
         for (int e = 0; e < 32; e += 4)
           *reinterpret_cast<float4 *>(to + tile_place(lane, e)) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
       };
-      auto finish = [&](int b, float *staged) {
-        finish_block<MODE, OUT>(g, step, staged, z, r0, column(b), dr, input, [&] { ask(b + 1); });
+      auto finish = [&](int b) {
+        finish_block<MODE, OUT>(g, step, tile, z, r0, column(b), dr, input, [&] { ask(b + 1); });
       };
       // in parts: this warp's place among the warps of all tiles, and its blocks
       const int64_t place = (int64_t(zt) * CG + rank) * kEpilogueWarps + warp - 4;
       const bool in_parts = MODE == kGram && parts > 1;
       if constexpr (SPLIT) {
-        static_assert(kBlocks <= 2, "the sums stay in registers");
-        float v[kBlocks][32];
-#pragma unroll
-        for (int b = 0; b < kBlocks; ++b) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) v[b][e] = 0.0f;
-        }
+        float v[32] = {};
         for (int k = k_from(part), last = k_from(part + 1); k < last; k = sum_end(k, last)) {
           if (!take()) break;
 #pragma unroll
-          for (int b = 0; b < kBlocks; ++b) {
+          for (int part_of = 0; part_of < 2; ++part_of) {  // hi hi, then hi lo + lo hi
             float f[32];
-            tmem_load32(tmem + at.sum.at * L::kColumns + uint32_t(b * 32), f);
+            tmem_load32(tmem + at.sum.at * L::kColumns + uint32_t(part_of * BN), f);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) v[b][e] += f[e];
-            if constexpr (kStacked) {
-              tmem_load32(tmem + at.sum.at * L::kColumns + uint32_t(BN + b * 32), f);
-#pragma unroll
-              for (int e = 0; e < 32; ++e) v[b][e] += f[e];
-            }
+            for (int e = 0; e < 32; ++e) v[e] += f[e];
           }
           give();
         }
         if (!go) break;
+        if (!wanted(0)) continue;
         __syncwarp();
-#pragma unroll
-        for (int b = 0; b < kBlocks; ++b) stage(tile + b * 1024, v[b]);
+        stage(tile, v);
         __syncwarp();
         if (in_parts) {
-          for (int b = 0; b < kBlocks && wanted(b); ++b) leave_part(g, tile + b * 1024, place * kBlocks + b, part);
-          if (!wanted(0) || !last_part(g, g.arrived + place)) continue;
-          for (int b = 0; b < kBlocks && wanted(b); ++b) join_parts(g, tile + b * 1024, place * kBlocks + b);
+          leave_part(g, tile, place, part);
+          if (!last_part(g, g.arrived + place)) continue;
+          join_parts(g, tile, place);
         }
         ask(0);  // not earlier: the sums fill the registers
-#pragma unroll 1
-        for (int b = 0; b < kBlocks && wanted(b); ++b) finish(b, tile + b * 1024);
+        finish(0);
       } else {
         if (!take()) break;
 #pragma unroll 1
@@ -914,14 +900,14 @@ __device__ __forceinline__ void run_product(const NsArgs &g, const Cut &c, int s
           stage(tile, v);
           __syncwarp();
           if (in_parts) leave_part(g, tile, place * kBlocks + b, part);
-          else finish(b, tile);
+          else finish(b);
         }
         give();
         if (in_parts && wanted(0) && last_part(g, g.arrived + place)) {
 #pragma unroll 1
           for (int b = 0; b < kBlocks && wanted(b); ++b) {
             join_parts(g, tile, place * kBlocks + b);
-            finish(b, tile);
+            finish(b);
           }
         }
       }
@@ -1540,23 +1526,24 @@ struct Plan {
 // The form with the least estimated time of a step. A product takes, for each
 // round of tiles over the units, its k-blocks times the clocks of a stage, and
 // at its end the last epilogue and the barrier. Both were measured for each
-// form (clocks; with SPLIT the flushes come on top) and are rounded here; the
-// estimate orders the forms as their times do, e.g. at 4096 x 4096 bf16 (us)
-// 1x64 1944, 1x128 1416, 1x256 1512, 2x128 1506, 2x256 1336; at 2048 x 2048
-// 334, 258, 366, 248, 363; at 1024 x 1024 134, 182, 283, 178, 283; 2048 x 2048
-// fp32 1048, 672, -, 638, -.
+// form (clocks) and are rounded here; the estimate mostly orders the forms as
+// their times do, e.g. bf16 (us) at 4096 x 4096 1x64 2341, 1x128 1534, 1x256
+// 1384, 2x128 1356, 2x256 1344; at 2048 x 2048 300, 245, 331, 236, 331; at 1024 x
+// 1024 111, 145, 218, 147, 218. Three products have one form, and only their
+// parts are chosen. (kUnits, not the device's multiprocessors: the workspace is
+// asked for without a device, and a launch never takes more blocks than run at once.)
 Plan plan_for(int64_t batch, int64_t s, int64_t w, bool split) {
   struct Form {
-    int cg, bn, stage, end, stage_split, end_split;
+    int cg, bn, stage, end;
   };
-  constexpr Form forms[] = {{1, 64, 330, 8000, 650, 12000}, {1, 128, 420, 11000, 1350, 16000}, {2, 128, 400, 11000, 1290, 16000},
-                            {1, 256, 600, 20000, 0, 0},     {2, 256, 560, 20000, 0, 0}};
+  constexpr Form single[] = {{1, 64, 330, 8000}, {1, 128, 420, 11000}, {2, 128, 400, 11000}, {1, 256, 600, 20000}, {2, 256, 560, 20000}};
+  constexpr Form three[] = {{1, 64, 650, 12000}};
   constexpr int kJoin = 8000;  // clocks to add up parts
   Plan best{};
   int64_t least = 0;
-  for (const Form &f : forms) {
-    const int64_t stage = split ? f.stage_split : f.stage, end = split ? f.end_split : f.end, units = kUnits / f.cg;
-    if (stage == 0) continue;
+  for (const Form *at = split ? three : single, *last = split ? std::end(three) : std::end(single); at != last; ++at) {
+    const Form &f = *at;
+    const int64_t stage = f.stage, units = kUnits / f.cg;
     auto rounds = [&](int64_t tiles) { return (tiles + units - 1) / units; };
     const int64_t sym = tile_count(true, s, s, 128 * f.cg, f.bn) * batch;
     const int64_t app = tile_count(false, s, w, 128 * f.cg, f.bn) * batch;
@@ -1565,7 +1552,7 @@ Plan plan_for(int64_t batch, int64_t s, int64_t w, bool split) {
     const int64_t parts =
         kw * stage < 2 * kJoin ? 1 : std::max<int64_t>(1, std::min<int64_t>(units / sym, kw * stage / 5000));
     const int64_t clocks = (rounds(sym * parts) * ((kw + parts - 1) / parts) + rounds(sym) * ks + rounds(app) * ks) * stage +
-                           (parts > 1 ? kJoin : 0) + 3 * end;
+                           (parts > 1 ? kJoin : 0) + 3 * f.end;
     if (least == 0 || clocks < least) {
       least = clocks;
       best = Plan{f.cg, f.bn, int(parts)};
@@ -1776,16 +1763,16 @@ void orthogonalise(UpdateArgs u, int grad_type, int64_t batch, int steps, float 
   const int form = plan.cg * 1000 + plan.bn;
   dispatch_value(fin.type, [&](auto out) {
     using OUT = decltype(out);
-    switch (form) {
-      case 2128: launch_newton_schulz<2, 128, OUT>(g, units, device, st); return;
-      case 1128: launch_newton_schulz<1, 128, OUT>(g, units, device, st); return;
-      case 1064: launch_newton_schulz<1, 64, OUT>(g, units, device, st); return;
-      default: break;
-    }
     if constexpr (std::is_same_v<OUT, BF16>) {  // wider tiles: single products only
-      if (form == 2256) launch_newton_schulz<2, 256, OUT>(g, units, device, st);
-      else launch_newton_schulz<1, 256, OUT>(g, units, device, st);
+      switch (form) {
+        case 1128: return launch_newton_schulz<1, 128, OUT>(g, units, device, st);
+        case 2128: return launch_newton_schulz<2, 128, OUT>(g, units, device, st);
+        case 1256: return launch_newton_schulz<1, 256, OUT>(g, units, device, st);
+        case 2256: return launch_newton_schulz<2, 256, OUT>(g, units, device, st);
+        default: break;
+      }
     }
+    launch_newton_schulz<1, 64, OUT>(g, units, device, st);
   });
   if (!fin.update) return;
   dispatch_value(fin.type, [&](auto out) {
