@@ -23,7 +23,10 @@
 //    hi hi + hi lo + lo hi, three times the matrix work, for errors of fp32's order.
 // Against 64 bits, for gradient-like matrices: 0.03 to 0.1 % from the single
 // products (bf16's own rounding is 0.17 %), 0.5e-6 to 1.3e-6 from the triple ones
-// (fp32 operations in place of them: 0.7e-6 to 3e-6).
+// (fp32 operations in place of them: 0.7e-6 to 3e-6). With 1 to 8 directions far
+// above the rest, where noise is magnified most, the triple products' error is
+// 0.2 to 0.9 of that of fp32 operations (100 x 200 to 2048 x 1024); X in fp32
+// beside the pair would take a tenth off it, for a third more of the workspace.
 //
 // A and A A are symmetric: only tiles that touch the lower triangle are
 // computed, and an element below the diagonal is written to both places by the
