@@ -310,6 +310,9 @@ int se_layer_norm_backward(int32_t value_dtype, int32_t param_dtype, const void 
                            void *workspace, size_t workspace_bytes, int32_t device, void *stream);
 int se_layer_norm_backward_workspace(size_t rows, int64_t dim, int32_t device, size_t *bytes);
 
+/* Or'ed to the dtype of a Muon call's result (and of its workspace): a bf16
+ * result of full products, as fp32 and f16 results always are. */
+#define SE_FULL_PRODUCTS 0x100
 /* Orthogonalises `batch` updates of m x n values by Newton-Schulz products:
  * X = U / (|U|_F + eps), then `steps` times (1 to 100) A = X X^T,
  * X = 3.4445 X + (-4.7750 A + 2.0315 A A) X (on U^T where m > n), which brings
@@ -317,8 +320,8 @@ int se_layer_norm_backward_workspace(size_t rows, int64_t dim, int32_t device, s
  * starts batch_stride values after matrix k - 1, its rows are row_stride
  * apart; out is batch x m x n without gaps, of the same dtype, and overlaps
  * no input. Products of f16 pairs with fp32 sums: a bf16 result is within its
- * own rounding of the exact one, fp32 and f16 results use three products for
- * one. `workspace`: se_muon_workspace bytes, 256-byte aligned. */
+ * own rounding of the exact one, fp32 and f16 results, and bf16 ones with
+ * SE_FULL_PRODUCTS, use three products for one. `workspace`: se_muon_workspace bytes, 256-byte aligned. */
 int se_orthogonalize(int32_t dtype, const void *update, size_t batch, int64_t m, int64_t n, int64_t batch_stride,
                      int64_t row_stride, int32_t steps, float eps, void *out, void *workspace,
                      size_t workspace_bytes, int32_t device, void *stream);

@@ -19,8 +19,9 @@
 //  * The diagonals of A and of B are kept apart in fp32, and the matrices hold
 //    zeros there: near the end A is close to the identity, and its rounding
 //    would be the largest error left. With A = D + O:  A A = O O + D O + O D + D D.
-//  * bf16 outputs: products of the hi parts alone. fp32 and f16 outputs:
-//    hi hi + hi lo + lo hi, three times the matrix work, for errors of fp32's order.
+//  * bf16 outputs: products of the hi parts alone, unless the caller asks for
+//    full ones. fp32 and f16 outputs, and bf16 ones then: hi hi + hi lo + lo hi,
+//    three times the matrix work, for errors of fp32's order.
 // Against 64 bits, for gradient-like matrices: 0.03 to 0.1 % from the single
 // products (bf16's own rounding is 0.17 %), 0.5e-6 to 1.3e-6 from the triple ones
 // (fp32 operations in place of them: 0.7e-6 to 3e-6). With 1 to 8 directions far
@@ -46,6 +47,8 @@ namespace {
 constexpr float kNsA = 3.4445f, kNsB = -4.7750f, kNsC = 2.0315f;
 constexpr float kScale = 8192.0f;  // S
 constexpr int kTileK = 64;         // k-values of a stage: one 128-byte swizzle row
+
+struct BF16Full : BF16 {};  // bf16 results of full products: any result type but BF16 has three for one
 
 // ---------------------------------------------------------------------------
 // Momentum, norm, and the scaled update X_0
@@ -1509,7 +1512,20 @@ CUtensorMap matrix_map(const __half *p, int64_t rows, int64_t cols, int64_t ld, 
   return map;
 }
 
-bool split_products(int32_t out_type) { return out_type != SE_BFLOAT16; }
+// A type argument, its flag taken off, and whether the products are full.
+struct ResultType {
+  int32_t type;
+  bool split;
+};
+ResultType result_type(int32_t t, const char *what) {
+  const int32_t type = t & ~SE_FULL_PRODUCTS;
+  check_value_dtype(type, what);
+  return {type, t != SE_BFLOAT16};
+}
+template <class F> void dispatch_result(int32_t type, bool split, F &&f) {
+  if (type == SE_BFLOAT16 && split) f(BF16Full{});
+  else dispatch_value(type, f);
+}
 
 int64_t tile_count(bool symmetric, int64_t rows, int64_t cols, int tm, int bn) {
   const int64_t ti = (rows + tm - 1) / tm, tj = (cols + bn - 1) / bn;
@@ -1712,9 +1728,10 @@ void orthogonalise(UpdateArgs u, int grad_type, int64_t batch, int steps, float 
       if (w > 128) start(std::integral_constant<int, 2>{});
       else start(std::integral_constant<int, 4>{});
     };
-    dispatch_value(fin.type, [&](auto out) {
-      if (!fin.update) launch(out, out, std::false_type{});  // an update and its result have one type
-      else if (grad_type == fin.type) launch(out, out, std::true_type{});
+    dispatch_result(fin.type, split, [&](auto out) {
+      using Grad = std::conditional_t<std::is_same_v<decltype(out), BF16Full>, BF16, decltype(out)>;
+      if (!fin.update) launch(Grad{}, out, std::false_type{});  // an update and its result have one type
+      else if (grad_type == fin.type) launch(Grad{}, out, std::true_type{});
       else launch(F32{}, out, std::true_type{});
     });
     launched("k_newton_schulz_small");
@@ -1764,7 +1781,7 @@ void orthogonalise(UpdateArgs u, int grad_type, int64_t batch, int steps, float 
   g.fin = fin;
   const int64_t units = std::max<int64_t>(int64_t(g.gram.tiles) * plan.parts, g.apply.tiles) * batch;
   const int form = plan.cg * 1000 + plan.bn;
-  dispatch_value(fin.type, [&](auto out) {
+  dispatch_result(fin.type, split, [&](auto out) {
     using OUT = decltype(out);
     if constexpr (std::is_same_v<OUT, BF16>) {  // wider tiles: single products only
       switch (form) {
@@ -1809,12 +1826,12 @@ using namespace se_gpu;
 
 extern "C" int se_muon_workspace(int32_t out_dtype, size_t batch, int64_t m, int64_t n, size_t *bytes) {
   return guarded([&] {
-    check_value_dtype(out_dtype, "out_dtype");
+    const ResultType out = result_type(out_dtype, "out_dtype");
     check_matrices(batch, m, n, 1, 0.0f);
     if (bytes == nullptr) throw std::invalid_argument("bytes is null");
     *bytes = batch == 0 || m == 0 || n == 0
                  ? 0
-                 : muon_space(nullptr, int64_t(batch), std::min(m, n), std::max(m, n), split_products(out_dtype)).bytes;
+                 : muon_space(nullptr, int64_t(batch), std::min(m, n), std::max(m, n), out.split).bytes;
   });
 }
 
@@ -1822,7 +1839,7 @@ extern "C" int se_orthogonalize(int32_t dtype, const void *update, size_t batch,
                                 int64_t batch_stride, int64_t row_stride, int32_t steps, float eps, void *out,
                                 void *workspace, size_t workspace_bytes, int32_t device, void *stream) {
   return guarded([&] {
-    check_value_dtype(dtype, "dtype");
+    const ResultType result = result_type(dtype, "dtype");
     check_matrices(batch, m, n, steps, eps);
     if (batch == 0 || m == 0 || n == 0) return;
     check_strides("update", batch, m, n, batch_stride, row_stride);
@@ -1837,10 +1854,10 @@ extern "C" int se_orthogonalize(int32_t dtype, const void *update, size_t batch,
     u.n = n;
     FinishArgs fin{};
     fin.out = out;
-    fin.type = dtype;
+    fin.type = result.type;
     fin.row = n;
     fin.batch = m * n;
-    orthogonalise(u, dtype, int64_t(batch), steps, eps, split_products(dtype), fin, workspace, workspace_bytes, device,
+    orthogonalise(u, result.type, int64_t(batch), steps, eps, result.split, fin, workspace, workspace_bytes, device,
                   static_cast<cudaStream_t>(stream));
   });
 }
@@ -1852,9 +1869,9 @@ extern "C" int se_muon_step(int32_t weight_dtype, int32_t grad_dtype, void *weig
                             double weight_decay, double scale, int32_t nesterov, int32_t steps, float eps,
                             void *workspace, size_t workspace_bytes, int32_t device, void *stream) {
   return guarded([&] {
-    check_value_dtype(weight_dtype, "weight_dtype");
+    const ResultType result = result_type(weight_dtype, "weight_dtype");
     check_value_dtype(grad_dtype, "grad_dtype");
-    if (grad_dtype != weight_dtype && grad_dtype != SE_FLOAT32)
+    if (grad_dtype != result.type && grad_dtype != SE_FLOAT32)
       throw std::invalid_argument("grad_dtype must be weight_dtype or float32");
     check_matrices(batch, m, n, steps, eps);
     if (!std::isfinite(lr) || !std::isfinite(beta) || !std::isfinite(weight_decay) || !std::isfinite(scale))
@@ -1879,13 +1896,13 @@ extern "C" int se_muon_step(int32_t weight_dtype, int32_t grad_dtype, void *weig
     u.n = n;
     FinishArgs fin{};
     fin.out = weight;
-    fin.type = weight_dtype;
+    fin.type = result.type;
     fin.update = 1;
     fin.row = weight_row_stride;
     fin.batch = weight_batch_stride;
     fin.keep = float(1.0 - lr * weight_decay);
     fin.rate = float(lr * scale);
-    orthogonalise(u, grad_dtype, int64_t(batch), steps, eps, split_products(weight_dtype), fin, workspace, workspace_bytes, device,
+    orthogonalise(u, grad_dtype, int64_t(batch), steps, eps, result.split, fin, workspace, workspace_bytes, device,
                   static_cast<cudaStream_t>(stream));
   });
 }

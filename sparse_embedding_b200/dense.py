@@ -227,22 +227,33 @@ def _matrices(x, what: str):
     return batch, m, n, (bs if batch > 1 else m * rs), rs
 
 
-def _muon_work(x, batch: int, m: int, n: int):
-    nbytes = _workspace_bytes("se_muon_workspace", _code(x.dtype), batch, m, n)
+_FULL_PRODUCTS = 0x100  # SE_FULL_PRODUCTS
+
+
+def _muon_code(x, precise: bool) -> int:
+    return _code(x.dtype) | (_FULL_PRODUCTS if precise else 0)
+
+
+def _muon_work(x, code: int, batch: int, m: int, n: int):
+    nbytes = _workspace_bytes("se_muon_workspace", code, batch, m, n)
     return _bytes(x, nbytes), nbytes
 
 
-def orthogonalize(update, steps: int = 5, eps: float = 1e-7):
+def orthogonalize(update, steps: int = 5, eps: float = 1e-7, precise: bool = False):
     """Newton-Schulz orthogonalisation of update [..., m, n] (float32, float16
     or bfloat16), as the Muon optimizer applies it: X = U / (|U| + eps), then
     `steps` times X = 3.4445 X + (-4.7750 A + 2.0315 A A) X with A = X X^T
     (from the smaller side). Leading axes are a batch of separate matrices.
-    Returns a new tensor of update's shape and dtype."""
+    Returns a new tensor of update's shape and dtype. A bfloat16 result comes
+    from products of 11-bit values, within about its own rounding; with
+    `precise` from products of 22 bits, as float32 and float16 results do, at
+    about three times the matrix work."""
     u = _cuda_tensor(update, "update")
     batch, m, n, bs, rs = _matrices(u, "update")
     out = _like(u)
-    work, nbytes = _muon_work(u, batch, m, n)
-    N.check(_entry("se_orthogonalize")(_code(u.dtype), u.data_ptr(), batch, m, n, bs, rs, int(steps), float(eps),
+    code = _muon_code(u, precise)
+    work, nbytes = _muon_work(u, code, batch, m, n)
+    N.check(_entry("se_orthogonalize")(code, u.data_ptr(), batch, m, n, bs, rs, int(steps), float(eps),
                                        out.data_ptr(), work.data_ptr(), nbytes, u.device.index, _stream(u)))
     return out
 
@@ -254,7 +265,8 @@ def _span(x):
 
 
 def muon_step(weight, grad, momentum, lr: float = 0.02, beta: float = 0.95, weight_decay: float = 0.0,
-              nesterov: bool = True, steps: int = 5, eps: float = 1e-7, scale: float | None = None) -> None:
+              nesterov: bool = True, steps: int = 5, eps: float = 1e-7, scale: float | None = None,
+              precise: bool = False) -> None:
     """One Muon step of weight [..., m, n], in place (outside autograd):
 
         momentum = beta momentum + grad
@@ -262,7 +274,8 @@ def muon_step(weight, grad, momentum, lr: float = 0.02, beta: float = 0.95, weig
         weight = (1 - lr weight_decay) weight - lr scale orthogonalize(U)
 
     momentum is float32 of weight's shape; grad has weight's dtype or float32.
-    scale is sqrt(max(1, m / n)) unless given. The three lie in memory of their
+    scale is sqrt(max(1, m / n)) unless given, `precise` as in orthogonalize
+    (for bfloat16 weights). The three lie in memory of their
     own: ranges that overlap, slices of one tensor among them, are refused."""
     w, g, mom = (_cuda_tensor(t, what) for t, what in ((weight, "weight"), (grad, "grad"), (momentum, "momentum")))
     torch = torch_mod()
@@ -283,8 +296,9 @@ def muon_step(weight, grad, momentum, lr: float = 0.02, beta: float = 0.95, weig
             raise ValueError("weight, grad and momentum must not share memory")
     if scale is None:
         scale = math.sqrt(max(1.0, m / n)) if n else 1.0
-    work, nbytes = _muon_work(w, batch, m, n)
-    N.check(_entry("se_muon_step")(_code(w.dtype), _code(g.dtype), w.data_ptr(), wbs, wrs, g.data_ptr(), gbs, grs,
+    code = _muon_code(w, precise)
+    work, nbytes = _muon_work(w, code, batch, m, n)
+    N.check(_entry("se_muon_step")(code, _code(g.dtype), w.data_ptr(), wbs, wrs, g.data_ptr(), gbs, grs,
                                    mom.data_ptr(), mbs, mrs, batch, m, n, float(lr), float(beta), float(weight_decay),
                                    float(scale), int(bool(nesterov)), int(steps), float(eps), work.data_ptr(), nbytes,
                                    w.device.index, _stream(w)))

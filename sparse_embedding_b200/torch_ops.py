@@ -67,12 +67,18 @@ class Muon(torch.optim.Optimizer):
     """Muon for the dense matrices of a model, next to the store's own row
     optimizers: each parameter [..., m, n] takes dense.muon_step with a float32
     momentum (leading axes are separate matrices: stacked layers or experts).
-    Vectors (biases, normalisation weights) need another optimizer."""
+    Vectors (biases, normalisation weights) need another optimizer. `precise`:
+    full products for bfloat16 parameters too (dense.orthogonalize)."""
 
     def __init__(self, params, lr: float = 0.02, momentum: float = 0.95, weight_decay: float = 0.0,
-                 nesterov: bool = True, steps: int = 5, eps: float = 1e-7):
+                 nesterov: bool = True, steps: int = 5, eps: float = 1e-7, precise: bool = False):
         super().__init__(params, dict(lr=lr, momentum=momentum, weight_decay=weight_decay, nesterov=nesterov,
-                                      steps=steps, eps=eps))
+                                      steps=steps, eps=eps, precise=precise))
+
+    def __setstate__(self, state) -> None:
+        super().__setstate__(state)
+        for group in self.param_groups:
+            group.setdefault("precise", False)  # states from before it was there
 
     def add_param_group(self, param_group) -> None:
         super().add_param_group(param_group)
@@ -107,5 +113,6 @@ class Muon(torch.optim.Optimizer):
                     state["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
                 dense.muon_step(p, p.grad.contiguous(), state["momentum_buffer"], lr=group["lr"],
                                 beta=group["momentum"], weight_decay=group["weight_decay"],
-                                nesterov=group["nesterov"], steps=group["steps"], eps=group["eps"])
+                                nesterov=group["nesterov"], steps=group["steps"], eps=group["eps"],
+                                precise=group["precise"])
         return loss

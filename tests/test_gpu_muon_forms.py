@@ -65,3 +65,39 @@ def test_form(shape, dt, form):
     again = torch.zeros_like(u)
     se.muon_step(again, u, torch.zeros_like(mom), lr=1.0, beta=0.0, scale=-1.0)
     assert torch.equal(again, w)
+
+
+@pytest.mark.parametrize("shape", [(40, 70), (3, 128, 200), (300, 520), (2, 1561, 129), (1300, 1200)])
+def test_full_products_for_bf16(shape):
+    """The same products as for fp32: the bf16 result is the fp32 one's rounding, bit by bit; a step's weights are within
+    half a step of bf16 of those from it, with 2^-22 |O| for its pair of f16 and fp32 roundings of lr and decay."""
+    u = matrix(*shape).to(BF16)
+    full = se.orthogonalize(u.float())
+    o = se.orthogonalize(u, precise=True)
+    assert o.dtype == BF16 and torch.equal(o, full.to(BF16))
+    assert not torch.equal(o, se.orthogonalize(u))
+    for grad in (u, u.float()):
+        w = matrix(*reversed(shape)).mT.reshape(shape).to(BF16).contiguous()
+        before, mom = w.double(), torch.zeros(shape, device="cuda")
+        se.muon_step(w, grad, mom, lr=0.5, beta=0.0, weight_decay=0.1, scale=2.0, precise=True)
+        want = before * 0.95 - full.double()
+        tol = 2.0**-8 * want.abs() + 2.0**-22 * (before.abs() + 2 * full.double().abs())
+        assert bool(((w.double() - want).abs() <= tol).all())
+
+
+def test_optimizer_takes_full_products():
+    from sparse_embedding_b200 import torch_ops
+
+    p = [torch.nn.Parameter(matrix(96, 64).to(BF16)) for _ in range(2)]
+    step = matrix(96, 65)[:, 1:].to(BF16).contiguous()
+    want = p[0].detach().clone()
+    se.muon_step(want, step, torch.zeros(96, 64, device="cuda"), lr=0.1, precise=True)
+    old = torch_ops.Muon([p[1]], lr=0.1)
+    state = old.state_dict()
+    del state["param_groups"][0]["precise"]  # a state from before
+    old.load_state_dict(state)
+    for q in p:
+        q.grad = step.clone()
+    torch_ops.Muon([p[0]], lr=0.1, precise=True).step()
+    old.step()
+    assert torch.equal(p[0], want) and not torch.equal(p[1], want)

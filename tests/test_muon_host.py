@@ -90,3 +90,13 @@ def test_optimizer_refuses_vectors():
     opt.step()  # no gradients: nothing to do
     with pytest.raises(ValueError, match="at least two dimensions"):
         opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(4))]})
+
+
+def test_full_products_flag():
+    full = dense._FULL_PRODUCTS
+    size = [C.c_size_t() for _ in range(4)]
+    for out, code in zip(size, (0, 2, 2 | full, full)):
+        N.check(N.lib().se_muon_workspace(code, 1, 1000, 2000, C.byref(out)))
+    assert size[1].value < size[2].value == size[0].value == size[3].value
+    assert orth(dtype=3 | full) == orth(dtype=2 | full << 1) == N.SE_ERR_INVALID_ARGUMENT
+    assert b"unsupported dtype" in N.lib().se_last_error()
