@@ -87,3 +87,31 @@ def test_many_tiles_a_block(rows, dim, dt, pad, offset):
     for _ in range(10):
         assert all(torch.equal(p, q) for p, q in zip(se.layer_norm_backward(g, x, zero, one, w), first))
         assert torch.equal(se.layer_norm(x, w), y)
+
+
+# Equal values whose rounding in a long chain of adds goes one way: c lies 0.49 of a step of [256, 512) above its grid.
+BIASED = (3277 + 0.49) * 2.0**-15
+
+
+@pytest.mark.parametrize("dim", [1 << 22, (1 << 23) + 5])
+def test_one_very_long_row(dim):
+    """A thread's sum is pieces of 64, those in pieces of 64, and at most 5 of those; then 10 levels over the block: 64 + 64 +
+    5 + 10 roundings and the quotient's, 150 u of equal values' sum. (One chain of dim / 512 adds is 900 u off and more.)"""
+    x = torch.full((1, dim), BIASED, device="cuda")
+    c = float(x[0, 0].double())
+    _, mean, rstd = se.layer_norm(x, eps=1.0, return_stats=True)
+    assert abs(float(mean) - c) <= 150 * U * c and abs(float(rstd) - 1.0) <= 4 * U
+    # with x = 1, mean = 0 and rstd = 1 both sums are of equal values: dx = g (1 - 1 - 1)
+    one = torch.ones(1, device="cuda")
+    dx, _, _ = se.layer_norm_backward(x, torch.ones_like(x), torch.zeros_like(one), one)
+    assert float((dx.double() + c).abs().max()) <= (2 * 150 + 4) * U * c
+
+
+def test_columns_of_many_long_rows():
+    """64 splits of the rows: as above, with 64 more adds of the splits."""
+    rows, dim = 400_000, 8200
+    x = torch.ones(rows, dim, dtype=torch.bfloat16, device="cuda")
+    r = torch.full((rows,), BIASED, device="cuda")
+    dw = se.layer_norm_backward(x, x, torch.zeros_like(r), r, torch.ones(dim, device="cuda"))[1]
+    want = rows * float(r[0].double())
+    assert float((dw.double() - want).abs().max()) <= (64 + 64 + 2 + 64) * U * want
