@@ -865,21 +865,27 @@ k_norm_columns_long(const typename V::T *__restrict__ grad, int64_t g_stride, co
 // the 32 threads of a column takes every 32nd block, then the 32 in order).
 // Launch and latency bound it: 3.6 us for 128 columns, 8.7 for 4,096.
 __global__ void __launch_bounds__(1024)
-k_norm_columns(const float *__restrict__ partial, int blocks, int64_t dim, void *__restrict__ dweight,
+k_norm_columns(const float *__restrict__ partial, int64_t blocks, int64_t dim, void *__restrict__ dweight,
                void *__restrict__ dbias, int ptype) {
   __shared__ float part[32][33];
   const int lane = threadIdx.x & 31, strip = threadIdx.x >> 5;
   const int64_t c = int64_t(blockIdx.x) * 32 + lane;
   pdl_wait();
-  float f = 0.0f;
+  LongSum sum;
   if (c < 2 * dim) {
+    for (int64_t base = 0; base < blocks; base += 32 * kPiece) {
+      const int count = int(min(blocks - base, int64_t(32 * kPiece)));
+      const float *from = partial + base * 2 * dim;
+      float f = 0.0f;
 #pragma unroll 8
-    for (int k = strip; k < blocks; k += 32) f += __ldcg(partial + int64_t(k) * 2 * dim + c);
+      for (int k = strip; k < count; k += 32) f += __ldcg(from + int64_t(k) * 2 * dim + c);
+      sum.add(f);
+    }
   }
-  part[strip][lane] = f;
+  part[strip][lane] = sum.total();
   __syncthreads();
   if (strip == 0 && c < 2 * dim) {
-    f = 0.0f;
+    float f = 0.0f;
 #pragma unroll
     for (int k = 0; k < 32; ++k) f += part[k][lane];
     if (c < dim) {
@@ -953,6 +959,18 @@ int norm_blocks(int64_t rows, const NormShape &s, int sms) {
   const int64_t per_block = int64_t(s.threads / s.lanes) * s.unroll;
   const int64_t need = (rows + per_block - 1) / per_block;
   return int(std::max<int64_t>(1, std::min<int64_t>(need, int64_t(sms) * (1024 / s.threads))));
+}
+
+// Rows of one launch of the backward with column sums: a thread of the fewest
+// blocks (one per multiprocessor) adds 512 rows, so that its fp32 chain is short;
+// more rows take more launches, whose sums lie side by side in the workspace.
+int64_t norm_chunk(const NormShape &s, int sms) { return int64_t(sms) * (s.threads / s.lanes) * 512; }
+
+// Most blocks' sums that a call leaves.
+int64_t norm_partials(int64_t rows, const NormShape &s, int sms) {
+  if (s.longer) return std::min<int64_t>(rows, kNormLongSplits);
+  const int64_t chunk = norm_chunk(s, sms), whole = rows / chunk, rest = rows - whole * chunk;
+  return whole * norm_blocks(chunk, s, sms) + (rest > 0 ? norm_blocks(rest, s, sms) : 0);
 }
 
 // The ring of a block takes at most 48 KB per array (two blocks of the backward,
@@ -1093,12 +1111,11 @@ extern "C" int se_layer_norm_backward_workspace(size_t rows, int64_t dim, int32_
     if (bytes == nullptr) throw std::invalid_argument("bytes is null");
     // Enough for every type and alignment of the same rows and dim.
     const int sms = sm_count(device);
-    int blocks = 1;
+    int64_t blocks = 1;
     for (const size_t vb : {size_t(2), size_t(4)}) {
       for (const bool aligned : {false, true}) {
         const NormShape s = norm_shape(dim, vb, aligned, false, true);
-        blocks = std::max(blocks, s.longer ? int(std::min<size_t>(rows, kNormLongSplits))
-                                           : norm_blocks(int64_t(rows), s, sms));
+        blocks = std::max(blocks, norm_partials(int64_t(rows), s, sms));
       }
     }
     *bytes = size_t(blocks) * 2 * size_t(dim) * sizeof(float);
@@ -1121,7 +1138,7 @@ extern "C" int se_layer_norm_backward(int32_t value_dtype, int32_t param_dtype, 
     const int sms = sm_count(device);
     uint32_t *status = WaitWords::get().of(device, st);
     const bool sums = dweight != nullptr || dbias != nullptr;
-    int blocks = 0;
+    int64_t blocks = 0;
     float *partial = nullptr;
     if (rows > 0) {
       check_device_ptr(grad, device, "grad");
@@ -1133,7 +1150,7 @@ extern "C" int se_layer_norm_backward(int32_t value_dtype, int32_t param_dtype, 
       const NormShape s = norm_shape(dim, vb, aligned16(x) && aligned16(grad) && aligned16(dx) &&
                                                   (rows == 1 || (x_stride * vb % 16 == 0 && grad_stride * vb % 16 == 0)),
                                      rows > 1 && (x_stride != dim || grad_stride != dim), true);
-      blocks = s.longer ? int(std::min<size_t>(rows, kNormLongSplits)) : norm_blocks(int64_t(rows), s, sms);
+      blocks = norm_partials(int64_t(rows), s, sms);
       if (sums) {
         check_device_ptr(workspace, device, "workspace");
         if (reinterpret_cast<uintptr_t>(workspace) % 4 != 0 ||
@@ -1164,12 +1181,19 @@ extern "C" int se_layer_norm_backward(int32_t value_dtype, int32_t param_dtype, 
                                          decltype(wide)::value, decltype(gather)::value, decltype(ring)::value,
                                          decltype(lanes)::value>;
           const size_t cols = s.wide || !sums ? 0 : size_t(s.threads / 32) * size_t(dim) * sizeof(float);
-          const NormLaunch l = norm_launch(kernel, s, int64_t(rows), dim, vb, 2, device, cols);
-          blocks = l.blocks;
-          kernel<<<blocks, s.threads, l.smem, st>>>(gp, grad_stride, xp, x_stride, int64_t(rows), int(dim), mean, rstd,
-                                                    weight, param_dtype, dxp, partial, s.lanes, l.stages, wait_limit().load(), status);
+          const int64_t all = int64_t(rows), chunk = sums ? norm_chunk(s, sms) : all;
+          blocks = 0;
+          for (int64_t row = 0; row < all; row += chunk) {
+            const int64_t count = std::min(chunk, all - row);
+            const NormLaunch l = norm_launch(kernel, s, count, dim, vb, 2, device, cols);
+            kernel<<<l.blocks, s.threads, l.smem, st>>>(gp + row * grad_stride, grad_stride, xp + row * x_stride, x_stride, count,
+                                                        int(dim), mean + row, rstd + row, weight, param_dtype, dxp + row * dim,
+                                                        sums ? partial + blocks * 2 * dim : nullptr, s.lanes, l.stages,
+                                                        wait_limit().load(), status);
+            launched("k_norm_backward");
+            blocks += l.blocks;
+          }
         });
-        launched("k_norm_backward");
       });
     }
     if (sums) {

@@ -50,7 +50,10 @@ RING = [(200_000, 128, torch.float32, 0, 0), (262_144, 256, torch.bfloat16, 0, 0
         (60_000, 301, torch.float32, 0, 1), (120_000, 301, torch.bfloat16, 2, 3), (60_000, 517, torch.float32, 0, 0),
         (60_000, 1001, torch.bfloat16, 0, 1), (60_000, 1037, torch.float32, 3, 1), (90_000, 1037, torch.bfloat16, 0, 0),
         (60_000, 1032, torch.float32, 0, 0), (65_536, 2048, torch.bfloat16, 0, 0), (33_000, 4096, torch.bfloat16, 0, 0),
-        (33_000, 4096, torch.float32, 0, 0), (33_000, 4104, torch.float16, 8, 0), (20_000, 8192, torch.bfloat16, 0, 0)]
+        (33_000, 4096, torch.float32, 0, 0), (33_000, 4104, torch.float16, 8, 0), (20_000, 8192, torch.bfloat16, 0, 0),
+        # more rows than one launch takes
+        (1_300_000, 128, torch.float32, 0, 0), (700_000, 301, torch.bfloat16, 2, 3), (3_000_000, 33, torch.bfloat16, 0, 1),
+        (160_000, 1037, torch.bfloat16, 0, 0), (160_000, 1032, torch.bfloat16, 8, 0)]
 
 
 def laid_out(values, pad, offset, dt):
@@ -89,8 +92,9 @@ def test_many_tiles_a_block(rows, dim, dt, pad, offset):
         assert torch.equal(se.layer_norm(x, w), y)
 
 
-# Equal values whose rounding in a long chain of adds goes one way: c lies 0.49 of a step of [256, 512) above its grid.
-BIASED = (3277 + 0.49) * 2.0**-15
+# Equal values whose rounding in a long chain of adds goes one way: c lies 0.49 of a step of [256, 512) above the grids of
+# [256, 512), [512, 1024) and [1024, 2048).
+BIASED = (3276 + 0.49) * 2.0**-15
 
 
 @pytest.mark.parametrize("dim", [1 << 22, (1 << 23) + 5])
@@ -115,3 +119,15 @@ def test_columns_of_many_long_rows():
     dw = se.layer_norm_backward(x, x, torch.zeros_like(r), r, torch.ones(dim, device="cuda"))[1]
     want = rows * float(r[0].double())
     assert float((dw.double() - want).abs().max()) <= (64 + 64 + 2 + 64) * U * want
+
+
+def test_columns_of_very_many_rows():
+    """A thread adds 512 rows at most, then come 5 levels of a warp, 8 warps, and the launches' blocks in pieces of 64
+    by 32 threads: 512 + 5 + 8 + 64 + 64 + 32 roundings at most. (One chain of all rows of a block, 6,700 here, is
+    1,200 u off and more.)"""
+    rows, dim = 6_000_000, 1032
+    x = torch.ones(rows, dim, dtype=torch.bfloat16, device="cuda")
+    r = torch.full((rows,), BIASED, device="cuda")
+    dw = se.layer_norm_backward(x, x, torch.zeros_like(r), r, torch.ones(dim, device="cuda"))[1]
+    want = rows * float(r[0].double())
+    assert float((dw.double() - want).abs().max()) <= (512 + 5 + 8 + 64 + 64 + 32) * U * want
