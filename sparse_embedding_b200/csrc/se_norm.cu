@@ -217,7 +217,11 @@ struct RowSum {
   int lanes;
   float (*buf)[32][4];  // [2][32][4]
   int phase = 0;
-  __device__ __forceinline__ void operator()(float (&v)[N]) {
+  __device__ __forceinline__ void operator()(float (&v)[N]) { vote<false>(v, false); }
+  // WIDE: the exchange's barrier also tells whether any thread's flag is set.
+  template <bool VOTE = true>
+  __device__ __forceinline__ bool vote(float (&v)[N], bool flag) {
+    bool any = false;
     const int lane = int(threadIdx.x) & 31, part = lanes < 32 ? lanes : 32;
     constexpr unsigned kAll = 0xffffffffu;
     if (N == 1 || part < N) {
@@ -257,7 +261,8 @@ struct RowSum {
 #pragma unroll
         for (int i = 0; i < N; ++i) buf[phase][warp][i] = v[i];
       }
-      __syncthreads();
+      if constexpr (VOTE) any = __syncthreads_or(flag) != 0;
+      else __syncthreads();
       const bool whole = (warps & (warps - 1)) == 0;  // a power of two: every lane's steps see all warps
       const int from = whole ? lane & (warps - 1) : lane;
 #pragma unroll
@@ -275,6 +280,7 @@ struct RowSum {
       }
       phase ^= 1;
     }
+    return any;
   }
 };
 
@@ -382,7 +388,8 @@ struct RowRing {
   }
   __device__ __forceinline__ bool ready() const { return wait_or_give_up<N == 1>(&bars[at], parity, given_up, limit); }
   // The tile has been read by all threads: refill its buffer. Each thread has
-  // passed fence_proxy_async_smem after its reads and then the block's barrier. The
+  // passed fence_proxy_async_smem after its reads and then a barrier of the block
+  // (that of its row's sum, where the block has one row at a time). The
   // barrier alone does not hold a copy back: a read that waits in the memory
   // pipe, behind stores that HBM holds up, comes after the copy (a warp's part of
   // one row in about 400,000 was a later row's, 32,768 x 4,096 bf16 backward).
@@ -456,7 +463,7 @@ k_norm_forward(const typename V::T *__restrict__ x, int64_t x_stride, int64_t ro
         else raw[u][v] = P::load(x + row * x_stride + c, lanes, n);
       }
     }
-    if constexpr (RING) {
+    if constexpr (RING && !WIDE) {
       fence_proxy_async_smem();
       if (__syncthreads_or(!ok)) {
         ring.drain(base, status);
@@ -477,7 +484,16 @@ k_norm_forward(const typename V::T *__restrict__ x, int64_t x_stride, int64_t ro
       }
       m[u] = vsum(t);
     }
-    sum(m);
+    if constexpr (WIDE) {
+      fence_proxy_async_smem();
+      if (sum.vote(m, !ok)) {
+        ring.drain(base, status);
+        return;
+      }
+      ring.next(base);
+    } else {
+      sum(m);
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       m[u] *= inv;
@@ -605,8 +621,9 @@ k_norm_forward_long(const typename V::T *__restrict__ x, int64_t x_stride, int64
 // [gridDim.x][2][dim] fp32, this block's sums of g h and of g per column
 // (null: no weight gradients wanted). Bound by HBM at vectors in a part of a
 // warp (212,992 x 128 fp32 58 us, 5.7 TB/s), by a block barrier a row at 16
-// warps an SM where a block takes one (32,768 x 4,096 bf16 155 us, 5.2; the
-// sums' registers allow no more), by instructions at single values (65,536 x 517
+// warps an SM where a block takes one (32,768 x 4,096 bf16 152 us with the column
+// kernel, 5.3; with a barrier of its own for the refill 174; the sums' registers
+// allow no more), by instructions at single values (65,536 x 517
 // fp32 83 us, 4.9; 9,973 x 1,037 bf16 28 us, 2.2).
 template <class V, int VEC, int NV, int U, bool WIDE, bool GATHER, bool RING, int LANES>
 __global__ void __launch_bounds__(WIDE ? kNormWideThreads : kNormNarrowThreads,
@@ -682,7 +699,7 @@ k_norm_backward(const typename V::T *__restrict__ grad, int64_t g_stride, const 
         }
       }
     }
-    if constexpr (RING) {
+    if constexpr (RING && !WIDE) {
       fence_proxy_async_smem();
       if (__syncthreads_or(!ok)) {
         ring.drain(base, status);
@@ -726,7 +743,12 @@ k_norm_backward(const typename V::T *__restrict__ grad, int64_t g_stride, const 
         both[2 * u] = s0[u];
         both[2 * u + 1] = s1[u];
       }
-      sum(both);
+      fence_proxy_async_smem();
+      if (sum.vote(both, !ok)) {
+        ring.drain(base, status);
+        return;
+      }
+      ring.next(base);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         s0[u] = both[2 * u];
