@@ -347,7 +347,9 @@ int se_muon_step(int32_t weight_dtype, int32_t grad_dtype, void *weight, int64_t
                  int64_t m, int64_t n, double lr, double beta, double weight_decay, double scale,
                  int32_t nesterov, int32_t steps, float eps, void *workspace, size_t workspace_bytes,
                  int32_t device, void *stream);
-/* Bytes of workspace for either call; out_dtype is the result's, or the weight's. */
+/* Bytes of workspace for either call; out_dtype is the result's, or the weight's.
+ * Matrices of up to 128 x 256 (or 256 x 128) are worked on chip: they use none
+ * (null is taken), and what is asked for does not grow with their batch. */
 int se_muon_workspace(int32_t out_dtype, size_t batch, int64_t m, int64_t n, size_t *bytes);
 
 /*

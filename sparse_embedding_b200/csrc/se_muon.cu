@@ -1128,6 +1128,7 @@ k_muon_weights(const __half *__restrict__ hi, const __half *__restrict__ lo, int
 
 constexpr int kSmallSide = 128, kSmallWide = 256;  // the largest s and w of the kernel below
 constexpr int kSmallTile = 128 * 128;              // bytes: 128 rows of 64 values
+constexpr bool on_chip(int64_t s, int64_t w) { return s <= kSmallSide && w <= kSmallWide; }
 
 // Place (in values) of (r, c) in a matrix of 64-column tiles of 128 rows with
 // 128-byte swizzle: what the matrix instructions read, K-major as rows of
@@ -1694,27 +1695,14 @@ void orthogonalise(UpdateArgs u, int grad_type, int64_t batch, int steps, float 
            (aligned16(u.momentum.p) && u.momentum.row % 4 == 0 && (batch == 1 || u.momentum.batch % 4 == 0)));
   const bool transposed = u.m > u.n;
   const int64_t s = std::min(u.m, u.n), w = std::max(u.m, u.n);
-  const Plan plan = plan_for(batch, s, w, split);
-  const Space sp = muon_space(workspace, batch, s, w, split);
-  if (workspace_bytes < sp.bytes) throw std::invalid_argument("workspace is smaller than se_muon_workspace asks for");
-  const int tm = 128 * plan.cg;
-  auto cut = [&](bool symmetric, int64_t cols, int64_t depth, int parts) {
-    const int64_t tiles = tile_count(symmetric, s, cols, tm, plan.bn);
-    if (tiles * parts * batch > 0x7fffffff) throw std::invalid_argument("batch x m x n is too large");
-    return Cut{int(s), int(cols), int((depth + kTileK - 1) / kTileK), int((cols + plan.bn - 1) / plan.bn), int(tiles), parts};
-  };
   NsArgs g{};
-  g.gram = cut(true, s, w, plan.parts);
-  g.square = cut(true, s, s, 1);
-  g.apply = cut(false, w, s, 1);
-  const int sms = sm_count(device);
   g.status = WaitWords::get().of(device, st);
   g.limit = wait_limit();
   fin.transposed = transposed;
   const size_t ob = value_bytes(fin.type);
   fin.vec = u.n % 4 == 0 && reinterpret_cast<uintptr_t>(fin.out) % (4 * ob) == 0 && fin.row % 4 == 0 &&
             (batch == 1 || fin.batch % 4 == 0);
-  if (s <= kSmallSide && w <= kSmallWide) {
+  if (on_chip(s, w)) {
     const int xtiles = int((w + 63) / 64), stiles = int((s + 63) / 64);
     const size_t smem = size_t(2 * xtiles + (split ? 2 : 1) * stiles) * kSmallTile + 1024;
     const uint32_t columns = (w > 128 ? 256 : 128) * (split ? 2 : 1);
@@ -1737,6 +1725,21 @@ void orthogonalise(UpdateArgs u, int grad_type, int64_t batch, int steps, float 
     launched("k_newton_schulz_small");
     return;
   }
+  check_device_ptr(workspace, device, "workspace");
+  if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0) throw std::invalid_argument("workspace must be 256-byte aligned");
+  const Plan plan = plan_for(batch, s, w, split);
+  const Space sp = muon_space(workspace, batch, s, w, split);
+  if (workspace_bytes < sp.bytes) throw std::invalid_argument("workspace is smaller than se_muon_workspace asks for");
+  const int tm = 128 * plan.cg;
+  auto cut = [&](bool symmetric, int64_t cols, int64_t depth, int parts) {
+    const int64_t tiles = tile_count(symmetric, s, cols, tm, plan.bn);
+    if (tiles * parts * batch > 0x7fffffff) throw std::invalid_argument("batch x m x n is too large");
+    return Cut{int(s), int(cols), int((depth + kTileK - 1) / kTileK), int((cols + plan.bn - 1) / plan.bn), int(tiles), parts};
+  };
+  g.gram = cut(true, s, w, plan.parts);
+  g.square = cut(true, s, s, 1);
+  g.apply = cut(false, w, s, 1);
+  const int sms = sm_count(device);
   const bool dense = u.grad.row == u.n && (u.momentum.p == nullptr || u.momentum.row == u.n);
   const int64_t spans = dense ? (u.m * u.n + kSpan - 1) / kSpan : u.m * ((u.n + kSpan - 1) / kSpan);
   const int nparts = int(std::min<int64_t>(std::min<int64_t>(kNormParts, spans), std::max<int64_t>(1, 4 * sms / batch)));
@@ -1829,6 +1832,9 @@ extern "C" int se_muon_workspace(int32_t out_dtype, size_t batch, int64_t m, int
     const ResultType out = result_type(out_dtype, "out_dtype");
     check_matrices(batch, m, n, 1, 0.0f);
     if (bytes == nullptr) throw std::invalid_argument("bytes is null");
+    // Matrices on chip use none: the answer is one matrix's, whatever the batch,
+    // so that it still tells calls with something to do from empty ones.
+    if (on_chip(std::min(m, n), std::max(m, n))) batch = std::min<size_t>(batch, 1);
     *bytes = batch == 0 || m == 0 || n == 0
                  ? 0
                  : muon_space(nullptr, int64_t(batch), std::min(m, n), std::max(m, n), out.split).bytes;
@@ -1846,8 +1852,6 @@ extern "C" int se_orthogonalize(int32_t dtype, const void *update, size_t batch,
     DeviceGuard dg(device);
     check_device_ptr(update, device, "update");
     check_device_ptr(out, device, "out");
-    check_device_ptr(workspace, device, "workspace");
-    if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0) throw std::invalid_argument("workspace must be 256-byte aligned");
     UpdateArgs u{};
     u.grad = {update, batch_stride, row_stride};
     u.m = m;
@@ -1885,8 +1889,6 @@ extern "C" int se_muon_step(int32_t weight_dtype, int32_t grad_dtype, void *weig
     check_device_ptr(weight, device, "weight");
     check_device_ptr(grad, device, "grad");
     check_device_ptr(momentum, device, "momentum");
-    check_device_ptr(workspace, device, "workspace");
-    if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0) throw std::invalid_argument("workspace must be 256-byte aligned");
     UpdateArgs u{};
     u.grad = {grad, grad_batch_stride, grad_row_stride};
     u.momentum = {momentum, momentum_batch_stride, momentum_row_stride};

@@ -101,3 +101,21 @@ def test_optimizer_takes_full_products():
     torch_ops.Muon([p[0]], lr=0.1, precise=True).step()
     old.step()
     assert torch.equal(p[0], want) and not torch.equal(p[1], want)
+
+
+def test_matrices_on_chip_need_no_workspace():
+    from sparse_embedding_b200 import _native as N
+
+    u = matrix(50, 40, 96).float()
+    out, st = torch.empty_like(u), torch.cuda.current_stream().cuda_stream
+    N.check(N.lib().se_orthogonalize(0, u.data_ptr(), 50, 40, 96, 40 * 96, 96, 5, 1e-7, out.data_ptr(), None, 0, 0, st))
+    assert torch.equal(out, se.orthogonalize(u))
+    big = matrix(130, 300).float()
+    rc = N.lib().se_orthogonalize(0, big.data_ptr(), 1, 130, 300, 39000, 300, 5, 1e-7, big.data_ptr(), None, 0, 0, st)
+    assert rc == N.SE_ERR_INVALID_ARGUMENT and b"workspace is null" in N.lib().se_last_error()
+    # 20,000 small matrices: 80 MB of them, and no more than their result beside them
+    many = torch.ones(20000, 32, 32, device="cuda")
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    se.orthogonalize(many)
+    assert torch.cuda.max_memory_allocated() - before < many.numel() * 4 + (1 << 20)

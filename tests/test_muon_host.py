@@ -100,3 +100,15 @@ def test_full_products_flag():
     assert size[1].value < size[2].value == size[0].value == size[3].value
     assert orth(dtype=3 | full) == orth(dtype=2 | full << 1) == N.SE_ERR_INVALID_ARGUMENT
     assert b"unsupported dtype" in N.lib().se_last_error()
+
+
+def test_matrices_on_chip_ask_for_no_more_in_a_batch():
+    def ask(code, batch, m, n):
+        size = C.c_size_t()
+        N.check(N.lib().se_muon_workspace(code, batch, m, n, C.byref(size)))
+        return size.value
+
+    for code in (0, 1, 2, 2 | dense._FULL_PRODUCTS):
+        for m, n in ((128, 256), (256, 128), (16, 16), (1, 1)):
+            assert 0 < ask(code, 65535, m, n) == ask(code, 1, m, n) < 1 << 20
+        assert ask(code, 3, 129, 256) > 2 * ask(code, 1, 129, 256)
