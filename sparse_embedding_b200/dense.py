@@ -227,6 +227,14 @@ def _matrices(x, what: str):
     return batch, m, n, (bs if batch > 1 else m * rs), rs
 
 
+def _check_sizes(batch: int, m: int, n: int) -> None:
+    """The C ABI's limits, before there is a call."""
+    if m > 1 << 20 or n > 1 << 20:
+        raise ValueError("m and n must be in [0, 2^20]")
+    if batch > 65535:
+        raise ValueError("batch must be at most 65535")
+
+
 _FULL_PRODUCTS = 0x100  # SE_FULL_PRODUCTS
 
 

@@ -66,8 +66,11 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
 class Muon(torch.optim.Optimizer):
     """Muon for the dense matrices of a model, next to the store's own row
     optimizers: each parameter [..., m, n] takes dense.muon_step with a float32
-    momentum (leading axes are separate matrices: stacked layers or experts).
-    Vectors (biases, normalisation weights) need another optimizer. `precise`:
+    momentum (leading axes are separate matrices: stacked layers or experts; a
+    convolution's [out, in, 3, 3] is out x in matrices of 3 x 3). Vectors (biases,
+    normalisation weights) need another optimizer; they, parameters without
+    contiguous rows (transposed ones) and batches of more than 65,535 matrices
+    are refused when they are added. `precise`:
     full products for bfloat16 parameters too (dense.orthogonalize)."""
 
     def __init__(self, params, lr: float = 0.02, momentum: float = 0.95, weight_decay: float = 0.0,
@@ -82,9 +85,14 @@ class Muon(torch.optim.Optimizer):
 
     def add_param_group(self, param_group) -> None:
         super().add_param_group(param_group)
-        for p in self.param_groups[-1]["params"]:
-            if p.dim() < 2:
-                raise ValueError("Muon steps matrices: every parameter needs at least two dimensions")
+        try:
+            for p in self.param_groups[-1]["params"]:
+                if p.dim() < 2:
+                    raise ValueError("Muon steps matrices: every parameter needs at least two dimensions")
+                dense._check_sizes(*dense._matrices(p, "every parameter")[:3])
+        except ValueError:  # the group is not taken, and the optimizer goes on with those that it had
+            self.param_groups.pop()
+            raise
 
     def load_state_dict(self, state_dict) -> None:
         super().load_state_dict(state_dict)
@@ -102,12 +110,12 @@ class Muon(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        if any(p.grad is not None and p.grad.is_sparse for group in self.param_groups for p in group["params"]):
+            raise ValueError("Muon needs dense gradients")  # before any parameter is stepped
         for group in self.param_groups:
             for p in group["params"]:
                 if p.grad is None:
                     continue
-                if p.grad.is_sparse:
-                    raise ValueError("Muon needs dense gradients")
                 state = self.state[p]
                 if "momentum_buffer" not in state:
                     state["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)

@@ -112,3 +112,26 @@ def test_matrices_on_chip_ask_for_no_more_in_a_batch():
         for m, n in ((128, 256), (256, 128), (16, 16), (1, 1)):
             assert 0 < ask(code, 65535, m, n) == ask(code, 1, m, n) < 1 << 20
         assert ask(code, 3, 129, 256) > 2 * ask(code, 1, 129, 256)
+
+
+def test_optimizer_refuses_a_group_whole():
+    param = lambda t: torch.nn.Parameter(t)  # noqa: E731
+    opt = torch_ops.Muon([param(torch.zeros(4, 4))])
+    base = torch.zeros(70000, 1, 1)
+    for bad, msg in ((torch.zeros(4), "at least two dimensions"), (torch.zeros(8, 4).t(), "every parameter must be matrices"),
+                     (base, "batch must be at most 65535"), (torch.zeros(1).expand(1, (1 << 20) + 1), "must be")):
+        with pytest.raises(ValueError, match=msg):
+            opt.add_param_group({"params": [param(torch.zeros(3, 5)), param(bad)]})
+        assert len(opt.param_groups) == 1 and len(opt.param_groups[0]["params"]) == 1
+        opt.step()  # nothing of the refused group is left
+    opt.add_param_group({"params": [param(torch.zeros(2, 3, 5)), param(torch.zeros(6, 9)[:, 2:7])], "lr": 0.5})
+    assert opt.param_groups[1]["lr"] == 0.5 and opt.param_groups[1]["precise"] is False
+
+
+def test_sparse_gradients_are_refused_before_any_step():
+    first, second = torch.nn.Parameter(torch.zeros(4, 4)), torch.nn.Parameter(torch.zeros(4, 4))
+    opt = torch_ops.Muon([first, second])
+    first.grad, second.grad = torch.ones(4, 4), torch.ones(4, 4).to_sparse()
+    with pytest.raises(ValueError, match="dense gradients"):  # not the first parameter's refusal (a host tensor)
+        opt.step()
+    assert not opt.state
