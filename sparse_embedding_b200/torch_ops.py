@@ -70,7 +70,9 @@ class Muon(torch.optim.Optimizer):
     convolution's [out, in, 3, 3] is out x in matrices of 3 x 3). Vectors (biases,
     normalisation weights) need another optimizer; they, parameters without
     contiguous rows (transposed ones) and batches of more than 65,535 matrices
-    are refused when they are added. `precise`:
+    are refused when they are added. A captured step keeps the lr and the other
+    values of its capture; the first step, which makes the momentum, is not
+    captured (RuntimeError). `precise`:
     full products for bfloat16 parameters too (dense.orthogonalize)."""
 
     def __init__(self, params, lr: float = 0.02, momentum: float = 0.95, weight_decay: float = 0.0,
@@ -118,6 +120,9 @@ class Muon(torch.optim.Optimizer):
                     continue
                 state = self.state[p]
                 if "momentum_buffer" not in state:
+                    if p.is_cuda and torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError("Muon's first step cannot be captured: a replayed graph would zero the "
+                                           "momentum every time; step once before the capture")
                     state["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
                 dense.muon_step(p, p.grad.contiguous(), state["momentum_buffer"], lr=group["lr"],
                                 beta=group["momentum"], weight_decay=group["weight_decay"],

@@ -84,3 +84,28 @@ def test_a_small_tower_of_16_bit_matrices(dt):
     ((Y @ W.t()) * c.double()).sum().backward()
     for got, want in ((x, X), (w, W), (s, S)):
         assert float((got.grad.double() - want.grad).norm() / want.grad.norm()) < 16 * torch.finfo(dt).eps / 2
+
+
+def test_captured_optimizer_steps():
+    """Replays go on with the momentum; a first step, whose zeros a graph would replay, is refused."""
+    params = [torch.nn.Parameter(rand(96, 64, seed=k)) for k in range(2)]
+    twins = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    grads = [rand(96, 64, seed=k + 5) for k in range(2)]
+    opt, twin = torch_ops.Muon(params, lr=0.1), torch_ops.Muon(twins, lr=0.1)
+    for p, q, g in zip(params, twins, grads):
+        p.grad, q.grad = g.clone(), g.clone()
+    with pytest.raises(RuntimeError, match="step once before the capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    assert not opt.state[params[0]] and all(torch.equal(p, q) for p, q in zip(params, twins))
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for _ in range(3):
+        graph.replay()
+    for _ in range(4):
+        twin.step()
+    torch.cuda.synchronize()
+    for p, q in zip(params, twins):
+        assert torch.equal(p, q) and torch.equal(opt.state[p]["momentum_buffer"], twin.state[q]["momentum_buffer"])
