@@ -699,7 +699,7 @@ k_norm_backward(const typename V::T *__restrict__ grad, int64_t g_stride, const 
         }
       }
     }
-    if constexpr (RING && !WIDE) {
+    if constexpr (RING && !WIDE && GATHER) {
       fence_proxy_async_smem();
       if (__syncthreads_or(!ok)) {
         ring.drain(base, status);
@@ -757,6 +757,17 @@ k_norm_backward(const typename V::T *__restrict__ grad, int64_t g_stride, const 
     } else {
       sum(s0);
       sum(s1);
+      // Vectors wait for their reads here, where the sums did already (100,000 x 512
+      // bf16 100 us before the sums, 72 behind them); single values before the sums,
+      // whose registers their refill would wait for (60,000 x 1,001 bf16 81 and 91 us).
+      if constexpr (RING && !GATHER) {
+        fence_proxy_async_smem();
+        if (__syncthreads_or(!ok)) {
+          ring.drain(base, status);
+          return;
+        }
+        ring.next(base);
+      }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
