@@ -949,10 +949,11 @@ __device__ __forceinline__ bool grid_wait(uint32_t *barrier, uint32_t target, Sh
 // over the grid after each (about 2,500 clocks). One launch per product took 81
 // us of host time and 10 us each at 1000 x 517; now a call takes 20 us of it.
 // What bounds it: large sides the tensor cores at the power limit (4096 x 4096
-// bf16 1,150 us, 1.2 PFLOP/s of the 1.37e12 counted operations; of each product
-// 70 of 85 thousand clocks are instructions, the rest its last epilogue and the
+// bf16 1,310 to 1,390 us in calls one after another, 1.0 PFLOP/s of the 1.37e12
+// counted operations, 1,170 on a card that rested; of each product 70 of 85
+// thousand clocks are instructions, the rest its last epilogue and the
 // barrier); 1,000 the chain of a product's stages, epilogue and barrier, 12 to
-// 20 thousand clocks, mostly latency (1000 x 517 fp32 160 us).
+// 20 thousand clocks, mostly latency (1000 x 517 fp32 151 us).
 template <int CG, int BN, class OUT>
 __global__ void __launch_bounds__(kThreads, 1) k_newton_schulz(const __grid_constant__ NsArgs g) {
   using L = Layout<CG, BN, !std::is_same_v<OUT, BF16>>;
@@ -1154,8 +1155,8 @@ __device__ __forceinline__ void open_eight(const uint4 &v, float (&f)[8]) {
 // memory, in the layout of the matrix instructions (X serves as a K-major
 // operand of X X^T and, the same bytes, as the MN-major one of B X). Between two products there is only a
 // barrier of the CTA, where the kernel for large matrices passes through L2
-// and a barrier of the grid (128 x 64 bf16: 64 us there with its launches, 23 us
-// here; 128 x 256 42 us, 64 matrices of 64 x 64 19 us).
+// and a barrier of the grid (128 x 64 bf16: 64 us there with its launches, 24 us
+// here; 128 x 256 43 us, 64 matrices of 64 x 64 19 us).
 // Bound by the instructions of one SM and the latency of 3 products a step;
 // with X and A in shared memory as f16 pairs, unpacked and packed again in
 // every epilogue, it took 33 us at 128 x 64 and 70 at 128 x 256.

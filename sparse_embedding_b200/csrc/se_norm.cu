@@ -412,9 +412,9 @@ struct RowRing {
 // Rows held in registers: `lanes` threads per row (a power of two up to 32, or
 // with WIDE the block), NV vectors of VEC values per thread, U rows at a time
 // (their loads are in flight together). Vectors are bound by HBM and, in short
-// 16-bit rows, by instructions between load and store (212,992 x 128 fp32 40 us,
-// 5.4 TB/s; 262,144 x 256 bf16 49 us, 5.5; 32,768 x 4,096 bf16 92 us, 5.9);
-// single values by their loads, stores and tests (65,536 x 517 fp32 45 us, 6.0;
+// 16-bit rows, by instructions between load and store (212,992 x 128 fp32 41 us,
+// 5.3 TB/s; 262,144 x 256 bf16 49 us, 5.5; 32,768 x 4,096 bf16 89 us, 6.0);
+// single values by their loads, stores and tests (65,536 x 517 fp32 46 us, 5.9;
 // 2^25 bf16 values in rows of 33 58 us, 2.3).
 template <class V, int VEC, int NV, int U, bool WIDE, bool GATHER, bool RING, int LANES>
 __global__ void __launch_bounds__(WIDE ? kNormWideThreads : kNormNarrowThreads,
@@ -620,11 +620,11 @@ k_norm_forward_long(const typename V::T *__restrict__ x, int64_t x_stride, int64
 // Backward of rows held in registers (layout as k_norm_forward). partial:
 // [gridDim.x][2][dim] fp32, this block's sums of g h and of g per column
 // (null: no weight gradients wanted). Bound by HBM at vectors in a part of a
-// warp (212,992 x 128 fp32 58 us, 5.7 TB/s), by a block barrier a row at 16
-// warps an SM where a block takes one (32,768 x 4,096 bf16 152 us with the column
-// kernel, 5.3; with a barrier of its own for the refill 174; the sums' registers
+// warp (with the column kernel 212,992 x 128 fp32 56 us, 5.9 TB/s), by a block
+// barrier a row at 16 warps an SM where a block takes one (32,768 x 4,096 bf16
+// 147 us, 5.5; with a barrier of its own for the refill 170; the sums' registers
 // allow no more), by instructions at single values (65,536 x 517
-// fp32 83 us, 4.9; 9,973 x 1,037 bf16 28 us, 2.2).
+// fp32 84 us, 4.8; 9,973 x 1,037 bf16 34 us, 28 without the column kernel, 2.2).
 template <class V, int VEC, int NV, int U, bool WIDE, bool GATHER, bool RING, int LANES>
 __global__ void __launch_bounds__(WIDE ? kNormWideThreads : kNormNarrowThreads,
                                   !WIDE && (GATHER ? VEC <= 16 : NV <= 2) ? 2 : 1)
