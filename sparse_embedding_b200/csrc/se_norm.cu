@@ -1030,7 +1030,8 @@ NormLaunch norm_launch(K *kernel, const NormShape &s, int64_t rows, int64_t dim,
 // values immediate offsets: rows of 65 fp32 values 69 -> 54 us forward, 116 -> 85
 // backward; and saves vectors the tests in the row sums: 262,144 x 256 bf16
 // forward 52 -> 49, 65,536 x 64 fp32 backward 15.1 -> 13.4; in place, 256 bf16
-// values with a gap of 8, backward 52 -> 44, forward 30 -> 33, so not there).
+// values with a gap of 8, backward 52 -> 44, forward 30 -> 33, so not there. 8
+// threads lose by it: 524,288 x 64 bf16 forward 28.1 -> 29.8, backward 38.8 -> 41.2).
 template <class V, bool BACKWARD, class F>
 void with_norm_shape(const NormShape &s, F &&f) {
   constexpr int kVec = int(16 / sizeof(typename V::T));
